@@ -42,7 +42,8 @@ def _e2m1(v):
 
 
 def _global_scale(x):
-    return (x.abs().amax().float() / 2688.0).clamp(min=2.0 ** -100)
+    top = x.abs().amax().float()
+    return (top / torch.full_like(top, 2688.0)).clamp(min=2.0 ** -100)  # by a number, torch multiplies with its reciprocal
 
 
 def _quantize(v, kind, g):
@@ -250,7 +251,7 @@ def exact(case, seed):
             v = v[:, cols:] * v[:, :cols] * torch.special.expit(v[:, :cols])
         g = one
         if kind == "nvfp4":
-            g = st["g"] if st["g"] is not None else (v.abs().max().float() / 2688.0).clamp(min=2.0 ** -100)
+            g = st["g"] if st["g"] is not None else (v.abs().max().float().double() / 2688).float().clamp(min=2.0 ** -100)
         return _exact_levels(v, kind, g)
     if op == "linear":
         codes, scales, gw = st["w"]
