@@ -25,6 +25,7 @@ BLUT_ERR_CUDA = -6
 FMT_R8, FMT_B, FMT_NESTED, FMT_DENSE = 1, 2, 3, 4
 LAYOUT_PAIRED, LAYOUT_TC = 1, 2
 F16, BF16, F32 = 0, 1, 2
+FP4_NV, FP4_MX = 1, 2
 
 
 class MatDesc(C.Structure):
@@ -60,6 +61,17 @@ EP_HANDLE_BYTES = 64
 class EpDesc(C.Structure):
     _fields_ = [("world", C.c_int32), ("rank", C.c_int32), ("capacity", C.c_int32), ("hidden", C.c_int32),
                 ("top_k", C.c_int32), ("dtype", C.c_int32), ("windows", C.c_void_p * EP_MAX_RANKS)]
+
+
+class FP4Desc(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("reserved", C.c_int32), ("rows", C.c_int64), ("cols", C.c_int64)]
+
+
+class FP4MMArgs(C.Structure):
+    _fields_ = [("w", FP4Desc), ("w_tiled", C.c_void_p), ("w_stride", C.c_int64), ("w_scale", C.c_void_p),
+                ("num_experts", C.c_int32), ("out_dtype", C.c_int32), ("offsets", C.c_void_p),
+                ("x_codes", C.c_void_p), ("x_scales", C.c_void_p), ("x_scale", C.c_void_p), ("x_rows", C.c_int64),
+                ("y", C.c_void_p), ("y_ld", C.c_int64)]
 
 
 # (name, restype, argtypes) of every exported entry point, in blut.h order.
@@ -101,6 +113,18 @@ SIGNATURES = [
     ("blut_ep_dispatch", C.c_int, [C.POINTER(EpDesc), _VP, _VP, _VP, _I32, _VP, _VP, _I32, _VP]),
     ("blut_ep_combine", C.c_int, [C.POINTER(EpDesc), _I32, _VP, _VP, _I32, _VP]),
     ("blut_ep_check_status", C.c_int, [C.POINTER(EpDesc), _VP]),
+    ("blut_fp4_codes_bytes", C.c_int64, [C.POINTER(FP4Desc)]),
+    ("blut_fp4_scales_bytes", C.c_int64, [C.POINTER(FP4Desc)]),
+    ("blut_fp4_tiled_bytes", C.c_int64, [C.POINTER(FP4Desc)]),
+    ("blut_fp4_global_scale", C.c_int, [_VP, _I32, _I64, _I64, _I64, _I32, _VP, _VP]),
+    ("blut_fp4_quantize", C.c_int, [C.POINTER(FP4Desc), _VP, _I32, _I64, _VP, _I64, _VP, _VP, _VP, _VP]),
+    ("blut_fp4_silu_mul_quantize", C.c_int, [C.POINTER(FP4Desc), _VP, _I32, _I64, _VP, _VP, _VP, _VP]),
+    ("blut_fp4_dequantize", C.c_int, [C.POINTER(FP4Desc), _VP, _VP, _VP, _VP, _I32, _I64, _VP]),
+    ("blut_fp4_import", C.c_int, [C.POINTER(FP4Desc), _VP, _VP, _VP, _VP, _VP]),
+    ("blut_fp4_export", C.c_int, [C.POINTER(FP4Desc), _VP, _VP, _VP, _VP, _VP]),
+    ("blut_fp4_pack_tiled", C.c_int, [C.POINTER(FP4Desc), _VP, _VP, _VP, _VP]),
+    ("blut_fp4_matmul", C.c_int, [C.POINTER(FP4MMArgs), _VP]),
+    ("blut_fp4_check_status", C.c_int, [_VP]),
 ]
 
 _lib = None

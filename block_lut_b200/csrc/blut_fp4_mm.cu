@@ -1,0 +1,511 @@
+// Products of 4-bit microscaled matrices on the block-scaled tensor cores
+// (blut_fp4_matmul): y[t] = W x_t for all rows of x, or for runs of rows with
+// one W per run.
+//
+//   y[t][n] = g_x g_w sum_k (q s)_w[n][k] (q s)_x[t][k],  float32 sums
+//
+// A CTA computes one tile of 128 weight rows x NT tokens over a K range
+// (D^T: weight rows are tensor-memory lanes, tokens are columns, so that a
+// few tokens cost a narrow MMA and not a padded one).  Per 128 columns:
+//
+//  * warp 0 (one lane) fetches the tile's unit - 8 KB of codes and the scales
+//    of 128 rows, contiguous - with one bulk copy, and the tokens' codes with
+//    four (a run of rows is contiguous per 32 columns);
+//  * warps 2, 3 bring the tokens' scales into the order that tcgen05.cp reads:
+//    they are the one operand whose position in a tile depends on where the
+//    run of rows starts;
+//  * warp 1 (one lane) copies both scales to tensor memory (tcgen05.cp,
+//    32x128b, replicated to the four lane quarters) and issues two
+//    tcgen05.mma of K = 64, kind::mxf4nvf4 (a scale per 16) or kind::mxf4 (a
+//    scale per 32), M = 128, N = the tile's tokens rounded to 16.
+//
+// Then all four warps read the accumulator, one lane quarter each.  Where
+// there are few tiles, a cluster of 2, 4 or 8 CTAs splits K: each leaves its
+// partial tile in its shared memory and sums a share of the tokens over the
+// cluster in rank order, so the result is the same in every run and no
+// workspace is needed.
+//
+// Every wait is bounded; one that runs out raises the CTA's abort flag and
+// the device status, and every role then leaves its loop, lets what it has in
+// flight land, and frees the tensor memory.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <atomic>
+
+#include "blut_fp4.cuh"
+#include "blut_mm.cuh"
+#include "blut_tc.cuh"
+
+namespace blut {
+namespace {
+
+__device__ int g_fp4_status;
+
+constexpr int kThreads = 128;
+constexpr int kHeader = 1024;  // barriers and flags before the ring
+constexpr int kPrefetch = 4;   // blocks of token scales held in registers
+
+template <bool kMX, int NT>
+struct Fp4Cfg {
+  static constexpr int kWords = kMX ? 1 : 2;           // scale words per 128 columns
+  static constexpr int kGroups = (NT + 127) / 128;     // 128-token groups of the scales
+  static constexpr int kA = kFp4UnitCodes + 512 * kWords;
+  static constexpr int kB = NT * 64;
+  static constexpr int kSB = 512 * kWords * kGroups;
+  static constexpr int kStage = kA + kB + kSB;
+  // Two CTAs per SM (three for few tokens) keep copies in flight while one of
+  // them starts or stores.
+  static constexpr int kCtas = NT <= 64 ? 3 : 2;
+  static constexpr int kStages = (kCtas == 3 ? 74 * 1024 : 111 * 1024) / kStage;
+  static constexpr int kSmem = kHeader + kStages * kStage;
+  // Tensor memory: NT accumulator columns, then slots of scales; a slot holds
+  // one block, 4 columns per word for the weights and for each token group.
+  static constexpr int kCols = NT <= 64 ? 128 : 256;
+  static constexpr int kWordCols = 4 + 4 * kGroups;
+  static constexpr int kSlotCols = kWords * kWordCols;
+  static constexpr int kSlots = (kCols - NT) / kSlotCols < kStages ? (kCols - NT) / kSlotCols : kStages;
+  static_assert(kStages >= 2 && kStages <= 8 && kSlots >= 2, "ring");
+};
+
+struct Fp4Params {
+  const uint8_t* w;
+  int64_t wstride;
+  const float* wg;
+  const int32_t* offsets;
+  int experts;
+  const uint8_t* xc;
+  const uint32_t* xs;
+  const float* xg;
+  int64_t x_rows;
+  int n;        // weight rows
+  int kblocks;  // 128-column blocks
+  int split;    // CTAs of a cluster along K
+  void* y;
+  int64_t ldy;
+  int out_dtype;
+  uint64_t wait_ns;
+};
+
+struct Fp4Header {
+  uint64_t wfull[8], sfull[8], empty[8], acc, fin;
+  uint32_t tmem;
+  int abort_flag;
+  int expert, row0, cnt;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+      : "=f"(v)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+// 32 rows x 16 bytes of shared memory to 4 columns of all four lane quarters.
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint32_t saddr) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(tc_desc(saddr, 512, 128))
+               : "memory");
+}
+
+template <bool kMX>
+__device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                        uint32_t acc) {
+  if constexpr (kMX) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::
+            "r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        : "memory");
+  }
+}
+
+// Instruction descriptor: A and B e2m1 K-major, M = 128, N = n, scales e4m3
+// or e8m0; mxfp4's scale word holds the scales of two MMAs, bytes 0-1 and 2-3.
+template <bool kMX>
+__device__ __forceinline__ uint32_t idesc_fp4(int n, int step) {
+  const uint32_t id = kMX ? 2u * step : 0u;
+  return (id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((kMX ? 1u : 0u) << 23) | (1u << 27) |
+         (id << 29);
+}
+
+// Which run tile `tile` of the token tiles belongs to (one warp): runs are
+// cut into ceil(rows / NT) tiles, in order.  Offsets are clamped to
+// [0, x_rows], so no offset leads out of the buffers.
+template <int NT>
+__device__ void find_tile(const Fp4Params& p, int tile, int lane, Fp4Header* h) {
+  int before = 0;
+  for (int e0 = 0; e0 < p.experts; e0 += 128) {  // four runs per lane
+    int o[5], tiles = 0;
+#pragma unroll
+    for (int j = 0; j < 5; ++j) {
+      const int e = min(e0 + 4 * lane + j, p.experts);
+      o[j] = (int)min((int64_t)max(p.offsets[e], 0), p.x_rows);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tiles += (max(o[j + 1] - o[j], 0) + NT - 1) / NT;
+    int incl = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    int t = tile - before - (incl - tiles);  // tile index within this lane's runs
+    if (t >= 0 && t < tiles) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int cnt = max(o[j + 1] - o[j], 0), nt = (cnt + NT - 1) / NT;
+        if (t >= 0 && t < nt) {
+          h->expert = e0 + 4 * lane + j;
+          h->row0 = o[j] + t * NT;
+          h->cnt = min(NT, cnt - t * NT);
+        }
+        t -= nt;
+      }
+    }
+    before += __shfl_sync(0xFFFFFFFFu, incl, 31);
+    if (before > tile) break;
+  }
+}
+
+__device__ __forceinline__ void store_y(void* y, int64_t i, int dtype, float v) {
+  if (dtype == BLUT_BF16)
+    static_cast<uint16_t*>(y)[i] = f32_to_act<true>(v);
+  else if (dtype == BLUT_F16)
+    static_cast<uint16_t*>(y)[i] = f32_to_act<false>(v);
+  else
+    static_cast<float*>(y)[i] = v;
+}
+
+template <bool kMX, int NT>
+__global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kernel(const Fp4Params p) {
+  using C = Fp4Cfg<kMX, NT>;
+  extern __shared__ __align__(1024) uint8_t fp4_smem[];
+  uint8_t* smem = fp4_smem;
+  Fp4Header* h = reinterpret_cast<Fp4Header*>(smem);
+  uint8_t* ring = smem + kHeader;
+  volatile int* abort_flag = &h->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.split > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / p.split;  // 128-row tile of W
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(smem_u32(h->wfull + s), 1);
+      mbar_init(smem_u32(h->sfull + s), 2);
+      mbar_init(smem_u32(h->empty + s), 1);
+    }
+    mbar_init(smem_u32(&h->acc), 1);
+    mbar_init(smem_u32(&h->fin), 1);
+    h->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&h->tmem)),
+                 "r"(C::kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (warp == 2) {
+    if (p.experts) {
+      if (lane == 0) h->cnt = 0;
+      __syncwarp();
+      find_tile<NT>(p, blockIdx.y, lane, h);
+    } else if (lane == 0) {
+      h->expert = 0;
+      h->row0 = blockIdx.y * NT;
+      h->cnt = (int)min((int64_t)NT, p.x_rows - h->row0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = h->tmem;
+  const int cnt = h->cnt, row0 = h->row0, expert = cnt > 0 ? h->expert : 0;
+  // this CTA's K range; every rank of a cluster has the same tile, so all or
+  // none of them have work
+  const int b0 = (int)((int64_t)p.kblocks * rank / p.split), b1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
+  const int nb = cnt > 0 ? b1 - b0 : 0;
+
+  if (cnt > 0) {
+    if (warp == 0) {
+      // ---------------------------------------------------------- producer --
+      if (lane == 0) {
+        const uint8_t* wsrc = p.w + expert * p.wstride + ((int64_t)tile * p.kblocks + b0) * C::kA;
+        const uint8_t* xsrc = p.xc + ((int64_t)b0 * 4 * p.x_rows + row0) * 16;
+        const uint32_t xbytes = (uint32_t)cnt * 16;
+        int i = 0;
+        for (; i < nb; ++i) {
+          const int s = i % C::kStages;
+          if (i >= C::kStages && !wait_or_abort(smem_u32(h->empty + s), (uint32_t)(i / C::kStages - 1) & 1u, abort_flag,
+                                                &g_fp4_status, p.wait_ns))
+            break;
+          const uint32_t bar = smem_u32(h->wfull + s), dst = smem_u32(ring + s * C::kStage);
+          mbar_expect_tx(bar, C::kA + 4 * xbytes);
+          bulk_g2s(dst, wsrc + (int64_t)i * C::kA, C::kA, bar);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            bulk_g2s(dst + C::kA + c * NT * 16, xsrc + ((int64_t)i * 4 + c) * p.x_rows * 16, xbytes, bar);
+        }
+        if (i < nb)  // gave up: let the copies in flight land
+          for (int j = max(0, i - C::kStages); j < i; ++j)
+            wait_drain(smem_u32(h->wfull + j % C::kStages), (uint32_t)(j / C::kStages) & 1u);
+      }
+    } else if (warp == 1) {
+      // --------------------------------------------------------------- MMA --
+      if (lane == 0) {
+        const int n = (cnt + 15) & ~15;
+        bool ok = true;
+        int i = 0;
+        for (; i < nb; ++i) {
+          const int s = i % C::kStages;
+          const uint32_t ph = (uint32_t)(i / C::kStages) & 1u;
+          ok = wait_or_abort(smem_u32(h->wfull + s), ph, abort_flag, &g_fp4_status, p.wait_ns) &&
+               wait_or_abort(smem_u32(h->sfull + s), ph, abort_flag, &g_fp4_status, p.wait_ns);
+          if (C::kSlots < C::kStages && ok && i >= C::kSlots) {
+            // the MMAs that read this slot of scales are done
+            const int j = i - C::kSlots;
+            ok = wait_or_abort(smem_u32(h->empty + j % C::kStages), (uint32_t)(j / C::kStages) & 1u, abort_flag,
+                               &g_fp4_status, p.wait_ns);
+          }
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(ring + s * C::kStage);
+          const uint32_t slot = tmem + NT + (i % C::kSlots) * C::kSlotCols;
+#pragma unroll
+          for (int w = 0; w < C::kWords; ++w) {
+            cp_scales(slot + w * C::kWordCols, st + kFp4UnitCodes + 512 * w);
+#pragma unroll
+            for (int g = 0; g < C::kGroups; ++g)
+              cp_scales(slot + w * C::kWordCols + 4 + 4 * g, st + C::kA + C::kB + 512 * (w * C::kGroups + g));
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t sc = slot + (kMX ? 0 : k * C::kWordCols);
+            mma_fp4<kMX>(tmem, tc_desc(st + k * 4096, 2048, 128), tc_desc(st + C::kA + k * 2 * NT * 16, NT * 16, 128),
+                         idesc_fp4<kMX>(n, k), sc, sc + 4, (uint32_t)(i | k));
+          }
+          tc_commit(smem_u32(h->empty + s));
+        }
+        if (ok) {
+          tc_commit(smem_u32(&h->acc));
+        } else if (i > 0) {  // gave up: let the MMAs issued so far finish
+          tc_commit(smem_u32(&h->fin));
+          wait_drain(smem_u32(&h->fin), 0);
+        }
+      }
+    } else {
+      // ------------------------------------------------------ token scales --
+      constexpr int kWordsAll = C::kWords * NT;
+      constexpr int kIt = (kWordsAll + 63) / 64;
+      const int t = threadIdx.x - 64;
+      const uint32_t* src[kIt];
+      uint32_t dst[kIt], buf[kPrefetch][kIt];
+      bool on[kIt];
+#pragma unroll
+      for (int q = 0; q < kIt; ++q) {
+        const int idx = t + 64 * q, r = idx % NT, w = idx / NT;
+        on[q] = idx < kWordsAll && r < cnt;
+        src[q] = p.xs + ((int64_t)b0 * C::kWords + w) * p.x_rows + row0 + r;
+        dst[q] = C::kA + C::kB + (w * C::kGroups + r / 128) * 512 + (r % 32) * 16 + ((r % 128) / 32) * 4;
+      }
+      const int64_t step = (int64_t)C::kWords * p.x_rows;
+#pragma unroll
+      for (int j = 0; j < kPrefetch; ++j)
+#pragma unroll
+        for (int q = 0; q < kIt; ++q) buf[j][q] = j < nb && on[q] ? __ldg(src[q] + j * step) : 0u;
+      bool ok = true;
+      for (int i0 = 0; i0 < nb && ok; i0 += kPrefetch) {
+#pragma unroll
+        for (int j = 0; j < kPrefetch; ++j) {
+          const int i = i0 + j, s = i % C::kStages;
+          if (i < nb && ok) {
+            if (i >= C::kStages) {
+              ok = wait_or_abort(smem_u32(h->empty + s), (uint32_t)(i / C::kStages - 1) & 1u, abort_flag, &g_fp4_status,
+                                 p.wait_ns);
+              ok = __all_sync(0xFFFFFFFFu, ok);
+            }
+            if (ok) {
+#pragma unroll
+              for (int q = 0; q < kIt; ++q)
+                if (on[q]) *reinterpret_cast<uint32_t*>(ring + s * C::kStage + dst[q]) = buf[j][q];
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(h->sfull + s));
+#pragma unroll
+              for (int q = 0; q < kIt; ++q)
+                if (i + kPrefetch < nb && on[q]) buf[j][q] = __ldg(src[q] + (i + kPrefetch) * step);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+
+    // ------------------------------------------------------------ epilogue --
+    bool ok = wait_or_abort(smem_u32(&h->acc), 0, abort_flag, &g_fp4_status, p.wait_ns);
+    ok = __all_sync(0xFFFFFFFFu, ok);
+    tc_fence_after();
+    const float alpha = (p.xg ? __ldg(p.xg) : 1.0f) * (p.wg ? __ldg(p.wg + expert) : 1.0f);
+    const int r = 32 * warp + lane;  // weight row inside the tile
+    const int64_t col = (int64_t)tile * 128 + r;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
+    if (p.split == 1) {
+      if (ok) {
+#pragma unroll 1
+        for (int c = 0; c < cnt; c += 16) {
+          uint32_t v[16];
+          tc_ld16(lane_base + c, v);
+          tc_wait_ld16(v);
+          if (col < p.n) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (c + j < cnt) store_y(p.y, (row0 + c + j) * p.ldy + col, p.out_dtype, __uint_as_float(v[j]) * alpha);
+          }
+        }
+      }
+    } else {
+      // the ring is free: the last MMA has read it
+      float* part = reinterpret_cast<float*>(ring);
+      if (ok) {
+#pragma unroll 1
+        for (int c = 0; c < cnt; c += 16) {
+          uint32_t v[16];
+          tc_ld16(lane_base + c, v);
+          tc_wait_ld16(v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c + j < NT) part[(c + j) * 128 + r] = __uint_as_float(v[j]);
+        }
+      }
+      cluster_sync();
+      if (ok) {
+        for (int c = rank; c < cnt; c += p.split) {
+          const uint32_t a = smem_u32(part + c * 128 + r);
+          float sum = 0.0f;
+          for (int q = 0; q < p.split; ++q) sum += ld_peer(a, q);
+          if (col < p.n) store_y(p.y, (row0 + c) * p.ldy + col, p.out_dtype, sum * alpha);
+        }
+      }
+      cluster_sync();  // no CTA leaves while another still reads its partial tile
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols));
+}
+
+template <bool kMX, int NT>
+int launch(const Fp4Params& p, int row_tiles, int64_t token_tiles, cudaStream_t stream) {
+  using C = Fp4Cfg<kMX, NT>;
+  auto kern = fp4_mm_kernel<kMX, NT>;
+  static std::atomic<bool> set[kMaxDevices];
+  const int dev = cache_device();
+  if (dev < 0 || !set[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
+      return BLUT_ERR_CUDA;
+    if (dev >= 0) set[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(row_tiles * p.split), (unsigned)token_tiles);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  if (p.split > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH;
+}
+
+template <bool kMX>
+int dispatch(Fp4Params& p, int64_t m, cudaStream_t stream) {
+  const int row_tiles = (p.n + 127) / 128;
+  // tokens per matrix: their number for one matrix, the mean for runs
+  const int64_t mean = p.experts ? (m + p.experts - 1) / p.experts : m;
+  const int nt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 192;
+  // bound on the token tiles: every run may end in a partial one
+  const int64_t tiles = p.experts ? m / nt + std::min<int64_t>(p.experts, m) : (m + nt - 1) / nt;
+  if (tiles > 65535) return BLUT_ERR_UNSUPPORTED;
+  p.split = 1;
+  if (nt <= 128)
+    while (p.split < 8 && tiles * row_tiles * p.split * 2 <= 296 && p.kblocks >= 4 * p.split) p.split *= 2;
+  switch (nt) {
+    case 32: return launch<kMX, 32>(p, row_tiles, tiles, stream);
+    case 64: return launch<kMX, 64>(p, row_tiles, tiles, stream);
+    case 128: return launch<kMX, 128>(p, row_tiles, tiles, stream);
+    default: return launch<kMX, 192>(p, row_tiles, tiles, stream);
+  }
+}
+
+}  // namespace
+}  // namespace blut
+
+using namespace blut;
+
+extern "C" {
+
+int blut_fp4_matmul(const blut_fp4_mm_args* a, void* stream) {
+  if (!a || !fp4_valid(a->w) || !a->w_tiled || !a->x_codes || !a->x_scales || !a->y) return BLUT_ERR_INVALID;
+  if (a->x_rows <= 0 || a->x_rows > kMaxSlots || a->y_ld < a->w.rows) return BLUT_ERR_INVALID;
+  if (a->num_experts < 0 || a->num_experts > kMaxExperts || (a->num_experts && !a->offsets)) return BLUT_ERR_INVALID;
+  if (a->num_experts > 1 && (a->w_stride < blut_fp4_tiled_bytes(&a->w) || a->w_stride % 16)) return BLUT_ERR_INVALID;
+  if (((uintptr_t)a->w_tiled | (uintptr_t)a->x_codes | (uintptr_t)a->x_scales) % 16 != 0) return BLUT_ERR_INVALID;
+  if (a->out_dtype != BLUT_F16 && a->out_dtype != BLUT_BF16 && a->out_dtype != BLUT_F32) return BLUT_ERR_UNSUPPORTED;
+  if ((uintptr_t)a->y % (a->out_dtype == BLUT_F32 ? 4 : 2) != 0) return BLUT_ERR_INVALID;
+  Fp4Params p = {};
+  p.w = static_cast<const uint8_t*>(a->w_tiled);
+  p.wstride = a->w_stride;
+  p.wg = a->w_scale;
+  p.offsets = a->offsets;
+  p.experts = a->num_experts;
+  p.xc = static_cast<const uint8_t*>(a->x_codes);
+  p.xs = static_cast<const uint32_t*>(a->x_scales);
+  p.xg = a->x_scale;
+  p.x_rows = a->x_rows;
+  p.n = (int)a->w.rows;
+  p.kblocks = fp4_kblocks(a->w.cols);
+  p.y = a->y;
+  p.ldy = a->y_ld;
+  p.out_dtype = a->out_dtype;
+  p.wait_ns = wait_limit_ns();
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return a->w.kind == BLUT_FP4_MX ? dispatch<true>(p, a->x_rows, s) : dispatch<false>(p, a->x_rows, s);
+}
+
+int blut_fp4_check_status(void* stream) {
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int st = 0, zero = 0;
+  if (cudaMemcpyFromSymbolAsync(&st, g_fp4_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return BLUT_ERR_CUDA;
+  if (!st) return BLUT_OK;
+  if (cudaMemcpyToSymbolAsync(g_fp4_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return BLUT_ERR_CUDA;
+  return BLUT_ERR_TIMEOUT;
+}
+
+}  // extern "C"

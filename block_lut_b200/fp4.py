@@ -1,0 +1,436 @@
+"""4-bit microscaled matrices: quantisation, and products of two of them.
+
+A matrix is held as 4-bit floats (e2m1) whose blocks of columns share an 8-bit
+scale: value = q * s * g.
+
+* ``nvfp4`` -- blocks of 16 columns, s in e4m3, one float32 g per matrix
+* ``mxfp4`` -- blocks of 32 columns, s a power of two, g = 1
+
+Unlike the LUT formats, whose products take 16-bit activations, both operands
+of these products are 4-bit and the tensor cores multiply them as they are:
+activations are quantised row by row (``quantize_fp4``, or fused with the
+gate's SiLU: ``silu_mul_quantize_fp4``), weights once at load time
+(``FP4Weight``).  ``fp4_matmul`` multiplies rows with one matrix
+(``FP4Linear`` quantises and multiplies), ``fp4_grouped_matmul`` runs of rows
+with one matrix per run, as the routed experts of a layer need it.
+
+There is no counterpart in the reference (its products take 16-bit
+activations: vllm_lut/quant_method.py:230-279).
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from dataclasses import dataclass
+from typing import Optional, Sequence, Union
+
+import torch
+
+from . import _lib
+
+_KIND = {"nvfp4": _lib.FP4_NV, "mxfp4": _lib.FP4_MX}
+_BLOCK = {"nvfp4": 16, "mxfp4": 32}
+_DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+MIN_GLOBAL_SCALE = 2.0 ** -100
+MAX_EXPERTS = 1024
+MAX_ROWS = 1 << 22  # rows of one product
+
+Scale = Union[None, float, torch.Tensor]
+
+
+def _desc(kind: str, rows: int, cols: int) -> _lib.FP4Desc:
+    if kind not in _KIND:
+        raise ValueError(f"unknown 4-bit kind {kind!r}: 'nvfp4' or 'mxfp4'")
+    return _lib.FP4Desc(_KIND[kind], 0, int(rows), int(cols))
+
+
+def _kblocks(cols: int) -> int:
+    return -(-cols // 128)
+
+
+def _rows2d(x: torch.Tensor, what: str) -> torch.Tensor:
+    """x as a CUDA matrix with contiguous rows (any row pitch), copied only when its rows are not."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor (no CPU path)")
+    if x.dtype not in _DT:
+        raise ValueError(f"{what} must be float16, bfloat16 or float32, not {x.dtype}")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"{what} must be a matrix [rows, columns] with at least one column")
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:  # transposed, expanded, overlapping rows
+        x = x.contiguous()
+    return x
+
+
+def _pitch(x: torch.Tensor) -> int:
+    """Elements between rows; a single row's stride says nothing."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _scale_tensor(g: Scale, n: int, device: torch.device, what: str) -> torch.Tensor:
+    """g as n float32 values on the device."""
+    if isinstance(g, torch.Tensor):
+        if g.numel() != n or g.dtype != torch.float32 or g.device != device:
+            raise ValueError(f"{what} must be a float32 tensor of {n} value(s) on {device}")
+        return g.reshape(n).contiguous()
+    g = float(g)
+    if not (math.isfinite(g) and g >= MIN_GLOBAL_SCALE):
+        raise ValueError(f"{what} must be finite and at least 2^-100, not {g}")
+    return torch.full((n,), g, dtype=torch.float32, device=device)
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _bytes_view(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.uint8 else t.view(torch.uint8)
+
+
+@dataclass
+class FP4Matrix:
+    """Rows in 4-bit form, as the quantisers write them (the FP4 layout of ``include/blut.h``).
+
+    ``codes`` uint8 [Kp / 32, rows, 16] and ``scales`` uint8 [words, rows, 4] with Kp = cols rounded up to 128;
+    ``global_scale`` float32 [1] (nvfp4) or None.
+    """
+    kind: str
+    rows: int
+    cols: int
+    codes: torch.Tensor
+    scales: torch.Tensor
+    global_scale: Optional[torch.Tensor] = None
+
+    @classmethod
+    def empty(cls, kind: str, rows: int, cols: int, device, global_scale: Optional[torch.Tensor] = None) -> "FP4Matrix":
+        _desc(kind, rows, cols)
+        kb = _kblocks(cols)
+        return cls(kind, int(rows), int(cols), torch.empty(4 * kb, rows, 16, dtype=torch.uint8, device=device),
+                   torch.empty((2 if kind == "nvfp4" else 1) * kb, rows, 4, dtype=torch.uint8, device=device), global_scale)
+
+    @classmethod
+    def from_checkpoint(cls, kind: str, codes: torch.Tensor, scales: torch.Tensor, cols: int,
+                        global_scale: Scale = None, stream=None) -> "FP4Matrix":
+        """From row-major bytes: codes [rows, nb * B / 2] (even column in the low half), scales [rows, nb]
+        (e4m3 or e8m0 bytes), nb = ceil(cols / B), B = 16 (nvfp4) or 32 (mxfp4)."""
+        return _import(kind, codes, scales, cols, global_scale, stream=stream)
+
+    @_lib.stream_ordered
+    def to_checkpoint(self, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Row-major (codes, scales), the arguments of ``from_checkpoint``."""
+        b = _BLOCK[self.kind]
+        nb = -(-self.cols // b)
+        codes = torch.empty(self.rows, nb * b // 2, dtype=torch.uint8, device=self.codes.device)
+        scales = torch.empty(self.rows, nb, dtype=torch.uint8, device=self.codes.device)
+        if self.rows:
+            d = _desc(self.kind, self.rows, self.cols)
+            with _lib.on_device(codes):
+                _lib.check(_lib.lib().blut_fp4_export(C.byref(d), self.codes.data_ptr(), self.scales.data_ptr(),
+                                                      codes.data_ptr(), scales.data_ptr(), _lib.stream_ptr(stream)),
+                           "fp4_export")
+        return codes, scales
+
+
+@_lib.stream_ordered
+def _import(kind, codes, scales, cols, global_scale, stream=None) -> FP4Matrix:
+    codes, scales = _bytes_view(codes), _bytes_view(scales)
+    rows, cols = codes.shape[0], int(cols)
+    d = _desc(kind, rows, cols)
+    nb = -(-cols // _BLOCK[kind])
+    if cols < 1 or tuple(codes.shape) != (rows, nb * _BLOCK[kind] // 2) or tuple(scales.shape) != (rows, nb):
+        raise ValueError(f"{kind} rows of {cols} columns are codes [rows, {nb * _BLOCK[kind] // 2}] and scales "
+                         f"[rows, {nb}], not {tuple(codes.shape)} and {tuple(scales.shape)}")
+    if not codes.is_cuda or scales.device != codes.device:
+        raise ValueError("codes and scales must be CUDA tensors of one device")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    g = _given_scale(kind, global_scale, codes.device)
+    m = FP4Matrix.empty(kind, rows, cols, codes.device, g)
+    if rows:
+        with _lib.on_device(codes):
+            _lib.check(_lib.lib().blut_fp4_import(C.byref(d), codes.data_ptr(), scales.data_ptr(), m.codes.data_ptr(),
+                                                  m.scales.data_ptr(), _lib.stream_ptr(stream)), "fp4_import")
+    return m
+
+
+def _given_scale(kind: str, g: Scale, device) -> Optional[torch.Tensor]:
+    if kind == "mxfp4":
+        if g is not None:
+            raise ValueError("mxfp4 has no global scale")
+        return None
+    return _scale_tensor(1.0 if g is None else g, 1, device, "global_scale")
+
+
+@_lib.stream_ordered
+def fp4_global_scale(x: torch.Tensor, silu_mul: bool = False, stream=None) -> torch.Tensor:
+    """The nvfp4 scale g of x [rows, cols], float32 [1]: max|x| / 2688 over the finite values (at least 2^-100), with
+    which the largest block's scale is 448, e4m3's last.  ``silu_mul``: of silu(gate) * up, x = [gate | up]."""
+    x = _rows2d(x, "x")
+    cols = _gate_cols(x) if silu_mul else x.shape[1]
+    buf = torch.empty(4, dtype=torch.float32, device=x.device)
+    if x.shape[0] == 0:
+        return buf.fill_(MIN_GLOBAL_SCALE)[:1]
+    with _lib.on_device(x):
+        _lib.check(_lib.lib().blut_fp4_global_scale(x.data_ptr(), _DT[x.dtype], x.shape[0], cols, _pitch(x),
+                                                    int(silu_mul), buf.data_ptr(), _lib.stream_ptr(stream)),
+                   "fp4_global_scale")
+    return buf[:1]
+
+
+def _gate_cols(x: torch.Tensor) -> int:
+    if x.shape[1] % 2:
+        raise ValueError(f"rows of gate and up have an even width, not {x.shape[1]}")
+    return x.shape[1] // 2
+
+
+def _row_scale(kind: str, g: Scale, x: torch.Tensor, silu_mul: bool, stream) -> Optional[torch.Tensor]:
+    if kind == "nvfp4" and g is None:
+        return fp4_global_scale(x, silu_mul, stream=stream)
+    return _given_scale(kind, g, x.device)
+
+
+@_lib.stream_ordered
+def quantize_fp4(x: torch.Tensor, kind: str = "nvfp4", global_scale: Scale = None,
+                 row_index: Optional[torch.Tensor] = None, stream=None) -> FP4Matrix:
+    """x [rows, cols] (float16, bfloat16 or float32, any row pitch) in 4-bit form.
+
+    nvfp4: s = e4m3(max|x| / (6 g)) per 16 columns; mxfp4: s = 2^(floor(log2 max|x|) - 2) per 32; q = e2m1(x / (s g)).
+    Roundings go by the exact quotients (nearest, ties to even, saturating); a block with an infinity or a NaN gets
+    the scale NaN.  ``global_scale`` (nvfp4): g as a float or a float32 [1] tensor, positive, finite, at least 2^-100;
+    None takes ``fp4_global_scale(x)``.  ``row_index`` int32 [n]: row i of the result is x[row_index[i]] (gathered in
+    the same pass), a row of zeros where the index is outside x.
+    """
+    x = _rows2d(x, "x")
+    n = x.shape[0]
+    if row_index is not None:
+        if row_index.dim() != 1 or row_index.dtype != torch.int32 or row_index.device != x.device:
+            raise ValueError("row_index must be an int32 vector on x's device")
+        row_index = row_index.contiguous()
+        n = row_index.shape[0]
+    d = _desc(kind, n, x.shape[1])
+    g = _row_scale(kind, global_scale, x, False, stream)
+    m = FP4Matrix.empty(kind, n, x.shape[1], x.device, g)
+    if n == 0:
+        return m
+    if x.shape[0] == 0:
+        raise ValueError("row_index into an x without rows")
+    with _lib.on_device(x):
+        _lib.check(_lib.lib().blut_fp4_quantize(C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(row_index),
+                                                x.shape[0], _p(g), m.codes.data_ptr(), m.scales.data_ptr(),
+                                                _lib.stream_ptr(stream)), "fp4_quantize")
+    return m
+
+
+@_lib.stream_ordered
+def silu_mul_quantize_fp4(gate_up: torch.Tensor, kind: str = "nvfp4", global_scale: Scale = None,
+                          stream=None) -> FP4Matrix:
+    """silu(gate) * up in 4-bit form, gate_up = [gate | up] [rows, 2 cols] as the gate/up products write it; rounded
+    once, from the exact product to its code.  Arguments as ``quantize_fp4``."""
+    x = _rows2d(gate_up, "gate_up")
+    cols = _gate_cols(x)
+    d = _desc(kind, x.shape[0], cols)
+    g = _row_scale(kind, global_scale, x, True, stream)
+    m = FP4Matrix.empty(kind, x.shape[0], cols, x.device, g)
+    if x.shape[0] == 0:
+        return m
+    with _lib.on_device(x):
+        _lib.check(_lib.lib().blut_fp4_silu_mul_quantize(C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(g),
+                                                         m.codes.data_ptr(), m.scales.data_ptr(),
+                                                         _lib.stream_ptr(stream)), "fp4_silu_mul_quantize")
+    return m
+
+
+@_lib.stream_ordered
+def dequantize_fp4(q: FP4Matrix, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
+    """The values q stands for, [rows, cols] in ``dtype`` (float32 products, rounded once to 16 bits)."""
+    if dtype not in _DT:
+        raise ValueError(f"dtype must be float16, bfloat16 or float32, not {dtype}")
+    out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.codes.device)
+    if q.rows == 0:
+        return out
+    d = _desc(q.kind, q.rows, q.cols)
+    with _lib.on_device(out):
+        _lib.check(_lib.lib().blut_fp4_dequantize(C.byref(d), q.codes.data_ptr(), q.scales.data_ptr(),
+                                                  _p(q.global_scale), out.data_ptr(), _DT[dtype], q.cols,
+                                                  _lib.stream_ptr(stream)), "fp4_dequantize")
+    return out
+
+
+@dataclass
+class FP4Weight:
+    """One weight matrix [rows, cols], or one per expert, in the products' tiled layout.
+
+    ``experts`` None for a single matrix; ``global_scale`` float32 [max(experts, 1)] (nvfp4) or None.
+    """
+    kind: str
+    rows: int
+    cols: int
+    experts: Optional[int]
+    tiled: torch.Tensor
+    stride: int
+    global_scale: Optional[torch.Tensor] = None
+
+    @classmethod
+    def from_quantized(cls, mats: Union[FP4Matrix, Sequence[FP4Matrix]], stream=None) -> "FP4Weight":
+        """Lay out one matrix, or a list of matrices of one kind and shape (the experts)."""
+        return _pack(mats, stream=stream)
+
+    @classmethod
+    def from_checkpoint(cls, kind: str, codes: torch.Tensor, scales: torch.Tensor, cols: int,
+                        global_scale: Scale = None, stream=None) -> "FP4Weight":
+        """From row-major bytes (``FP4Matrix.from_checkpoint``), [rows, ...] or [experts, rows, ...] with one global
+        scale per expert."""
+        return _weight_from_checkpoint(kind, codes, scales, cols, global_scale, stream=stream)
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor, kind: str = "nvfp4", stream=None) -> "FP4Weight":
+        """From float weights [rows, cols] or [experts, rows, cols], each matrix with a global scale of its own."""
+        return _weight_quantize(w, kind, stream=stream)
+
+    def weight_bytes(self, experts: int = 1) -> int:
+        """Bytes streamed for ``experts`` matrices."""
+        return experts * self.stride
+
+
+@_lib.stream_ordered
+def _pack(mats, stream=None) -> FP4Weight:
+    single = isinstance(mats, FP4Matrix)
+    mats = [mats] if single else list(mats)
+    if not mats or any((m.kind, m.rows, m.cols, m.codes.device) != (mats[0].kind, mats[0].rows, mats[0].cols,
+                                                                    mats[0].codes.device) for m in mats):
+        raise ValueError("FP4Weight needs matrices of one kind, shape and device")
+    if len(mats) > MAX_EXPERTS:
+        raise ValueError(f"at most {MAX_EXPERTS} experts")
+    m0 = mats[0]
+    d = _desc(m0.kind, m0.rows, m0.cols)
+    stride = int(_lib.lib().blut_fp4_tiled_bytes(C.byref(d)))
+    if stride <= 0:
+        raise ValueError(f"no 4-bit weight layout for [{m0.rows}, {m0.cols}]")
+    dev = m0.codes.device
+    tiled = torch.empty(len(mats) * stride, dtype=torch.uint8, device=dev)
+    with _lib.on_device(tiled):
+        for i, m in enumerate(mats):
+            _lib.check(_lib.lib().blut_fp4_pack_tiled(C.byref(d), m.codes.data_ptr(), m.scales.data_ptr(),
+                                                      tiled.data_ptr() + i * stride, _lib.stream_ptr(stream)),
+                       "fp4_pack_tiled")
+    g = None if m0.kind == "mxfp4" else torch.cat([m.global_scale.reshape(1) for m in mats])
+    return FP4Weight(m0.kind, m0.rows, m0.cols, None if single else len(mats), tiled, stride, g)
+
+
+@_lib.stream_ordered
+def _weight_from_checkpoint(kind, codes, scales, cols, global_scale, stream=None) -> FP4Weight:
+    if codes.dim() == 2:
+        return _pack(_import(kind, codes, scales, cols, global_scale))
+    if codes.dim() != 3 or scales.dim() != 3 or scales.shape[0] != codes.shape[0] or codes.shape[0] == 0:
+        raise ValueError("expert codes and scales are [experts, rows, bytes]")
+    n = codes.shape[0]
+    g = [None] * n
+    if kind == "nvfp4":
+        g = list(_scale_tensor(1.0 if global_scale is None else global_scale, n, codes.device, "global_scale").split(1))
+    elif global_scale is not None:
+        raise ValueError("mxfp4 has no global scale")
+    return _pack([_import(kind, codes[e], scales[e], cols, g[e]) for e in range(n)])
+
+
+@_lib.stream_ordered
+def _weight_quantize(w, kind, stream=None) -> FP4Weight:
+    if w.dim() == 3:
+        return _pack([quantize_fp4(w[e], kind) for e in range(w.shape[0])])
+    return _pack(quantize_fp4(w, kind))
+
+
+def _product(x: FP4Matrix, w: FP4Weight, offsets, out, out_dtype, stream) -> torch.Tensor:
+    if not isinstance(x, FP4Matrix) or not isinstance(w, FP4Weight):
+        raise ValueError("4-bit products take an FP4Matrix and an FP4Weight")
+    if (x.kind, x.cols) != (w.kind, w.cols):
+        raise ValueError(f"x is {x.kind} of {x.cols} columns, the weight {w.kind} of {w.cols}")
+    dev = x.codes.device
+    if w.tiled.device != dev:
+        raise ValueError(f"x is on {dev}, the weight on {w.tiled.device}")
+    if x.rows > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows in one product")
+    if out is None:
+        out = torch.empty(x.rows, w.rows, dtype=out_dtype or torch.bfloat16, device=dev)
+    if out.dtype not in _DT or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError("the output is float16, bfloat16 or float32 (and of out_dtype, where both are given)")
+    if tuple(out.shape) != (x.rows, w.rows) or out.device != dev:
+        raise ValueError(f"out must be [{x.rows}, {w.rows}] on {dev}")
+    if x.rows == 0:
+        return out
+    if out.stride(1) != 1 and w.rows > 1 or (x.rows > 1 and out.stride(0) < w.rows):
+        raise ValueError("out must have contiguous, separate rows")
+    a = _lib.FP4MMArgs()
+    a.w = _desc(w.kind, w.rows, w.cols)
+    a.w_tiled, a.w_stride, a.w_scale = w.tiled.data_ptr(), w.stride, _p(w.global_scale)
+    a.num_experts = 0 if offsets is None else w.experts
+    a.out_dtype = _DT[out.dtype]
+    a.offsets = _p(offsets)
+    a.x_codes, a.x_scales, a.x_scale = x.codes.data_ptr(), x.scales.data_ptr(), _p(x.global_scale)
+    a.x_rows = x.rows
+    a.y, a.y_ld = out.data_ptr(), _pitch(out)
+    with _lib.on_device(out):
+        _lib.check(_lib.lib().blut_fp4_matmul(C.byref(a), _lib.stream_ptr(stream)), "fp4_matmul")
+    return out
+
+
+@_lib.stream_ordered
+def fp4_matmul(x: FP4Matrix, w: FP4Weight, out: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None, stream=None) -> torch.Tensor:
+    """y = x W^T, [x.rows, w.rows] in bfloat16 (``out_dtype``: or float16, float32); float32 sums."""
+    if isinstance(w, FP4Weight) and w.experts is not None:
+        raise ValueError("a stack of experts goes through fp4_grouped_matmul")
+    return _product(x, w, None, out, out_dtype, stream)
+
+
+@_lib.stream_ordered
+def fp4_grouped_matmul(x: FP4Matrix, w: FP4Weight, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
+                       out_dtype: Optional[torch.dtype] = None, stream=None) -> torch.Tensor:
+    """y[t] = W_e x_t for offsets[e] <= t < offsets[e + 1].
+
+    ``offsets`` int32 [experts + 1] on the device, not decreasing; it is read by the kernel, so nothing waits for
+    the host and the call can be captured.  Runs may be empty or start anywhere.  Rows of ``out`` outside every run
+    (before offsets[0], from offsets[-1]) are left as they were; without ``out`` they are undefined.
+    """
+    if not isinstance(w, FP4Weight) or w.experts is None:
+        raise ValueError("fp4_grouped_matmul takes a stack of experts")
+    if not isinstance(offsets, torch.Tensor) or offsets.dtype != torch.int32 or tuple(offsets.shape) != (w.experts + 1,) \
+            or offsets.device != w.tiled.device:
+        raise ValueError(f"offsets must be an int32 vector of {w.experts + 1} on the weights' device")
+    return _product(x, w, offsets.contiguous(), out, out_dtype, stream)
+
+
+def fp4_check_status(device=None, stream=None) -> None:
+    """Raise if a device-side wait of the products on ``device`` (default: current) timed out; synchronises."""
+    with torch.cuda.device(device) if device is not None else torch.cuda.device(torch.cuda.current_device()):
+        _lib.check(_lib.lib().blut_fp4_check_status(_lib.stream_ptr(stream)), "fp4 status")
+
+
+class FP4Linear:
+    """y = x W^T with a 4-bit weight and activations quantised on the way in.
+
+    ``act_scale`` (nvfp4): the activations' global scale, from calibration (float or float32 [1] tensor); None takes
+    each call's own maximum (one more pass over x).
+    """
+
+    def __init__(self, weight: FP4Weight, act_scale: Scale = None):
+        if weight.experts is not None:
+            raise ValueError("FP4Linear takes a single matrix")
+        self.weight, self.rows, self.cols = weight, weight.rows, weight.cols
+        self.act_scale = None if act_scale is None else _given_scale(weight.kind, act_scale, weight.tiled.device)
+
+    @_lib.stream_ordered
+    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                stream=None) -> torch.Tensor:
+        """x [..., cols] -> [..., rows] in x's dtype (or ``out_dtype``)."""
+        if x.shape[-1] != self.cols:
+            raise ValueError(f"x must be [..., {self.cols}]")
+        x2 = x if x.dim() == 2 else x.reshape(-1, self.cols)
+        q = quantize_fp4(x2, self.weight.kind, self.act_scale)
+        if out is not None:
+            if tuple(out.shape) != tuple(x.shape[:-1]) + (self.rows,):
+                raise ValueError(f"out must be {list(x.shape[:-1]) + [self.rows]}")
+            o2 = out if out.dim() == 2 else out.view(-1, self.rows)
+            fp4_matmul(q, self.weight, o2, out_dtype)
+            return out
+        y = fp4_matmul(q, self.weight, None, out_dtype or x.dtype)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.rows)
+
+    __call__ = forward

@@ -440,6 +440,101 @@ BLUT_API int blut_ep_combine(const blut_ep_desc* d, int num_tokens, const float*
  * this rank's exchanges gave up. */
 BLUT_API int blut_ep_check_status(const blut_ep_desc* d, void* stream);
 
+/* ------------------------------------------------- 4-bit microscaled ----
+ * Matrices whose blocks of columns share an 8-bit scale and whose values are
+ * 4-bit floats (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives):
+ *   value = q * s * g
+ *   BLUT_FP4_NV  blocks of 16 columns, s in e4m3, one float32 g per matrix
+ *   BLUT_FP4_MX  blocks of 32 columns, s a power of two (e8m0), g = 1
+ * Both operands of the products are in this form; the tensor cores multiply
+ * them as they are (no counterpart in the reference, whose products take
+ * 16-bit activations).
+ *
+ * FP4 layout, of a matrix [rows][cols], Kp = cols rounded up to 128:
+ *   codes  [Kp / 32][rows][16]  32 columns of a row, column 2j in the low
+ *                               half of byte j; zero past cols
+ *   scales [Kp / 64 (NV) | Kp / 128 (MX)][rows][4]  four blocks of a row
+ * Row-major form (checkpoints): codes [rows][nb * B / 2], scales [rows][nb],
+ * nb = ceil(cols / B), B = 16 or 32. */
+enum { BLUT_FP4_NV = 1, BLUT_FP4_MX = 2 };
+
+typedef struct {
+  int32_t kind; /* BLUT_FP4_*                                                   */
+  int32_t reserved;
+  int64_t rows; /* 1 .. 2^31 - 1                                                */
+  int64_t cols; /* 1 .. 2^24                                                    */
+} blut_fp4_desc;
+
+/* Bytes of the FP4 layout's codes and scales, and of the tiled layout (the
+ * weight operand; rows are padded to 128); < 0 for an invalid description. */
+BLUT_API int64_t blut_fp4_codes_bytes(const blut_fp4_desc* desc);
+BLUT_API int64_t blut_fp4_scales_bytes(const blut_fp4_desc* desc);
+BLUT_API int64_t blut_fp4_tiled_bytes(const blut_fp4_desc* desc);
+
+/* out[0] = max(max|x| / 2688, 2^-100) over the finite values of x [rows][cols]
+ * (row pitch ld elements, BLUT_F16 / BF16 / F32), or, with silu_mul, of
+ * silu(x[:, :cols]) * x[:, cols:2 cols] computed in float32.  out: 16 bytes,
+ * 16-byte aligned; the last 8 are scratch. */
+BLUT_API int blut_fp4_global_scale(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
+                                   int32_t silu_mul, float* out, void* stream);
+
+/* x [src_rows][cols] -> FP4 layout of desc, row r from source row
+ * row_index[r] (an index outside [0, src_rows) gives a row of zeros), or from
+ * row r with row_index NULL (src_rows = desc->rows then).
+ *   NV: s = e4m3(max|x| / (6 g)), nearest even, at most 448; g = *global_scale
+ *       (device; positive, finite, at least 2^-100)
+ *   MX: s = 2^(floor(log2 max|x|) - 2), within 2^-127 .. 2^125; global_scale unused
+ *   q = e2m1(x / (s g)), nearest even, at most 6 in magnitude; 0 where s = 0
+ * Both roundings go by the exact quotient.  A block that holds an infinity or
+ * a NaN gets the scale NaN.  codes and scales 16-byte aligned. */
+BLUT_API int blut_fp4_quantize(const blut_fp4_desc* desc, const void* x, int32_t dtype, int64_t ld,
+                               const int32_t* row_index, int64_t src_rows, const float* global_scale, void* codes,
+                               void* scales, void* stream);
+/* The same of silu(gate) * up, rounded once: gate_up [rows][2 cols], gate in
+ * the first half of a row (the order of the gate/up products here). */
+BLUT_API int blut_fp4_silu_mul_quantize(const blut_fp4_desc* desc, const void* gate_up, int32_t dtype, int64_t ld,
+                                        const float* global_scale, void* codes, void* scales, void* stream);
+/* FP4 layout -> out [rows][cols] (row pitch ld elements); global_scale NULL: 1. */
+BLUT_API int blut_fp4_dequantize(const blut_fp4_desc* desc, const void* codes, const void* scales,
+                                 const float* global_scale, void* out, int32_t dtype, int64_t ld, void* stream);
+
+/* Row-major form -> FP4 layout, and back. */
+BLUT_API int blut_fp4_import(const blut_fp4_desc* desc, const void* row_codes, const void* row_scales, void* codes,
+                             void* scales, void* stream);
+BLUT_API int blut_fp4_export(const blut_fp4_desc* desc, const void* codes, const void* scales, void* row_codes,
+                             void* row_scales, void* stream);
+/* FP4 layout -> tiled layout (blut_fp4_tiled_bytes, 16-byte aligned). */
+BLUT_API int blut_fp4_pack_tiled(const blut_fp4_desc* desc, const void* codes, const void* scales, void* tiled,
+                                 void* stream);
+
+typedef struct {
+  blut_fp4_desc w;        /* one weight matrix W [rows][cols]                   */
+  const void* w_tiled;    /* max(num_experts, 1) matrices in the tiled layout   */
+  int64_t w_stride;       /* bytes between them, a multiple of 16               */
+  const float* w_scale;   /* g of each matrix (device), NULL: 1                 */
+  int32_t num_experts;    /* 0: one matrix; E (at most 1024): grouped           */
+  int32_t out_dtype;      /* BLUT_F16, BF16 or F32                              */
+  const int32_t* offsets; /* grouped: [E + 1] (device), rows offsets[e] ..
+                             offsets[e + 1] - 1 of x belong to matrix e; must
+                             not decrease.  Values are clamped to [0, x_rows]   */
+  const void* x_codes;    /* x [x_rows][cols], FP4 layout of w.kind             */
+  const void* x_scales;
+  const float* x_scale;   /* g of x (device), NULL: 1                           */
+  int64_t x_rows;         /* 1 .. 2^22                                          */
+  void* y;                /* [x_rows][rows], pitch y_ld elements                */
+  int64_t y_ld;
+} blut_fp4_mm_args;
+
+/* y[t] = W x_t for every row of x, or, grouped, y[t] = W_e x_t for the rows
+ * of each expert's run; rows outside every run are left as they were.
+ * float32 accumulation on the tensor cores, one launch, no workspace; the
+ * result does not depend on timing. */
+BLUT_API int blut_fp4_matmul(const blut_fp4_mm_args* args, void* stream);
+/* Reads and clears the device status of this device's blut_fp4_matmul calls:
+ * BLUT_ERR_TIMEOUT when a bounded wait gave up.  Synchronises the stream;
+ * diagnostic only. */
+BLUT_API int blut_fp4_check_status(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,151 @@
+"""4-bit microscaled operators without a GPU: sizes, refusals, and the float64 restatement against itself."""
+import ctypes as C
+
+import pytest
+import torch
+
+from block_lut_b200 import _lib
+from block_lut_b200 import fp4 as F
+from tests import _fp4_ref as R
+
+
+def desc(kind=1, rows=4, cols=64):
+    return _lib.FP4Desc(kind, 0, rows, cols)
+
+
+@pytest.mark.parametrize("kind,rows,cols,codes,scales,tiled", [
+    (1, 1, 1, 64, 8, 9216), (2, 1, 1, 64, 4, 8704), (1, 128, 128, 8192, 1024, 9216), (2, 129, 256, 129 * 128, 129 * 8, 4 * 8704),
+    (1, 2816, 2048, 2816 * 1024, 2816 * 128, 22 * 16 * 9216)])
+def test_sizes(kind, rows, cols, codes, scales, tiled):
+    L, d = _lib.lib(), desc(kind, rows, cols)
+    assert L.blut_fp4_codes_bytes(C.byref(d)) == codes
+    assert L.blut_fp4_scales_bytes(C.byref(d)) == scales
+    assert L.blut_fp4_tiled_bytes(C.byref(d)) == tiled
+
+
+@pytest.mark.parametrize("d", [desc(0), desc(3), desc(rows=0), desc(cols=0), desc(rows=-1), desc(rows=1 << 31), desc(cols=(1 << 24) + 1)])
+def test_bad_descriptions(d):
+    L = _lib.lib()
+    for f in (L.blut_fp4_codes_bytes, L.blut_fp4_scales_bytes, L.blut_fp4_tiled_bytes):
+        assert f(C.byref(d)) == _lib.BLUT_ERR_INVALID
+    assert L.blut_fp4_codes_bytes(None) == _lib.BLUT_ERR_INVALID
+    P = 256
+    assert L.blut_fp4_quantize(C.byref(d), P, 1, 1 << 25, None, d.rows, P, P, P, None) == _lib.BLUT_ERR_INVALID
+    assert L.blut_fp4_dequantize(C.byref(d), P, P, P, P, 1, 1 << 25, None) == _lib.BLUT_ERR_INVALID
+    assert L.blut_fp4_pack_tiled(C.byref(d), P, P, P, None) == _lib.BLUT_ERR_INVALID
+
+
+def test_c_refusals():
+    """Every refusal comes from the host, before any launch."""
+    L, P, bad, uns = _lib.lib(), 256, _lib.BLUT_ERR_INVALID, _lib.BLUT_ERR_UNSUPPORTED
+    d = desc()
+    q = L.blut_fp4_quantize
+    assert q(None, P, 1, 64, None, 4, P, P, P, None) == bad
+    for hole in range(3):
+        a = [P, P, P]
+        a[hole] = None
+        assert q(C.byref(d), a[0], 1, 64, None, 4, P, a[1], a[2], None) == bad
+    assert q(C.byref(d), P, 1, 63, None, 4, P, P, P, None) == bad  # pitch below the columns
+    assert q(C.byref(d), P, 1, 64, None, 5, P, P, P, None) == bad  # rows without an index
+    assert q(C.byref(d), P, 1, 64, P, 0, P, P, P, None) == bad  # an index into nothing
+    assert q(C.byref(d), P, 1, 64, None, 4, None, P, P, None) == bad  # nvfp4 without g
+    assert q(C.byref(d), P, 1, 64, None, 4, P, P + 8, P, None) == bad  # alignment
+    assert q(C.byref(d), P + 1, 1, 64, None, 4, P, P, P, None) == bad
+    assert q(C.byref(d), P, 7, 64, None, 4, P, P, P, None) == uns
+    s = L.blut_fp4_silu_mul_quantize
+    assert s(C.byref(d), P, 1, 127, P, P, P, None) == bad
+    assert s(None, P, 1, 128, P, P, P, None) == bad
+    assert L.blut_fp4_dequantize(C.byref(d), P, P, P, P, 1, 63, None) == bad
+    assert L.blut_fp4_dequantize(C.byref(d), P, P, P, P, 9, 64, None) == uns
+    assert L.blut_fp4_global_scale(P, 1, 0, 64, 64, 0, P, None) == bad
+    assert L.blut_fp4_global_scale(P, 1, 4, 64, 64, 1, P, None) == bad
+    assert L.blut_fp4_global_scale(P, 1, 4, 64, 64, 0, P + 4, None) == bad
+    assert L.blut_fp4_global_scale(P, 5, 4, 64, 64, 0, P, None) == uns
+    assert L.blut_fp4_import(C.byref(d), None, P, P, P, None) == bad
+    assert L.blut_fp4_export(C.byref(d), P, P, P, None, None) == bad
+
+
+def mm_args(**kw):
+    a = _lib.FP4MMArgs()
+    a.w = desc(1, 256, 128)
+    a.w_tiled = a.x_codes = a.x_scales = a.y = a.offsets = 256
+    a.w_stride = 2 * 9216
+    a.out_dtype, a.x_rows, a.y_ld = _lib.BF16, 8, 256
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(w_tiled=None), -1), (dict(x_codes=None), -1), (dict(x_scales=None), -1), (dict(y=None), -1), (dict(x_rows=0), -1),
+    (dict(x_rows=(1 << 22) + 1), -1), (dict(y_ld=255), -1), (dict(num_experts=-1), -1), (dict(num_experts=1025), -1),
+    (dict(num_experts=2, offsets=None), -1), (dict(num_experts=2, w_stride=9216), -1), (dict(num_experts=2, w_stride=18440), -1),
+    (dict(w_tiled=264), -1), (dict(x_codes=260), -1), (dict(y=257), -1), (dict(out_dtype=3), -2), (dict(w=desc(9)), -1)])
+def test_product_refusals(kw, rc):
+    a = mm_args(**kw)
+    assert _lib.lib().blut_fp4_matmul(C.byref(a), None) == rc
+    assert _lib.lib().blut_fp4_matmul(None, None) == -1
+
+
+def test_python_refusals():
+    x = torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        F.quantize_fp4(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        F.silu_mul_quantize_fp4(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        F.fp4_global_scale(x)
+    with pytest.raises(ValueError, match="kind"):
+        F.FP4Matrix.empty("fp4", 1, 1, "cpu")
+    with pytest.raises(ValueError, match="codes"):
+        F.FP4Matrix.from_checkpoint("nvfp4", torch.zeros(4, 31, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8), 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        F.FP4Matrix.from_checkpoint("nvfp4", torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8), 64)
+    with pytest.raises(ValueError, match="no global scale"):
+        F._given_scale("mxfp4", 1.0, x.device)
+    for g in (0.0, -1.0, float("inf"), float("nan"), 1e-40, torch.ones(2), torch.ones(1, dtype=torch.float64)):
+        with pytest.raises(ValueError, match="global_scale"):
+            F._given_scale("nvfp4", g, x.device)
+    m = F.FP4Matrix.empty("nvfp4", 4, 64, "cpu", torch.ones(1))
+    w = F.FP4Weight("nvfp4", 128, 64, None, torch.zeros(9216, dtype=torch.uint8), 9216, torch.ones(1))
+    ws = F.FP4Weight("nvfp4", 128, 64, 2, torch.zeros(2 * 9216, dtype=torch.uint8), 9216, torch.ones(2))
+    off = torch.zeros(3, dtype=torch.int32)
+    for bad, match in (((F.fp4_matmul, m, ws), "grouped"), ((F.fp4_grouped_matmul, m, w, off), "stack"),
+                       ((F.fp4_grouped_matmul, m, ws, off[:2]), "offsets"), ((F.fp4_grouped_matmul, m, ws, off.long()), "offsets"),
+                       ((F.fp4_matmul, x, w), "FP4Matrix"),
+                       ((F.fp4_matmul, F.FP4Matrix.empty("mxfp4", 4, 64, "cpu"), w), "columns"),
+                       ((F.fp4_matmul, F.FP4Matrix.empty("nvfp4", 4, 65, "cpu"), w), "columns"),
+                       ((F.fp4_matmul, m, w, torch.zeros(4, 127)), "out must"),
+                       ((F.fp4_matmul, m, w, torch.zeros(4, 128, dtype=torch.int32)), "output"),
+                       ((F.fp4_matmul, m, w, torch.zeros(4, 128), torch.bfloat16), "output"),
+                       ((F.fp4_matmul, m, w, torch.zeros(128, 4).t()), "contiguous"),
+                       ((F.fp4_matmul, m, w, torch.zeros(1, 128).expand(4, -1)), "separate")):
+        with pytest.raises(ValueError, match=match):
+            bad[0](*bad[1:])
+    with pytest.raises(ValueError, match="single"):
+        F.FP4Linear(ws)
+    with pytest.raises(ValueError, match="one kind"):
+        F.FP4Weight.from_quantized([])
+    with pytest.raises(ValueError, match="dtype"):
+        F.dequantize_fp4(m, torch.int8)
+
+
+@pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
+def test_restatement(kind):
+    """Every value of the 4-bit form is its own quantisation, and rounding goes to the nearest one."""
+    r = torch.Generator().manual_seed(0)
+    b = R.BLOCK[kind]
+    codes = torch.randint(0, 256, (5, 2 * b), generator=r, dtype=torch.uint8)
+    codes[:, 0::b // 2] = 0x7F  # a 6 in every block fixes its scale (even column -6, odd column 6)
+    scales = torch.randint(20, 100, (5, 4), generator=r, dtype=torch.uint8)
+    v = R.values(codes, scales, kind, 4 * b, 0.5 if kind == "nvfp4" else 1.0)
+    c, s = R.quantize(v, kind, 0.5 if kind == "nvfp4" else 1.0)
+    assert torch.equal(s, scales) and torch.equal(c, codes)
+    x = torch.randn(7, 3 * b + 5, generator=r)
+    g = 0.001 if kind == "nvfp4" else 1.0
+    c, s = R.quantize(x, kind, g)
+    unit = R.values(torch.full_like(c, 0x22), s, kind, x.shape[1], g)  # code 2 is 1: the blocks' units
+    t = (x.double() / unit).abs().clamp(max=6)
+    best = (t[..., None] - R.LEVELS).abs().min(-1).values
+    got = (R.values(c, s, kind, x.shape[1], g) / unit).abs()
+    assert torch.allclose((t - got).abs(), best, rtol=0, atol=1e-12)

@@ -1,0 +1,236 @@
+"""The 4-bit microscaled operators on the GPU against their float64 restatement."""
+import pytest
+import torch
+
+from tests import _fp4_ref as R
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["nvfp4", "mxfp4"]
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def fp4():
+    from block_lut_b200 import fp4 as F
+    return F
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rand(rows, cols, dtype, seed=0, spread=2.0):
+    r = gen(seed)
+    x = torch.randn(rows, cols, generator=r, device="cuda") * torch.exp(spread * torch.randn(rows, cols, generator=r, device="cuda"))
+    return x.to(dtype)
+
+
+def g_of(kind, x, pow2=False):
+    if kind == "mxfp4":
+        return None
+    a = x.double().abs().max().clamp(min=1e-20) / 2688
+    g = torch.exp2(torch.log2(a).ceil()) if pow2 else a * 1.07
+    return g.float().reshape(1)
+
+
+def assert_same_codes(q, ref, what=""):
+    codes, scales = q.to_checkpoint()
+    assert torch.equal(scales, ref[1]), f"{what}: {int((scales != ref[1]).sum())} scales differ"
+    assert torch.equal(codes, ref[0]), f"{what}: {int((codes != ref[0]).sum())} code bytes differ"
+
+
+# --------------------------------------------------------------------- quantisation --
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 16), (1, 1), (3, 15), (8, 33), (9, 127), (17, 128), (5, 129), (2, 500), (7, 513),
+                                       (40, 1408), (1, 2048), (33, 2056)])
+@pytest.mark.parametrize("pow2", [False, True])
+def test_quantize_bits(kind, dtype, rows, cols, pow2):
+    F = fp4()
+    x = rand(rows, cols, dtype, rows * 7 + cols)
+    g = g_of(kind, x, pow2)
+    q = F.quantize_fp4(x, kind, global_scale=g)
+    ref = R.quantize(x, kind, 1.0 if g is None else g)
+    assert_same_codes(q, ref)
+    # the way back is q * s * g, one float32 rounding and one to the output type
+    v = R.values(*ref, kind, cols, 1.0 if g is None else g)
+    for out in DTYPES:
+        assert torch.equal(F.dequantize_fp4(q, out), v.float().to(out))
+    # columns past the matrix are zero in the layout
+    assert int(q.codes.view(-1, rows, 16)[-(-cols // 32):].count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_ties(dtype):
+    """Every border of e2m1 times every e4m3 mantissa, exactly on the border and next to it on both sides."""
+    F = fp4()
+    border = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], device="cuda", dtype=torch.float64)
+    rows = []
+    for m in range(8):
+        s = (1 + m / 8) * 2.0 ** 3
+        row = torch.zeros(16, device="cuda", dtype=torch.float64)
+        row[0] = 6 * s  # its block's maximum: the scale is s for g = 1
+        row[1:8] = border * s
+        row[8:15] = -border * s
+        rows.append(row)
+    x = torch.stack(rows).to(dtype)
+    bits = {2: torch.int16, 4: torch.int32}[x.element_size()]
+    near = []
+    for step in (-1, 0, 1):
+        y = (x.view(bits) + step).view(dtype)
+        y[:, 0], y[:, 15] = x[:, 0], 0
+        near.append(y)
+    x = torch.cat(near)
+    for g in (1.0, 0.25, 3.0, 0.7):
+        gt = torch.tensor([g], device="cuda")
+        assert_same_codes(F.quantize_fp4(x, "nvfp4", global_scale=gt), R.quantize(x, "nvfp4", gt), f"g={g}")
+        assert_same_codes(F.quantize_fp4(x, "nvfp4", global_scale=g), R.quantize(x, "nvfp4", gt), f"g={g}")
+    assert_same_codes(F.quantize_fp4(x, "mxfp4"), R.quantize(x, "mxfp4"))
+
+
+def test_scale_borders():
+    """Block maxima on and next to every border between two e4m3 scales."""
+    F = fp4()
+    t = R.e4m3_values("cuda")
+    mid = ((t[1:] + t[:-1]) / 2 * 6).float()
+    a = torch.cat([(mid.view(torch.int32) + d).view(torch.float32) for d in (-1, 0, 1)])
+    x = torch.zeros(a.numel(), 16, device="cuda")
+    x[:, 3] = a
+    x[:, 5] = -a / 3
+    for g in (1.0, 0.5, 0.3):
+        gt = torch.tensor([g], device="cuda")
+        assert_same_codes(F.quantize_fp4(x * g if g != 0.3 else x, "nvfp4", global_scale=gt),
+                          R.quantize(x * g if g != 0.3 else x, "nvfp4", gt))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_extremes(kind, dtype):
+    F = fp4()
+    fi = torch.finfo(dtype)
+    vals = [0.0, -0.0, fi.max, -fi.max, fi.smallest_normal, fi.smallest_normal / 4, 1.0, 3e-3]
+    x = torch.zeros(len(vals) + 1, 64, device="cuda", dtype=dtype)
+    for i, v in enumerate(vals):
+        x[i, 5] = v
+        x[i, 40:] = v / 3
+    x[-1] = torch.linspace(-1, 1, 64).to(dtype)
+    for g in ([1.0, 2.0 ** -100, 2.0 ** 100] if kind == "nvfp4" else [None]):
+        gt = None if g is None else torch.tensor([g], device="cuda")
+        q = F.quantize_fp4(x, kind, global_scale=gt)
+        assert_same_codes(q, R.quantize(x, kind, 1.0 if g is None else gt), f"g={g}")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_not_finite(kind, dtype):
+    """A block with an infinity or a NaN stands for NaN; its neighbours are untouched."""
+    F = fp4()
+    x = rand(6, 256, dtype, 3, 0.5)
+    x[0, 3], x[1, 40], x[2, 255], x[3, 128] = float("nan"), float("inf"), float("-inf"), float("nan")
+    g = None if kind == "mxfp4" else torch.tensor([0.01], device="cuda")
+    q = F.quantize_fp4(x, kind, global_scale=g)
+    assert_same_codes(q, R.quantize(x, kind, 1.0 if g is None else g))
+    v = F.dequantize_fp4(q, torch.float32)
+    b = R.BLOCK[kind]
+    want = torch.zeros(6, 256, dtype=torch.bool, device="cuda")
+    for r, c in ((0, 3), (1, 40), (2, 255), (3, 128)):
+        want[r, c // b * b: c // b * b + b] = True
+    assert torch.equal(v.isnan(), want) and not v.isinf().any()
+    if kind == "nvfp4":  # the maximum is taken over the finite values
+        f = torch.where(torch.isfinite(x), x, torch.zeros_like(x)).double().abs().max()
+        assert torch.equal(F.fp4_global_scale(x), (f / 2688).float().reshape(1))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_strides_and_gather(kind, dtype):
+    F = fp4()
+    big = rand(70, 3 * 160 + 5, dtype, 5)
+    g = g_of(kind, big)
+    gr = 1.0 if g is None else g
+    for x in (big[:, 160:320], big[::3, 1:200], big[5:6, 3:40], big[:, :32].t(), big[:1].expand(9, -1)[:, :48]):
+        assert_same_codes(F.quantize_fp4(x, kind, global_scale=g), R.quantize(x, kind, gr))
+    x = big[:, 8:200]
+    idx = torch.tensor([3, 3, 69, 0, -1, 70, 1 << 30, -(1 << 31), 12], dtype=torch.int32, device="cuda")
+    want = torch.zeros(9, 192, dtype=dtype, device="cuda")
+    for i, j in enumerate(idx.tolist()):
+        if 0 <= j < 70:
+            want[i] = x[j]
+    assert_same_codes(F.quantize_fp4(x, kind, global_scale=g, row_index=idx), R.quantize(want, kind, gr))
+    assert F.quantize_fp4(x, kind, global_scale=g, row_index=idx[:0]).codes.numel() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 7), (5, 2048), (300, 1400)])
+def test_global_scale(dtype, rows, cols):
+    F = fp4()
+    x = rand(rows, cols, dtype, 11)
+    want = (x.double().abs().max() / 2688).float().reshape(1)  # 53 bits: rounding twice changes nothing
+    assert torch.equal(F.fp4_global_scale(x), want)
+    q = F.quantize_fp4(x)
+    assert torch.equal(q.global_scale, want)
+    assert_same_codes(q, R.quantize(x, "nvfp4", want))
+    assert int(q.to_checkpoint()[1].max()) == 0x7E  # the largest block has the last scale
+    zero = torch.zeros(rows, cols, dtype=dtype, device="cuda")
+    assert float(F.fp4_global_scale(zero)) == 2.0 ** -100
+    assert int(F.quantize_fp4(zero).codes.count_nonzero()) == 0
+    if cols % 2 == 0:
+        h = R.silu_mul(x).abs().max()
+        # expf, the quotient and two products: below 2^-20 of the value
+        assert abs(float(F.fp4_global_scale(x, silu_mul=True)) / float(h / 2688) - 1) < 2.0 ** -20
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 16), (3, 15), (9, 130), (64, 1408), (700, 768)])
+def test_silu_mul_bits(kind, dtype, rows, cols):
+    F = fp4()
+    r = gen(rows + cols)
+    gu = (torch.randn(rows, 2 * cols, generator=r, device="cuda") * 2).to(dtype)
+    h = R.silu_mul(gu)
+    g = g_of(kind, h)
+    assert_same_codes(F.silu_mul_quantize_fp4(gu, kind, global_scale=g), R.quantize(h, kind, 1.0 if g is None else g))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_silu_mul_range(kind):
+    """Gates far from zero on both sides, zeros, ties (up = 0), and what is not finite."""
+    F = fp4()
+    gate = torch.tensor([-300.0, -100, -89, -88, -85, -80, -60, -20, -1, 0, 1, 20, 88, 100, 300, 1e4], device="cuda")
+    up = torch.tensor([0.0, 1, -1, 1e-3, 3e4, 1e20, -1e30, 1e35], device="cuda")
+    rows = []
+    for u in up:
+        for c in range(0, 16, 4):
+            rows.append(torch.cat((gate.roll(c), gate, gate[:4].repeat(8)[:32], u.repeat(64))))
+    for gt in gate:
+        rows.append(torch.cat((gt.repeat(64), up.repeat(8))))
+    gu = torch.stack(rows)
+    h = R.silu_mul(gu)
+    over = h.abs() > torch.finfo(torch.float32).max  # past float32: not finite
+    href = torch.where(over, torch.full_like(h, float("inf")), h)
+    for g in ([1.0, 2.0 ** -90] if kind == "nvfp4" else [None]):
+        gt = None if g is None else torch.tensor([g], device="cuda")
+        assert_same_codes(F.silu_mul_quantize_fp4(gu, kind, global_scale=gt), R.quantize(href, kind, 1.0 if g is None else gt))
+    gu[0, 3], gu[1, 70], gu[2, 5] = float("nan"), float("inf"), float("inf")
+    gt = None if kind == "mxfp4" else torch.tensor([1.0], device="cuda")
+    s = F.silu_mul_quantize_fp4(gu, kind, global_scale=gt).to_checkpoint()[1]
+    nan = 127 if kind == "nvfp4" else 255
+    b = R.BLOCK[kind]
+    assert s[0, 3 // b] == nan and s[1, 6 // b] == nan and s[2, 5 // b] == nan
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_checkpoint_round_trip(kind):
+    F = fp4()
+    for rows, cols in ((1, 5), (130, 200), (33, 1408)):
+        x = rand(rows, cols, torch.bfloat16, 9)
+        g = g_of(kind, x)
+        ref = R.quantize(x, kind, 1.0 if g is None else g)
+        codes, scales = ref
+        m = F.FP4Matrix.from_checkpoint(kind, codes, scales, cols, global_scale=g)
+        assert_same_codes(m, ref)
+        q = F.quantize_fp4(x, kind, global_scale=g)
+        assert torch.equal(m.codes, q.codes) and torch.equal(m.scales, q.scales)
+        if kind == "nvfp4":
+            f8 = F.FP4Matrix.from_checkpoint(kind, codes, scales.view(torch.float8_e4m3fn), cols, global_scale=g)
+            assert torch.equal(f8.scales, q.scales)

@@ -1,0 +1,255 @@
+"""Products of 4-bit microscaled matrices on the GPU against float64."""
+import pytest
+import torch
+
+from tests import _fp4_ref as R
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["nvfp4", "mxfp4"]
+
+
+def fp4():
+    from block_lut_b200 import fp4 as F
+    return F
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def operand(rows, cols, kind, seed, scale=1.0):
+    """Quantised rows and the float64 values they stand for."""
+    F = fp4()
+    x = torch.randn(rows, cols, generator=gen(seed), device="cuda") * scale
+    q = F.quantize_fp4(x, kind)
+    g = 1.0 if q.global_scale is None else q.global_scale
+    return q, R.values(*R.quantize(x, kind, g), kind, cols, g)
+
+
+def check(y, x, w, what=""):
+    ref, tol = R.product_bound(x, w, y.dtype)
+    d = (y.double() - ref).abs()
+    assert torch.isfinite(y).all() and (d <= tol).all(), f"{what}: off by up to {float((d / tol).max()):.3g} of the bound"
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 1, 16), (5, 130, 200), (16, 128, 64), (17, 256, 1408), (32, 640, 2048),
+                                   (33, 129, 256), (64, 384, 500), (65, 128, 2048), (128, 200, 1024), (129, 300, 640),
+                                   (192, 128, 128), (193, 257, 2048), (500, 640, 1408), (1000, 1000, 1000)])
+def test_matmul(kind, m, n, k):
+    F = fp4()
+    xq, x = operand(m, k, kind, 1)
+    wq, w = operand(n, k, kind, 2, 0.05)
+    W = F.FP4Weight.from_quantized(wq)
+    y = F.fp4_matmul(xq, W, out_dtype=torch.float32)
+    check(y, x, w, "float32")
+    check(F.fp4_matmul(xq, W), x, w, "bfloat16")
+    check(F.fp4_matmul(xq, W, out_dtype=torch.float16), x, w, "float16")
+    assert torch.equal(y, F.fp4_matmul(xq, W, out_dtype=torch.float32))  # the same bits every time
+    F.fp4_check_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_every_element_has_its_place(kind):
+    """One nonzero weight column and one nonzero token at a time would take long; a rank-one pattern of distinct
+    powers shows a swapped row, token, block or half just as well."""
+    F = fp4()
+    for m, n, k in ((40, 256, 384), (200, 128, 256)):
+        xv = torch.zeros(m, k, device="cuda")
+        for t in range(m):
+            xv[t, (t * 37) % k] = [1.0, 2.0, 3.0, 4.0, 6.0][t % 5]
+        wv = torch.zeros(n, k, device="cuda")
+        r = torch.arange(n, device="cuda")[:, None]
+        c = torch.arange(k, device="cuda")[None]
+        lv = R.LEVELS.float().cuda()
+        wv = lv[(r * 5 + c * 3) % 8] * torch.where((r + c) % 3 == 0, -1.0, 1.0) * torch.exp2(((r + c // 32) % 5).float())
+        g = None if kind == "mxfp4" else 1.0
+        xq, wq = F.quantize_fp4(xv, kind, global_scale=g), F.quantize_fp4(wv, kind, global_scale=g)
+        x = F.dequantize_fp4(xq, torch.float32).double()
+        w = F.dequantize_fp4(wq, torch.float32).double()
+        y = F.fp4_matmul(xq, F.FP4Weight.from_quantized(wq), out_dtype=torch.float32)
+        assert torch.equal(y.double(), x @ w.T)  # single products: exact
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_not_finite_blocks_stay_in_their_rows(kind):
+    F = fp4()
+    x = torch.randn(40, 256, generator=gen(0), device="cuda")
+    w = torch.randn(200, 256, generator=gen(1), device="cuda")
+    clean = F.fp4_matmul(F.quantize_fp4(x, kind, 0.01 if kind == "nvfp4" else None),
+                         F.FP4Weight.from_quantized(F.quantize_fp4(w, kind, 0.01 if kind == "nvfp4" else None)))
+    x[7, 100], w[130, 5] = float("nan"), float("inf")
+    y = F.fp4_matmul(F.quantize_fp4(x, kind, 0.01 if kind == "nvfp4" else None),
+                     F.FP4Weight.from_quantized(F.quantize_fp4(w, kind, 0.01 if kind == "nvfp4" else None)))
+    bad = torch.zeros(40, 200, dtype=torch.bool, device="cuda")
+    bad[7], bad[:, 130] = True, True
+    assert torch.equal(y.isnan(), bad)
+    assert torch.equal(y[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_output_pitch(kind):
+    F = fp4()
+    xq, x = operand(21, 256, kind, 1)
+    wq, w = operand(200, 256, kind, 2)
+    W = F.FP4Weight.from_quantized(wq)
+    big = torch.full((21, 333), 7.0, device="cuda", dtype=torch.bfloat16)
+    y = F.fp4_matmul(xq, W, out=big[:, 11:211])
+    assert y.data_ptr() == big[:, 11:211].data_ptr()
+    check(y, x, w)
+    assert (big[:, :11] == 7).all() and (big[:, 211:] == 7).all()
+    assert F.fp4_matmul(F.quantize_fp4(torch.zeros(0, 256, device="cuda"), kind), W).shape == (0, 200)
+
+
+def runs_case(E, counts, lead, tail, n, k, kind, seed=0):
+    F = fp4()
+    m = lead + sum(counts) + tail
+    xq, x = operand(m, k, kind, seed)
+    ws = [operand(n, k, kind, 100 + seed * 1000 + e, 0.05 * (1 + e % 3)) for e in range(E)]
+    off = torch.tensor([lead] + [lead + sum(counts[: e + 1]) for e in range(E)], dtype=torch.int32, device="cuda")
+    return m, xq, x, F.FP4Weight.from_quantized([q for q, _ in ws]), [w for _, w in ws], off
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("counts,lead,tail", [
+    ([1], 0, 0), ([0, 0, 5, 0], 0, 0), ([3, 0, 1, 40, 0, 33], 2, 7), ([0] * 7, 0, 9), ([200, 1, 0, 65], 1, 1),
+    ([1] * 8 + [0] * 120, 0, 0), ([2, 0, 1] * 43, 3, 64), ([300, 300, 5], 0, 0), ([0, 700, 0, 1], 17, 0), ([90, 100, 80], 0, 3)])
+def test_grouped(kind, counts, lead, tail):
+    F = fp4()
+    n, k = 200, 384
+    E = len(counts)
+    m, xq, x, W, ws, off = runs_case(E, counts, lead, tail, n, k, kind)
+    for dt in (torch.bfloat16, torch.float32):
+        out = torch.full((m, n), 7.0, device="cuda", dtype=dt)
+        y = F.fp4_grouped_matmul(xq, W, off, out=out)
+        assert y.data_ptr() == out.data_ptr()
+        at = off.tolist()
+        for e in range(E):
+            if at[e + 1] > at[e]:
+                check(y[at[e]:at[e + 1]], x[at[e]:at[e + 1]], ws[e], f"run {e}")
+        assert (y[:lead] == 7).all() and (y[m - tail:] == 7).all()
+    again = F.fp4_grouped_matmul(xq, W, off, out=torch.full_like(out, 7.0))
+    assert torch.equal(again, out)
+    F.fp4_check_status()
+
+
+def test_grouped_many_experts():
+    F = fp4()
+    counts = [(e * 7) % 4 for e in range(300)]
+    m, xq, x, W, ws, off = runs_case(300, counts, 0, 0, 128, 128, "nvfp4")
+    y = F.fp4_grouped_matmul(xq, W, off, out_dtype=torch.float32)
+    at = off.tolist()
+    for e in range(300):
+        if counts[e]:
+            check(y[at[e]:at[e + 1]], x[at[e]:at[e + 1]], ws[e], f"run {e}")
+
+
+def test_offsets_stay_in_the_buffer():
+    """Offsets outside [0, rows] are clamped by the kernel: no row outside the buffers is read or written."""
+    F = fp4()
+    m, xq, x, W, ws, off = runs_case(3, [4, 5, 6], 0, 0, 130, 128, "nvfp4")
+    guard = torch.full((m + 8, 130), 7.0, device="cuda", dtype=torch.float32)
+    out = guard[4:4 + m]
+    F.fp4_grouped_matmul(xq, W, torch.tensor([-5, 4, 9, 1 << 30], dtype=torch.int32, device="cuda"), out=out)
+    check(out[:4], x[:4], ws[0])
+    check(out[4:9], x[4:9], ws[1])
+    check(out[9:], x[9:], ws[2])
+    assert (guard[:4] == 7).all() and (guard[4 + m:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear(kind, dtype):
+    F = fp4()
+    w = torch.randn(300, 500, generator=gen(5), device="cuda") * 0.05
+    W = F.FP4Weight.quantize(w, kind)
+    gw = 1.0 if W.global_scale is None else W.global_scale
+    wv = R.values(*R.quantize(w, kind, gw), kind, 500, gw)
+    for shape, scale in (((3, 500), None), ((2, 5, 500), 0.004), ((500,), None), ((0, 500), None), ((1, 1, 500), 0.01)):
+        x = torch.randn(*shape, generator=gen(6), device="cuda").to(dtype)
+        lin = F.FP4Linear(W, None if kind == "mxfp4" else scale)
+        y = lin(x)
+        assert y.shape == x.shape[:-1] + (300,) and y.dtype == dtype
+        x2 = x.reshape(-1, 500)
+        if x2.shape[0]:
+            g = 1.0 if kind == "mxfp4" else torch.tensor([scale], device="cuda") if scale else (x2.double().abs().max() / 2688).float()
+            check(y.reshape(-1, 300), R.values(*R.quantize(x2, kind, g), kind, 500, g), wv)
+            out = torch.empty_like(y)
+            assert lin(x, out=out) is out and torch.equal(out, y)
+
+
+def test_streams_and_graphs():
+    """A side stream, and two captured graphs replayed beside each other and beside eager calls: no shared state."""
+    F = fp4()
+    xq, x = operand(24, 2048, "nvfp4", 1)
+    wq, w = operand(640, 2048, "nvfp4", 2)
+    W = F.FP4Weight.from_quantized(wq)
+    want = F.fp4_matmul(xq, W)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    y = F.fp4_matmul(xq, W, stream=s)
+    s.synchronize()
+    assert torch.equal(y, want)
+    lin = F.FP4Linear(W)
+    xs = [torch.randn(24, 2048, generator=gen(i), device="cuda").bfloat16() for i in range(2)]
+    want = [lin(v) for v in xs]
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for v in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(lin(v))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+        graphs[1].replay()
+        eager = lin(xs[0])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[0])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_expert_layer(kind):
+    """The operators as a layer of routed experts runs them: gather + quantise, gate/up, SiLU + quantise, down.  Each
+    step is held to its own bound on the rows that the step before it gave."""
+    F = fp4()
+    T, k, E, H, I = 37, 2, 6, 256, 200
+    r = gen(8)
+    x = torch.randn(T, H, generator=r, device="cuda").bfloat16()
+    ids = torch.rand(T, E, generator=r, device="cuda").topk(k).indices
+    order = ids.flatten().argsort(stable=True)
+    off = torch.searchsorted(ids.flatten()[order].contiguous(), torch.arange(E + 1, device="cuda")).int()
+    w13 = torch.randn(E, 2 * I, H, generator=r, device="cuda") * 0.08
+    w2 = torch.randn(E, H, I, generator=r, device="cuda") * 0.08
+    W13, W2 = F.FP4Weight.quantize(w13, kind), F.FP4Weight.quantize(w2, kind)
+    tok = (order // k).int()
+    xq = F.quantize_fp4(x, kind, row_index=tok)
+    gx = 1.0 if kind == "mxfp4" else xq.global_scale
+    gu = F.fp4_grouped_matmul(xq, W13, off)
+    hq = F.silu_mul_quantize_fp4(gu, kind)
+    y = F.fp4_grouped_matmul(hq, W2, off, out_dtype=torch.float32)
+    xv = R.values(*R.quantize(x[tok.long()], kind, gx), kind, H, gx)
+    gh = 1.0 if kind == "mxfp4" else hq.global_scale
+    hv = R.values(*R.quantize(R.silu_mul(gu), kind, gh), kind, I, gh)
+    at = off.tolist()
+    for e in range(E):
+        lo, hi = at[e], at[e + 1]
+        if hi == lo:
+            continue
+        g13 = 1.0 if kind == "mxfp4" else W13.global_scale[e]
+        g2 = 1.0 if kind == "mxfp4" else W2.global_scale[e]
+        check(gu[lo:hi], xv[lo:hi], R.values(*R.quantize(w13[e], kind, g13), kind, H, g13))
+        check(y[lo:hi], hv[lo:hi], R.values(*R.quantize(w2[e], kind, g2), kind, I, g2))
+    # the layer's result is near the unquantised one: 4-bit noise, not a wrong expert
+    full = torch.zeros(T * k, H, dtype=torch.float64, device="cuda")
+    for i, (t, e) in enumerate(zip(tok.tolist(), ids.flatten()[order].tolist())):
+        full[i] = R.silu_mul(x[t].double() @ w13[e].double().T) @ w2[e].double().T
+    # noise of a 4-bit value: at most a quarter of it between two levels, in rms about 0.1; five such factors
+    # (x twice through the product of gate and up, two weights, h) stay below 0.5 of the result in the 2-norm
+    assert float((y.double() - full).norm() / full.norm()) < 0.5
