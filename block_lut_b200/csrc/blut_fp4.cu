@@ -14,9 +14,14 @@
 // compared with x in float64, in which border * s * g (2 + 4 + 24 bits) is
 // exact.  Borders are met often when g is a power of two (0.8 % of bf16
 // values are ties) and cost a few instructions each.  silu(gate) * up is
-// rounded once, to its code: it is computed in float32 (relative error below
-// 2^-20, window 2^-18); a block with a value near a border is done again in
-// float64 (about 1 block in 2000).
+// rounded once, to its code: it is computed in float32 from the hardware's
+// approximate exponential and reciprocal (relative error below 2^-18, window
+// 2^-17); a block with a value near a border is done again in float64, a
+// column a lane (about 1 block in 3000).
+//
+// All kernels here are bound by instructions before they are bound by memory,
+// so a warp takes several rows of one 512-column stretch: their loads are in
+// flight together and the address arithmetic is shared.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -25,10 +30,10 @@
 namespace blut {
 namespace {
 
-constexpr int kQRows = 8;      // rows per CTA, a warp each
+constexpr int kQWarps = 8;
 constexpr int kQCols = 512;    // columns per CTA, 16 per lane
 constexpr int kQChunks = kQCols / 32;
-constexpr int kQPitch = kQRows * 16 + 16;  // bytes of a staged chunk: 16 more than its rows, against bank conflicts
+constexpr float kSiluWin = 0x1p-17f;  // twice the error of a float32 silu(gate) * up / (s g)
 constexpr float kMinGlobal = 7.888609052210118e-31f;  // 2^-100
 
 template <int DT>
@@ -52,38 +57,29 @@ struct Elem<BLUT_F32> {
   static __device__ __forceinline__ float from(float v) { return v; }
 };
 
-// 16 consecutive values of a row, zeros past the n valid ones.  kVec: the
-// address of every such run is a multiple of 16 bytes.
-template <int DT, bool kVec>
+// 16 consecutive values of a row, zeros past the n valid ones.
+template <int DT>
 __device__ __forceinline__ void load16(const typename Elem<DT>::T* p, int n, float (&v)[16]) {
-  if (kVec && n >= 16) {
-    if constexpr (DT == BLUT_F32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p) + i);
-        v[4 * i] = a.x, v[4 * i + 1] = a.y, v[4 * i + 2] = a.z, v[4 * i + 3] = a.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[8 * i + 2 * j] = Elem<DT>::f((uint16_t)(w[j] & 0xFFFFu));
-          v[8 * i + 2 * j + 1] = Elem<DT>::f((uint16_t)(w[j] >> 16));
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = i < n ? Elem<DT>::f(p[i]) : 0.0f;
-  }
+  for (int i = 0; i < 16; ++i) v[i] = i < n ? Elem<DT>::f(p[i]) : 0.0f;
 }
 
-// silu(g) * u in float32, relative error below 2^-20 for g >= -80.
-__device__ __forceinline__ float silu_mul_f32(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
+// silu(g) * u in float32 for g >= -80: the exponent's rounding costs at most
+// 2^-18.5 (at g = -80), ex2 and rcp 2^-22 each, three products 2^-24 each.
+__device__ __forceinline__ float silu_mul_f32(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
 __device__ __forceinline__ double silu_mul_f64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
+
+// max(a, |b|, |c|); NaN if one of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
+}
 
 // Border between e2m1 codes c and c + 1 (c = 0 .. 6).
 __device__ __forceinline__ float e2m1_border(uint32_t c) {
@@ -113,12 +109,14 @@ __device__ __forceinline__ uint32_t e4m3_scale(double a, float g, float t) {
 
 // The scale byte and the 16 codes of this lane's columns.  A block is one
 // lane (nvfp4) or two neighbouring lanes (mxfp4).  v: the values; kSilu:
-// float32 approximations whose exact forms exact(j) gives.
-template <bool kMX, bool kSilu, class Exact>
-__device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool unsure, uint32_t& sbyte, Exact exact) {
-  uint32_t top = 0;
+// float32 approximations, and `unsure` is raised for a block that a more
+// exact form could change.
+template <bool kMX, bool kSilu>
+__device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool& unsure, uint32_t& sbyte) {
+  float most = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < 16; i += 2) most = max3_abs(most, v[i], v[i + 1]);
+  uint32_t top = __float_as_uint(most) & 0x7FFFFFFFu;  // bits of non-negative floats order as integers, NaN last
   if (kMX) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
   const bool bad = top >= 0x7F800000u;  // an infinity or a NaN: the block has no scale
   const float a = __uint_as_float(top);
@@ -128,14 +126,13 @@ __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool un
     sbyte = e > 2 ? (uint32_t)(e - 2) : 0u;
     r = __uint_as_float((254u - sbyte) << 23);
     if (kSilu) {  // near a power of two, or where float32 has lost digits
-      unsure |= (__float_as_uint(a * (1.0f + 0x1p-18f)) >> 23) != (__float_as_uint(a * (1.0f - 0x1p-18f)) >> 23);
+      unsure |= (__float_as_uint(a * (1.0f + kSiluWin)) >> 23) != (__float_as_uint(a * (1.0f - kSiluWin)) >> 23);
       unsure |= a < 0x1p-100f && top != 0;
-      unsure |= __shfl_xor_sync(0xFFFFFFFFu, unsure ? 1 : 0, 1) != 0;
     }
   } else {
     const float t = a * __frcp_rn(6.0f * g);
     if (kSilu) {
-      const uint32_t both = e4m3x2_sat(t * (1.0f + 0x1p-18f), t * (1.0f - 0x1p-18f));
+      const uint32_t both = e4m3x2_sat(t * (1.0f + kSiluWin), t * (1.0f - kSiluWin));
       sbyte = both & 0xFFu;
       unsure |= sbyte != both >> 8;
     } else {
@@ -151,7 +148,7 @@ __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool un
     for (int i = 0; i < 16; ++i) w[i] = v[i] * r;
     c = make_uint2(e2m1x8(w), e2m1x8(w + 8));
   } else {
-    constexpr float kWin = kSilu ? 0x1p-18f : 0x1p-21f;
+    constexpr float kWin = kSilu ? kSiluWin : 0x1p-21f;
     const float ru = r * (1.0f + kWin), rd = r * (1.0f - kWin);
     float w[16];
 #pragma unroll
@@ -175,36 +172,11 @@ __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool un
       }
     } else {
       unsure |= (d0 | d1) != 0;
-      if (kMX) unsure |= __shfl_xor_sync(0xFFFFFFFFu, unsure ? 1 : 0, 1) != 0;
-      if (unsure && !bad) {  // mxfp4: both lanes of the block or neither
-        double m = 0.0;
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i) m = fmax(m, fabs(exact(i)));
-        double un;
-        if constexpr (kMX) {
-          m = fmax(m, __shfl_xor_sync(3u << (threadIdx.x & 30u), m, 1));
-          const int e = m > 0.0 ? ilogb(m) - 2 : -127;
-          sbyte = (uint32_t)(min(max(e, -127), 127) + 127);
-          un = ldexp(1.0, (int)sbyte - 127);
-        } else {
-          sbyte = e4m3_scale(m, g, (float)(m / (6.0 * (double)g)));
-          un = (double)e4m3_f32(sbyte) * (double)g;
-        }
-        c = make_uint2(0, 0);
-#pragma unroll 1
-        for (int i = 0; i < 16; ++i) {
-          const double x = exact(i);
-          uint32_t q = 0;
-#pragma unroll 1
-          for (uint32_t k = 0; k < 7 && q == k && un > 0.0; ++k) q = e2m1_decide(fabs(x), un, k);
-          q |= signbit(x) ? 8u : 0u;
-          if (i < 8)
-            c.x |= q << (4 * i);
-          else
-            c.y |= q << (4 * (i - 8));
-        }
-      }
     }
+  }
+  if (kSilu) {
+    unsure = unsure && !bad;
+    if (kMX) unsure |= __shfl_xor_sync(0xFFFFFFFFu, unsure ? 1 : 0, 1) != 0;
   }
   if (bad) {
     sbyte = kMX ? 0xFFu : 0x7Fu;
@@ -213,71 +185,183 @@ __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool un
   return c;
 }
 
-// x [rows][ld] -> FP4 layout.  A warp takes one row and 512 columns; codes
-// and scales go through shared memory, so that each store to a chunk covers
-// 8 rows.  Bound by memory: rows * cols * (2 B in, 0.5 + 1/16 or 1/32 B out).
-template <int DT, bool kMX, bool kSilu, bool kVec>
-__global__ void __launch_bounds__(32 * kQRows)
+// Block `block` (16 or 32 columns from column c0 of a row of gate and up) of
+// silu(gate) * up in float64: one column a lane, the whole warp.  The lanes
+// that hold the block's codes get them and the scale.
+template <int DT, bool kMX>
+__device__ __noinline__ void encode_block_f64(const typename Elem<DT>::T* row, int cols, int c0, float g, int owner,
+                                              uint2& c, uint32_t& sbyte) {
+  const int lane = threadIdx.x & 31;
+  double x = 0.0;
+  if (lane < (kMX ? 32 : 16) && c0 + lane < cols)
+    x = silu_mul_f64((double)Elem<DT>::f(row[c0 + lane]), (double)Elem<DT>::f(row[cols + c0 + lane]));
+  double m = fabs(x);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmax(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+  uint32_t s;
+  double unit;
+  if constexpr (kMX) {
+    s = m > 0.0 ? (uint32_t)(min(max(ilogb(m) - 2, -127), 127) + 127) : 0u;
+    unit = ldexp(1.0, (int)s - 127);
+  } else {
+    s = e4m3_scale(m, g, (float)(m / (6.0 * (double)g)));
+    unit = (double)e4m3_f32(s) * (double)g;
+  }
+  uint32_t q = 0;
+#pragma unroll
+  for (uint32_t k = 0; k < 7; ++k)
+    if (unit > 0.0 && q == k) q = e2m1_decide(fabs(x), unit, k);
+  q |= signbit(x) ? 8u : 0u;
+  q <<= 4 * (lane & 7);  // eight lanes make a word
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) q |= __shfl_xor_sync(0xFFFFFFFFu, q, d);
+  const int from = kMX ? 16 * (lane & 1) : 0;  // mxfp4: the odd lane holds columns 16 .. 31
+  const uint2 w = make_uint2(__shfl_sync(0xFFFFFFFFu, q, from), __shfl_sync(0xFFFFFFFFu, q, from + 8));
+  if (kMX ? (lane | 1) == (owner | 1) : lane == owner) c = w, sbyte = s;
+}
+
+// 16 values of a row as they are in memory.  kVec: the boundary in bytes that
+// every such run starts on (32 or 16), or 0 for any other.
+template <int DT>
+struct Raw {
+  static constexpr int kN = DT == BLUT_F32 ? 4 : 2;
+  uint4 w[kN];
+};
+template <int DT, int kVec>
+__device__ __forceinline__ void raw_load(const typename Elem<DT>::T* p, Raw<DT>& r) {
+  if constexpr (kVec == 16) {
+#pragma unroll
+    for (int i = 0; i < Raw<DT>::kN; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Raw<DT>::kN; i += 2)
+      asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+          : "=r"(r.w[i].x), "=r"(r.w[i].y), "=r"(r.w[i].z), "=r"(r.w[i].w), "=r"(r.w[i + 1].x), "=r"(r.w[i + 1].y),
+            "=r"(r.w[i + 1].z), "=r"(r.w[i + 1].w)
+          : "l"(reinterpret_cast<const uint4*>(p) + i));
+  }
+}
+template <int DT>
+__device__ __forceinline__ void raw_unpack(const Raw<DT>& r, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < Raw<DT>::kN; ++i) {
+    const uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == BLUT_F32) {
+        v[4 * i + j] = __uint_as_float(w[j]);
+      } else if constexpr (DT == BLUT_BF16) {
+        v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+        v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[8 * i + 2 * j] = f.x;
+        v[8 * i + 2 * j + 1] = f.y;
+      }
+    }
+  }
+}
+
+// Bytes of a staged chunk: 16 more than its rows, against bank conflicts.
+__host__ __device__ constexpr int q_pitch(int rows) { return rows * 16 + 16; }
+
+// x [rows][ld] -> FP4 layout.  A warp takes kPer rows of one 512-column
+// stretch, 16 columns a lane; codes and scales go through shared memory, so
+// that each store to a chunk covers all the CTA's rows.  The rows are taken
+// from the last to the first: what was written last (x by the layer before,
+// or what blut_fp4_global_scale read last) is what the L2 still holds.
+template <int DT, bool kMX, bool kSilu, int kVec, int kPer>
+__global__ void __launch_bounds__(32 * kQWarps, kPer > 1 ? 4 : 1)
     fp4_quantize_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t ld, const int32_t* __restrict__ row_index,
                         int64_t src_rows, const float* __restrict__ gptr, int64_t rows, int cols, int kp,
-                        uint8_t* __restrict__ codes, uint32_t* __restrict__ scales) {
-  __shared__ alignas(16) uint8_t sc[kQChunks * kQPitch];
-  __shared__ uint32_t ss[kQCols / 64][kQRows];
+                        uint8_t* __restrict__ codes, uint32_t* __restrict__ scales, int signal) {
+  // the product that follows in the same call may start its weight copies
+  if (signal) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int kRows = kQWarps * kPer, kPitch = q_pitch(kRows);
+  constexpr int kWordCols = kMX ? 128 : 64, kWords = kQCols / kWordCols;
+  __shared__ alignas(16) uint8_t sc[kQChunks * kPitch];
+  __shared__ uint32_t ss[kWords * kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row0 = (int64_t)blockIdx.x * kQRows, row = row0 + warp;
+  const int64_t row0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * kRows;
   const int col0 = blockIdx.y * kQCols, col = col0 + 16 * lane;
   const int n = min(16, max(0, cols - col));
   const float g = kMX ? 1.0f : __ldg(gptr);
-  int64_t src = row < rows ? row : -1;
-  if (row_index && src >= 0) {
-    src = row_index[row];
-    if (src >= src_rows) src = -1;
-  }
-  float v[16];
-  bool unsure = false;
-  const typename Elem<DT>::T* p = x + (src < 0 ? 0 : src) * ld + col;
-  if (src < 0 || n == 0) {
+  const typename Elem<DT>::T* p[kPer];  // null: no row, or no columns
+  Raw<DT> raw[kPer], raw_up[kSilu ? kPer : 1];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-  } else if constexpr (kSilu) {
-    float u[16];
-    load16<DT, kVec>(p, n, v);
-    load16<DT, kVec>(p + cols, n, u);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      unsure |= v[i] < -80.0f;  // exp(-gate) nears the end of float32
-      v[i] = silu_mul_f32(v[i], u[i]);
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t row = row0 + warp + kQWarps * i;
+    int64_t src = row < rows ? row : -1;
+    if (row_index && src >= 0) {
+      src = row_index[row];
+      if (src >= src_rows) src = -1;
     }
-  } else {
-    load16<DT, kVec>(p, n, v);
+    p[i] = src < 0 || n == 0 ? nullptr : x + src * ld + col;
+    if (kVec && n == 16 && p[i]) {
+      raw_load<DT, kVec>(p[i], raw[i]);
+      if constexpr (kSilu) raw_load<DT, kVec>(p[i] + cols, raw_up[i]);
+    }
   }
-  uint32_t sbyte;
-  const uint2 c = encode16<kMX, kSilu>(v, g, unsure, sbyte, [&](int i) {
-    if (src < 0 || i >= n) return 0.0;
-    return silu_mul_f64((double)Elem<DT>::f(p[i]), (double)Elem<DT>::f(p[cols + i]));
-  });
-  *reinterpret_cast<uint2*>(sc + (lane >> 1) * kQPitch + warp * 16 + (lane & 1) * 8) = c;
-  {
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    float v[16];
+    bool unsure = false;
+    if (!p[i]) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+    } else {
+      if (kVec && n == 16)
+        raw_unpack<DT>(raw[i], v);
+      else
+        load16<DT>(p[i], n, v);
+      if constexpr (kSilu) {
+        float u[16], least = 0.0f;
+        if (kVec && n == 16)
+          raw_unpack<DT>(raw_up[i], u);
+        else
+          load16<DT>(p[i] + cols, n, u);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          least = fminf(least, v[j]);
+          v[j] = silu_mul_f32(v[j], u[j]);
+        }
+        unsure = least < -80.0f;  // exp(-gate) nears the end of float32
+      }
+    }
+    uint32_t sbyte;
+    uint2 c = encode16<kMX, kSilu>(v, g, unsure, sbyte);
+    const int r = warp + kQWarps * i;
+    if constexpr (kSilu) {
+      for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, unsure); todo;) {
+        const int owner = __ffs(todo) - 1;
+        todo &= ~((kMX ? 3u : 1u) << owner);  // mxfp4: both lanes of a block are marked, the even one comes first
+        encode_block_f64<DT, kMX>(x + (row0 + r) * ld, cols, col0 + 16 * owner, g, owner, c, sbyte);
+      }
+    }
+    *reinterpret_cast<uint2*>(sc + (lane >> 1) * kPitch + r * 16 + (lane & 1) * 8) = c;
     uint8_t* s8 = reinterpret_cast<uint8_t*>(ss);
     if (kMX) {
-      if ((lane & 1) == 0) s8[((lane >> 3) * kQRows + warp) * 4 + ((lane >> 1) & 3)] = (uint8_t)sbyte;
+      if ((lane & 1) == 0) s8[((lane >> 3) * kRows + r) * 4 + ((lane >> 1) & 3)] = (uint8_t)sbyte;
     } else {
-      s8[((lane >> 2) * kQRows + warp) * 4 + (lane & 3)] = (uint8_t)sbyte;
+      s8[((lane >> 2) * kRows + r) * 4 + (lane & 3)] = (uint8_t)sbyte;
     }
   }
   __syncthreads();
-  const int t = threadIdx.x, r = t & (kQRows - 1);
-  if (row0 + r >= rows) return;
-  const int ch = t >> 3;  // 32 threads' worth of chunks: 16 chunks x 8 rows use half the threads
-  if (t < kQChunks * kQRows) {
-    if (col0 + 32 * ch < kp)
-      *reinterpret_cast<uint4*>(codes + (((int64_t)(col0 / 32) + ch) * rows + row0 + r) * 16) =
-          *reinterpret_cast<const uint4*>(sc + ch * kQPitch + r * 16);
-  } else {
-    constexpr int kWordCols = kMX ? 128 : 64;
-    const int w = ch - kQChunks;
-    if (w < kQCols / kWordCols && col0 + kWordCols * w < kp)
-      scales[((int64_t)(col0 / kWordCols) + w) * rows + row0 + r] = ss[w][r];
+  const int left = (int)min((int64_t)kRows, rows - row0);
+  uint8_t* dst = codes + ((int64_t)(col0 / 32) * rows + row0) * 16;
+  const int nch = min(kQChunks, (kp - col0) / 32);
+#pragma unroll
+  for (int t = threadIdx.x; t < kQChunks * kRows; t += 32 * kQWarps) {
+    const int ch = t / kRows, r = t % kRows;
+    if (ch < nch && r < left)
+      *reinterpret_cast<uint4*>(dst + ((int64_t)ch * rows + r) * 16) =
+          *reinterpret_cast<const uint4*>(sc + ch * kPitch + r * 16);
+  }
+  uint32_t* sdst = scales + (int64_t)(col0 / kWordCols) * rows + row0;
+#pragma unroll
+  for (int t = threadIdx.x; t < kWords * kRows; t += 32 * kQWarps) {
+    const int w = t / kRows, r = t % kRows;
+    if (w * kWordCols < kp - col0 && r < left) sdst[(int64_t)w * rows + r] = ss[t];
   }
 }
 
@@ -285,29 +369,62 @@ __global__ void __launch_bounds__(32 * kQRows)
 // block's scale is 448.  out[0]: g, out[1] and out[2]: the running maximum's
 // bits and the CTAs that are done (zeroed before the launch).  The maximum
 // does not depend on the order of the atomics.
-template <int DT, bool kSilu, bool kVec>
+template <int DT, bool kSilu, int kVec>
 __global__ void __launch_bounds__(256)
     fp4_global_scale_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t ld, int64_t rows, int cols,
                             float* out) {
+  constexpr int kDepth = 2;  // stretches of 16 columns in flight
   const int per_row = (cols + 15) / 16;
-  const int64_t total = rows * per_row;
+  const int64_t stride = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t srow = stride / per_row;
+  const int scol = (int)(stride - srow * per_row);
+  int64_t row = first / per_row;
+  int c = (int)(first - row * per_row);
   uint32_t top = 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / per_row;
-    const int col = (int)(i - row * per_row) * 16, n = min(16, cols - col);
-    const typename Elem<DT>::T* p = x + row * ld + col;
-    float v[16];
-    load16<DT, kVec>(p, n, v);
-    if constexpr (kSilu) {
-      float u[16];
-      load16<DT, kVec>(p + cols, n, u);
+  while (row < rows) {
+    Raw<DT> raw[kDepth], raw_up[kSilu ? kDepth : 1];
+    const typename Elem<DT>::T* p[kDepth];
+    int n[kDepth];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = silu_mul_f32(v[j], u[j]);
+    for (int i = 0; i < kDepth; ++i) {
+      n[i] = row < rows ? min(16, cols - 16 * c) : 0;
+      p[i] = x + row * ld + 16 * c;
+      if (kVec && n[i] == 16) {
+        raw_load<DT, kVec>(p[i], raw[i]);
+        if constexpr (kSilu) raw_load<DT, kVec>(p[i] + cols, raw_up[i]);
+      }
+      row += srow, c += scol;
+      if (c >= per_row) c -= per_row, ++row;
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-      top = max(top, b < 0x7F800000u ? b : 0u);
+    for (int i = 0; i < kDepth; ++i) {
+      if (!n[i]) continue;
+      float v[16];
+      if (kVec && n[i] == 16)
+        raw_unpack<DT>(raw[i], v);
+      else
+        load16<DT>(p[i], n[i], v);
+      if constexpr (kSilu) {
+        float u[16];
+        if (kVec && n[i] == 16)
+          raw_unpack<DT>(raw_up[i], u);
+        else
+          load16<DT>(p[i] + cols, n[i], u);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = silu_mul_f32(v[j], u[j]);
+      }
+      float most = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) most = max3_abs(most, v[j], v[j + 1]);
+      if (__float_as_uint(most) < 0x7F800000u) {
+        top = max(top, __float_as_uint(most));
+      } else {  // something is not finite: value by value
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+          top = max(top, b < 0x7F800000u ? b : 0u);
+        }
+      }
     }
   }
   top = __reduce_max_sync(0xFFFFFFFFu, top);
@@ -326,57 +443,94 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// FP4 layout -> q * s * g, [rows][ld]; the product q * s is exact.
-template <int DT, bool kMX, bool kVec>
-__global__ void __launch_bounds__(32 * kQRows)
+// FP4 layout -> q * s * g, [rows][ld]; the product q * s is exact (for nvfp4
+// in float16 too: 6 bits, 2^-10 .. 2688).
+template <int DT, bool kMX, bool kVec, int kPer>
+__global__ void __launch_bounds__(32 * kQWarps)
     fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint32_t* __restrict__ scales,
                           const float* __restrict__ gptr, typename Elem<DT>::T* __restrict__ out, int64_t ld,
                           int64_t rows, int cols, int kp) {
-  __shared__ alignas(16) uint8_t sc[kQChunks * kQPitch];
-  __shared__ uint32_t ss[kQCols / 64][kQRows];
-  constexpr int kWordCols = kMX ? 128 : 64;
-  const int64_t row0 = (int64_t)blockIdx.x * kQRows;
+  constexpr int kRows = kQWarps * kPer, kPitch = q_pitch(kRows);
+  constexpr int kWordCols = kMX ? 128 : 64, kWords = kQCols / kWordCols;
+  __shared__ alignas(16) uint8_t sc[kQChunks * kPitch];
+  __shared__ uint32_t ss[kWords * kRows];
+  const int64_t row0 = (int64_t)blockIdx.x * kRows;
   const int col0 = blockIdx.y * kQCols;
   const float g = kMX || !gptr ? 1.0f : __ldg(gptr);
+  const int left = (int)min((int64_t)kRows, rows - row0);
   {
-    const int t = threadIdx.x, r = t & (kQRows - 1), ch = t >> 3;
-    if (row0 + r < rows) {
-      if (t < kQChunks * kQRows) {
-        if (col0 + 32 * ch < kp)
-          *reinterpret_cast<uint4*>(sc + ch * kQPitch + r * 16) =
-              __ldg(reinterpret_cast<const uint4*>(codes + (((int64_t)(col0 / 32) + ch) * rows + row0 + r) * 16));
-      } else {
-        const int w = ch - kQChunks;
-        if (w < kQCols / kWordCols && col0 + kWordCols * w < kp)
-          ss[w][r] = __ldg(scales + ((int64_t)(col0 / kWordCols) + w) * rows + row0 + r);
-      }
+    const uint8_t* src = codes + ((int64_t)(col0 / 32) * rows + row0) * 16;
+    const int nch = min(kQChunks, (kp - col0) / 32);
+#pragma unroll
+    for (int t = threadIdx.x; t < kQChunks * kRows; t += 32 * kQWarps) {
+      const int ch = t / kRows, r = t % kRows;
+      if (ch < nch && r < left)
+        *reinterpret_cast<uint4*>(sc + ch * kPitch + r * 16) =
+            __ldg(reinterpret_cast<const uint4*>(src + ((int64_t)ch * rows + r) * 16));
+    }
+    const uint32_t* ssrc = scales + (int64_t)(col0 / kWordCols) * rows + row0;
+#pragma unroll
+    for (int t = threadIdx.x; t < kWords * kRows; t += 32 * kQWarps) {
+      const int w = t / kRows, r = t % kRows;
+      if (w * kWordCols < kp - col0 && r < left) ss[t] = __ldg(ssrc + (int64_t)w * rows + r);
     }
   }
   __syncthreads();
+  // A lane writes 16 bytes at a time, the warp 512 contiguous ones: kCols
+  // columns of a stretch of 32 * kCols, stretch after stretch.
+  constexpr int kCols = DT == BLUT_F32 ? 4 : 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = row0 + warp;
-  const int col = col0 + 16 * lane, n = min(16, cols - col);
-  if (row >= rows || n <= 0) return;
-  const uint2 c = *reinterpret_cast<const uint2*>(sc + (lane >> 1) * kQPitch + warp * 16 + (lane & 1) * 8);
-  const uint32_t sb = kMX ? (ss[lane >> 3][warp] >> (8 * ((lane >> 1) & 3))) & 0xFFu
-                          : (ss[lane >> 2][warp] >> (8 * (lane & 3))) & 0xFFu;
-  const float s = fp4_scale_f32<kMX>(sb);
-  typename Elem<DT>::T o[16];
+  const uint8_t* s8 = reinterpret_cast<const uint8_t*>(ss);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 q = e2m1x2_f32(((i < 4 ? c.x : c.y) >> (8 * (i & 3))) & 0xFFu);
-    o[2 * i] = Elem<DT>::from(q.x * s * g);
-    o[2 * i + 1] = Elem<DT>::from(q.y * s * g);
-  }
-  typename Elem<DT>::T* p = out + row * ld + col;
-  if (kVec && n == 16) {
-    constexpr int kV = 16 / sizeof(o[0]);
+  for (int i = 0; i < kPer; ++i) {
+    const int r = warp + kQWarps * i;
+    if (r >= left) break;
+    typename Elem<DT>::T* p = out + (row0 + r) * ld + col0;
 #pragma unroll
-    for (int i = 0; i < 16 / kV; ++i) reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<const uint4*>(o + kV * i);
-  } else {
+    for (int k = 0; k < kQCols / (32 * kCols); ++k) {
+      const int c = k * 32 * kCols + lane * kCols, n = cols - col0 - c;  // column inside the 512
+      if (n <= 0) break;
+      const int blk = c / (kMX ? 32 : 16);
+      const float s = fp4_scale_f32<kMX>(s8[((blk >> 2) * kRows + r) * 4 + (blk & 3)]);
+      uint32_t cw = *reinterpret_cast<const uint32_t*>(sc + (c >> 5) * kPitch + r * 16 + ((c & 31) >> 3) * 4);
+      if (kCols == 4) cw >>= 4 * (c & 4);
+      uint32_t q[4], o[4];
+      e2m1x8_f16(cw, q);
+      const __half2 sh = __float2half2_rn(kMX ? 0.0f : s);
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < n) p[i] = o[i];
+      for (int j = 0; j < kCols / 2; ++j) {
+        __half2 h = *reinterpret_cast<const __half2*>(&q[j]);
+        if constexpr (!kMX) h = __hmul2(h, sh);
+        float2 f = __half22float2(h);
+        if constexpr (kMX) {
+          f.x *= s, f.y *= s;
+        } else {
+          f.x *= g, f.y *= g;
+        }
+        if constexpr (DT == BLUT_F32) {
+          o[2 * j] = __float_as_uint(f.x);
+          o[2 * j + 1] = __float_as_uint(f.y);
+        } else if constexpr (DT == BLUT_BF16) {
+          const __nv_bfloat162 b = __float22bfloat162_rn(f);
+          o[j] = *reinterpret_cast<const uint32_t*>(&b);
+        } else {
+          const __half2 b = __float22half2_rn(f);
+          o[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+      }
+      if (kVec && n >= kCols) {
+        *reinterpret_cast<uint4*>(p + c) = make_uint4(o[0], o[1], o[2], o[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+          if (j >= n) break;
+          if constexpr (DT == BLUT_F32)
+            p[c + j] = __uint_as_float(o[j]);
+          else
+            p[c + j] = (uint16_t)(o[j / 2] >> (16 * (j & 1)));
+        }
+      }
+    }
   }
 }
 
@@ -428,41 +582,68 @@ __global__ void fp4_pack_kernel(const uint4* __restrict__ codes, const uint32_t*
         in ? scales[((int64_t)b * words + w) * rows + row] : 0u;
 }
 
-inline bool aligned16(const void* p, int64_t ld_bytes) { return (((uintptr_t)p) | (uintptr_t)ld_bytes) % 16 == 0; }
+// Boundary that p, and p plus multiples of the two byte distances, start on: 32, 16 or 0.
+inline int alignment(const void* p, int64_t a, int64_t b) {
+  const uint64_t all = (uint64_t)(uintptr_t)p | (uint64_t)a | (uint64_t)b;
+  return all % 32 == 0 ? 32 : all % 16 == 0 ? 16 : 0;
+}
 inline int64_t elem_size(int dtype) { return dtype == BLUT_F32 ? 4 : 2; }
 inline int launched() { return cudaGetLastError() == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH; }
 
+// Rows a warp takes: several once that still leaves every SM a few CTAs, one
+// below (32 rows x 2048: 1.7 us with one; 32768 x 2048: 44 us with one).
+inline bool many_rows(int64_t rows, int kp) {
+  return rows * ((kp + kQCols - 1) / kQCols) >= 148ll * 4 * 4 * kQWarps;
+}
+
+template <int DT, bool kMX, bool kSilu, int kVec, int kPer>
+void launch_quantize_as(const blut_fp4_desc& d, const void* x, int64_t ld, const int32_t* row_index, int64_t src_rows,
+                        const float* g, void* codes, void* scales, int signal, int kp, cudaStream_t stream) {
+  const dim3 grid((unsigned)((d.rows + kPer * kQWarps - 1) / (kPer * kQWarps)), (unsigned)((kp + kQCols - 1) / kQCols));
+  fp4_quantize_kernel<DT, kMX, kSilu, kVec, kPer><<<grid, 32 * kQWarps, 0, stream>>>(
+      static_cast<const typename Elem<DT>::T*>(x), ld, row_index, src_rows, g, d.rows, (int)d.cols, kp,
+      static_cast<uint8_t*>(codes), static_cast<uint32_t*>(scales), signal);
+}
+
 template <int DT, bool kSilu>
 int launch_quantize(const blut_fp4_desc& d, const void* x, int64_t ld, const int32_t* row_index, int64_t src_rows,
-                    const float* g, void* codes, void* scales, cudaStream_t stream) {
-  using T = typename Elem<DT>::T;
-  const int64_t es = sizeof(T);
-  const bool vec = aligned16(x, ld * es) && (!kSilu || (d.cols * es) % 16 == 0);
+                    const float* g, void* codes, void* scales, int signal, cudaStream_t stream) {
+  const int64_t es = sizeof(typename Elem<DT>::T);
+  const int vec = alignment(x, ld * es, kSilu ? d.cols * es : 0);
   const int kp = fp4_kblocks(d.cols) * kFp4BlockCols;
-  const dim3 grid((unsigned)((d.rows + kQRows - 1) / kQRows), (unsigned)((kp + kQCols - 1) / kQCols));
-#define BLUT_Q(MX, VEC)                                                                                            \
-  fp4_quantize_kernel<DT, MX, kSilu, VEC><<<grid, 32 * kQRows, 0, stream>>>(                                       \
-      static_cast<const T*>(x), ld, row_index, src_rows, g, d.rows, (int)d.cols, kp, static_cast<uint8_t*>(codes), \
-      static_cast<uint32_t*>(scales))
+  // Four CTAs per SM, and the rows that their 64 registers hold: nvfp4 of
+  // 32768 x 2048 bf16 takes 38.1 us with 4 rows (3 CTAs: 40.1, 2 rows: 41.5,
+  // one: 42.2), mxfp4 30.8 (33.3, 34.1, 36.7); the SiLU form of 196608 x 1408
+  // 237 us with 2 rows (3 CTAs: 273, one row: 239, 4 rows: 308).
+  constexpr int kMany = kSilu || DT == BLUT_F32 ? 2 : 4;
+  const bool many = many_rows(d.rows, kp);
+#define BLUT_Q(MX, VEC, PER) \
+  launch_quantize_as<DT, MX, kSilu, VEC, PER>(d, x, ld, row_index, src_rows, g, codes, scales, signal, kp, stream)
+#define BLUT_V(MX)                                                                                      \
+  if (vec == 32) { if (many) BLUT_Q(MX, 32, kMany); else BLUT_Q(MX, 32, 1); }                             \
+  else if (vec == 16) { if (many) BLUT_Q(MX, 16, kMany); else BLUT_Q(MX, 16, 1); }                        \
+  else BLUT_Q(MX, 0, 1)
   if (d.kind == BLUT_FP4_MX) {
-    if (vec) BLUT_Q(true, true); else BLUT_Q(true, false);
+    BLUT_V(true);
   } else {
-    if (vec) BLUT_Q(false, true); else BLUT_Q(false, false);
+    BLUT_V(false);
   }
+#undef BLUT_V
 #undef BLUT_Q
   return launched();
 }
 
 int quantize(const blut_fp4_desc* d, const void* x, int32_t dtype, int64_t ld, const int32_t* row_index,
-             int64_t src_rows, const float* g, void* codes, void* scales, bool silu, cudaStream_t stream) {
+             int64_t src_rows, const float* g, void* codes, void* scales, bool silu, bool signal,
+             cudaStream_t stream) {
   if (!d || !fp4_valid(*d) || !x || !codes || !scales || ld < (silu ? 2 : 1) * d->cols || src_rows <= 0)
     return BLUT_ERR_INVALID;
   if (!row_index && src_rows != d->rows) return BLUT_ERR_INVALID;
   if (d->kind == BLUT_FP4_NV && !g) return BLUT_ERR_INVALID;
   if (((uintptr_t)codes | (uintptr_t)scales) % 16 != 0 || (uintptr_t)x % elem_size(dtype) != 0) return BLUT_ERR_INVALID;
 #define BLUT_Q(DT)                                                                                            \
-  return silu ? launch_quantize<DT, true>(*d, x, ld, row_index, src_rows, g, codes, scales, stream)           \
-              : launch_quantize<DT, false>(*d, x, ld, row_index, src_rows, g, codes, scales, stream)
+  return silu ? launch_quantize<DT, true>(*d, x, ld, row_index, src_rows, g, codes, scales, signal, stream)   \
+              : launch_quantize<DT, false>(*d, x, ld, row_index, src_rows, g, codes, scales, signal, stream)
   switch (dtype) {
     case BLUT_F16: BLUT_Q(BLUT_F16);
     case BLUT_BF16: BLUT_Q(BLUT_BF16);
@@ -476,35 +657,41 @@ template <int DT>
 int launch_global(const void* x, int64_t rows, int64_t cols, int64_t ld, bool silu, float* out, cudaStream_t stream) {
   using T = typename Elem<DT>::T;
   const int64_t es = sizeof(T);
-  const bool vec = aligned16(x, ld * es) && (!silu || (cols * es) % 16 == 0);
+  const int vec = alignment(x, ld * es, silu ? cols * es : 0);
   const int64_t ctas = (rows * ((cols + 15) / 16) + 255) / 256;
   const unsigned grid = (unsigned)(ctas < 148 * 8 ? ctas : 148 * 8);
   const T* p = static_cast<const T*>(x);
+#define BLUT_G(SILU, VEC) fp4_global_scale_kernel<DT, SILU, VEC><<<grid, 256, 0, stream>>>(p, ld, rows, (int)cols, out)
   if (silu) {
-    if (vec) fp4_global_scale_kernel<DT, true, true><<<grid, 256, 0, stream>>>(p, ld, rows, (int)cols, out);
-    else fp4_global_scale_kernel<DT, true, false><<<grid, 256, 0, stream>>>(p, ld, rows, (int)cols, out);
+    if (vec == 32) BLUT_G(true, 32); else if (vec == 16) BLUT_G(true, 16); else BLUT_G(true, 0);
   } else {
-    if (vec) fp4_global_scale_kernel<DT, false, true><<<grid, 256, 0, stream>>>(p, ld, rows, (int)cols, out);
-    else fp4_global_scale_kernel<DT, false, false><<<grid, 256, 0, stream>>>(p, ld, rows, (int)cols, out);
+    if (vec == 32) BLUT_G(false, 32); else if (vec == 16) BLUT_G(false, 16); else BLUT_G(false, 0);
   }
+#undef BLUT_G
   return launched();
+}
+
+template <int DT, bool kMX, bool kVec, int kPer>
+void launch_dequantize_as(const blut_fp4_desc& d, const void* codes, const void* scales, const float* g, void* out,
+                          int64_t ld, int kp, cudaStream_t stream) {
+  const dim3 grid((unsigned)((d.rows + kPer * kQWarps - 1) / (kPer * kQWarps)),
+                  (unsigned)((d.cols + kQCols - 1) / kQCols));
+  fp4_dequantize_kernel<DT, kMX, kVec, kPer><<<grid, 32 * kQWarps, 0, stream>>>(
+      static_cast<const uint8_t*>(codes), static_cast<const uint32_t*>(scales), g,
+      static_cast<typename Elem<DT>::T*>(out), ld, d.rows, (int)d.cols, kp);
 }
 
 template <int DT>
 int launch_dequantize(const blut_fp4_desc& d, const void* codes, const void* scales, const float* g, void* out,
                       int64_t ld, cudaStream_t stream) {
-  using T = typename Elem<DT>::T;
-  const bool vec = aligned16(out, ld * (int64_t)sizeof(T));
+  const bool vec = alignment(out, ld * (int64_t)sizeof(typename Elem<DT>::T), 0) != 0;
   const int kp = fp4_kblocks(d.cols) * kFp4BlockCols;
-  const dim3 grid((unsigned)((d.rows + kQRows - 1) / kQRows), (unsigned)((d.cols + kQCols - 1) / kQCols));
-#define BLUT_D(MX, VEC)                                                                                    \
-  fp4_dequantize_kernel<DT, MX, VEC><<<grid, 32 * kQRows, 0, stream>>>(                                    \
-      static_cast<const uint8_t*>(codes), static_cast<const uint32_t*>(scales), g, static_cast<T*>(out), ld, d.rows, \
-      (int)d.cols, kp)
+  const bool many = many_rows(d.rows, kp);
+#define BLUT_D(MX, VEC, PER) launch_dequantize_as<DT, MX, VEC, PER>(d, codes, scales, g, out, ld, kp, stream)
   if (d.kind == BLUT_FP4_MX) {
-    if (vec) BLUT_D(true, true); else BLUT_D(true, false);
+    if (!vec) BLUT_D(true, false, 1); else if (many) BLUT_D(true, true, 4); else BLUT_D(true, true, 1);
   } else {
-    if (vec) BLUT_D(false, true); else BLUT_D(false, false);
+    if (!vec) BLUT_D(false, false, 1); else if (many) BLUT_D(false, true, 4); else BLUT_D(false, true, 1);
   }
 #undef BLUT_D
   return launched();
@@ -529,6 +716,12 @@ int rows_convert(const blut_fp4_desc* d, void* rc, void* rs, void* codes, void* 
 inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 }  // namespace
+
+int fp4_quantize_for_product(const blut_fp4_desc& d, const void* x, int32_t dtype, int64_t ld, const float* g,
+                             void* codes, void* scales, cudaStream_t stream) {
+  return quantize(&d, x, dtype, ld, nullptr, d.rows, g, codes, scales, false, true, stream);
+}
+
 }  // namespace blut
 
 using namespace blut;
@@ -566,12 +759,13 @@ int blut_fp4_global_scale(const void* x, int32_t dtype, int64_t rows, int64_t co
 
 int blut_fp4_quantize(const blut_fp4_desc* d, const void* x, int32_t dtype, int64_t ld, const int32_t* row_index,
                       int64_t src_rows, const float* global_scale, void* codes, void* scales, void* stream) {
-  return quantize(d, x, dtype, ld, row_index, src_rows, global_scale, codes, scales, false, S(stream));
+  return quantize(d, x, dtype, ld, row_index, src_rows, global_scale, codes, scales, false, false, S(stream));
 }
 
 int blut_fp4_silu_mul_quantize(const blut_fp4_desc* d, const void* gate_up, int32_t dtype, int64_t ld,
                                const float* global_scale, void* codes, void* scales, void* stream) {
-  return quantize(d, gate_up, dtype, ld, nullptr, d ? d->rows : 0, global_scale, codes, scales, true, S(stream));
+  return quantize(d, gate_up, dtype, ld, nullptr, d ? d->rows : 0, global_scale, codes, scales, true, false,
+                  S(stream));
 }
 
 int blut_fp4_dequantize(const blut_fp4_desc* d, const void* codes, const void* scales, const float* global_scale,

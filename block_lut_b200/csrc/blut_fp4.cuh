@@ -40,6 +40,10 @@ __host__ __device__ inline int fp4_words(int kind) { return kind == BLUT_FP4_NV 
 __host__ __device__ inline int fp4_block(int kind) { return kind == BLUT_FP4_NV ? 16 : 32; }
 __host__ __device__ inline int fp4_unit_bytes(int kind) { return kFp4UnitCodes + 512 * fp4_words(kind); }
 
+// blut_fp4_quantize whose kernel lets a following early launch (blut_fp4_linear's product) begin.
+int fp4_quantize_for_product(const blut_fp4_desc& d, const void* x, int32_t dtype, int64_t ld, const float* g,
+                             void* codes, void* scales, cudaStream_t stream);
+
 // e4m3 byte (0 .. 0x7E) -> float.
 __device__ __forceinline__ float e4m3_f32(uint32_t b) {
   uint32_t h2;
@@ -55,14 +59,13 @@ __device__ __forceinline__ float fp4_scale_f32(uint32_t b) {
     return e4m3_f32(b);
   }
 }
-// Two e2m1 codes (low half first) -> two floats.
-__device__ __forceinline__ float2 e2m1x2_f32(uint32_t byte) {
-  uint32_t h2;
-  asm("{\n\t.reg .b8 b, u1, u2, u3;\n\tmov.b32 {b, u1, u2, u3}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
-      : "=r"(h2)
-      : "r"(byte));
-  return make_float2(__half2float(__ushort_as_half((uint16_t)(h2 & 0xFFFFu))),
-                     __half2float(__ushort_as_half((uint16_t)(h2 >> 16))));
+// Eight e2m1 codes (low half first) -> four float16 pairs.
+__device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t* h) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
 }
 // Eight floats -> eight e2m1 codes, round to nearest even, at most 6.
 __device__ __forceinline__ uint32_t e2m1x8(const float* v) {

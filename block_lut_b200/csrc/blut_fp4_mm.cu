@@ -84,6 +84,7 @@ struct Fp4Params {
   void* y;
   int64_t ldy;
   int out_dtype;
+  int vec;      // rows of y start on 16-byte boundaries
   uint64_t wait_ns;
 };
 
@@ -102,15 +103,19 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
-  float v;
+__device__ __forceinline__ float4 ld_peer4(uint32_t addr, uint32_t rank) {
+  float4 v;
   asm volatile(
-      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
-      : "=f"(v)
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
       : "r"(addr), "r"(rank)
       : "memory");
   return v;
 }
+// Waits until the kernels before this one on the stream are complete (a
+// launch that may begin before that, see launch()); otherwise does nothing.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // 32 rows x 16 bytes of shared memory to 4 columns of all four lane quarters.
 __device__ __forceinline__ void cp_scales(uint32_t taddr, uint32_t saddr) {
@@ -185,13 +190,67 @@ __device__ void find_tile(const Fp4Params& p, int tile, int lane, Fp4Header* h) 
   }
 }
 
-__device__ __forceinline__ void store_y(void* y, int64_t i, int dtype, float v) {
-  if (dtype == BLUT_BF16)
-    static_cast<uint16_t*>(y)[i] = f32_to_act<true>(v);
-  else if (dtype == BLUT_F16)
-    static_cast<uint16_t*>(y)[i] = f32_to_act<false>(v);
+// Two values in the output's 16-bit type, the first in the low half.
+__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
+  return dtype == BLUT_BF16 ? (uint32_t)f32_to_act<true>(a) | ((uint32_t)f32_to_act<true>(b) << 16)
+                            : (uint32_t)f32_to_act<false>(a) | ((uint32_t)f32_to_act<false>(b) << 16);
+}
+__device__ __forceinline__ void store1(const Fp4Params& p, int64_t token, int64_t row, float v) {
+  if (row >= p.n) return;
+  const int64_t i = token * p.ldy + row;
+  if (p.out_dtype == BLUT_F32)
+    static_cast<float*>(p.y)[i] = v;
   else
-    static_cast<float*>(y)[i] = v;
+    static_cast<uint16_t*>(p.y)[i] = p.out_dtype == BLUT_BF16 ? f32_to_act<true>(v) : f32_to_act<false>(v);
+}
+// Rows row .. row + 3 (row % 4 == 0) of one token.
+__device__ __forceinline__ void store4(const Fp4Params& p, int64_t token, int64_t row, float4 v) {
+  if (p.vec && row + 4 <= p.n) {
+    const int64_t i = token * p.ldy + row;
+    if (p.out_dtype == BLUT_F32)
+      *reinterpret_cast<float4*>(static_cast<float*>(p.y) + i) = v;
+    else
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + i) =
+          make_uint2(pack2(v.x, v.y, p.out_dtype), pack2(v.z, v.w, p.out_dtype));
+  } else {
+    store1(p, token, row, v.x);
+    store1(p, token, row + 1, v.y);
+    store1(p, token, row + 2, v.z);
+    store1(p, token, row + 3, v.w);
+  }
+}
+
+// This CTA's share of the tokens, summed over the cluster's partial tiles in
+// rank order.  A thread takes 4 rows of a token; its loads are in flight
+// together.
+template <int S>
+__device__ __forceinline__ void reduce_cluster(const Fp4Params& p, const float* part, int rank, int cnt, int64_t row0,
+                                               int64_t col0, float alpha) {
+  const int quad = 4 * (threadIdx.x & 31);
+  for (int c = rank + S * (threadIdx.x >> 5); c < cnt; c += S * (kThreads / 32)) {
+    const uint32_t a = smem_u32(part + c * 128 + quad);
+    float4 v[S];
+#pragma unroll
+    for (int q = 0; q < S; ++q) v[q] = ld_peer4(a, q);
+    float4 t = v[0];
+#pragma unroll
+    for (int q = 1; q < S; ++q) t.x += v[q].x, t.y += v[q].y, t.z += v[q].z, t.w += v[q].w;
+    store4(p, row0 + c, col0 + quad, make_float4(t.x * alpha, t.y * alpha, t.z * alpha, t.w * alpha));
+  }
+}
+
+// 32 consecutive tensor-memory columns of this thread's lane.
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
 }
 
 template <bool kMX, int NT>
@@ -206,62 +265,83 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
   const int rank = p.split > 1 ? (int)cluster_rank() : 0;
   const int tile = blockIdx.x / p.split;  // 128-row tile of W
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(smem_u32(h->wfull + s), 1);
-      mbar_init(smem_u32(h->sfull + s), 2);
-      mbar_init(smem_u32(h->empty + s), 1);
+  // Warp 0 finds the tile, sets the barriers up and starts the first weight
+  // copies at once, beside the tensor-memory allocation of warp 1.
+  const uint8_t* wsrc = nullptr;
+  int nb = 0, b0 = 0, cnt = 0, row0 = 0, expert = 0, started = 0;
+  const auto bring_w = [&](int i) {
+    const int s = i % C::kStages;
+    const uint32_t bar = smem_u32(h->wfull + s);
+    mbar_expect_tx(bar, C::kA + 4 * (uint32_t)cnt * 16);
+    bulk_g2s(smem_u32(ring + s * C::kStage), wsrc + (int64_t)i * C::kA, C::kA, bar);
+  };
+  const auto my_range = [&]() {
+    // this CTA's K range; every rank of a cluster has the same tile, so all
+    // or none of them have work
+    cnt = h->cnt, row0 = h->row0, expert = cnt > 0 ? h->expert : 0;
+    b0 = (int)((int64_t)p.kblocks * rank / p.split);
+    const int b1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
+    nb = cnt > 0 ? b1 - b0 : 0;
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int s = 0; s < C::kStages; ++s) {
+        mbar_init(smem_u32(h->wfull + s), 1);
+        mbar_init(smem_u32(h->sfull + s), 2);
+        mbar_init(smem_u32(h->empty + s), 1);
+      }
+      mbar_init(smem_u32(&h->acc), 1);
+      mbar_init(smem_u32(&h->fin), 1);
+      h->abort_flag = 0;
+      fence_mbar_init();
+      h->cnt = 0;
+      if (!p.experts) {
+        h->expert = 0;
+        h->row0 = blockIdx.y * NT;
+        h->cnt = (int)min((int64_t)NT, p.x_rows - h->row0);
+      }
     }
-    mbar_init(smem_u32(&h->acc), 1);
-    mbar_init(smem_u32(&h->fin), 1);
-    h->abort_flag = 0;
-    fence_mbar_init();
-  }
-  if (warp == 1) {
+    __syncwarp();
+    if (p.experts) find_tile<NT>(p, blockIdx.y, lane, h);
+    __syncwarp();
+    if (lane == 0) {
+      my_range();
+      wsrc = p.w + expert * p.wstride + ((int64_t)tile * p.kblocks + b0) * C::kA;
+      for (; started < min(nb, C::kStages); ++started) bring_w(started);
+    }
+  } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&h->tmem)),
                  "r"(C::kCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  if (warp == 2) {
-    if (p.experts) {
-      if (lane == 0) h->cnt = 0;
-      __syncwarp();
-      find_tile<NT>(p, blockIdx.y, lane, h);
-    } else if (lane == 0) {
-      h->expert = 0;
-      h->row0 = blockIdx.y * NT;
-      h->cnt = (int)min((int64_t)NT, p.x_rows - h->row0);
-    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = h->tmem;
-  const int cnt = h->cnt, row0 = h->row0, expert = cnt > 0 ? h->expert : 0;
-  // this CTA's K range; every rank of a cluster has the same tile, so all or
-  // none of them have work
-  const int b0 = (int)((int64_t)p.kblocks * rank / p.split), b1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
-  const int nb = cnt > 0 ? b1 - b0 : 0;
+  my_range();
 
   if (cnt > 0) {
     if (warp == 0) {
       // ---------------------------------------------------------- producer --
       if (lane == 0) {
-        const uint8_t* wsrc = p.w + expert * p.wstride + ((int64_t)tile * p.kblocks + b0) * C::kA;
         const uint8_t* xsrc = p.xc + ((int64_t)b0 * 4 * p.x_rows + row0) * 16;
-        const uint32_t xbytes = (uint32_t)cnt * 16;
-        int i = 0;
-        for (; i < nb; ++i) {
+        const auto bring_x = [&](int i) {
           const int s = i % C::kStages;
-          if (i >= C::kStages && !wait_or_abort(smem_u32(h->empty + s), (uint32_t)(i / C::kStages - 1) & 1u, abort_flag,
-                                                &g_fp4_status, p.wait_ns))
-            break;
-          const uint32_t bar = smem_u32(h->wfull + s), dst = smem_u32(ring + s * C::kStage);
-          mbar_expect_tx(bar, C::kA + 4 * xbytes);
-          bulk_g2s(dst, wsrc + (int64_t)i * C::kA, C::kA, bar);
+          const uint32_t bar = smem_u32(h->wfull + s), dst = smem_u32(ring + s * C::kStage + C::kA);
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            bulk_g2s(dst + C::kA + c * NT * 16, xsrc + ((int64_t)i * 4 + c) * p.x_rows * 16, xbytes, bar);
+            bulk_g2s(dst + c * NT * 16, xsrc + ((int64_t)i * 4 + c) * p.x_rows * 16, (uint32_t)cnt * 16, bar);
+        };
+        grid_dependency_wait();  // x may still be in the making; the weights are not
+        int i = 0;
+        for (; i < started; ++i) bring_x(i);
+        for (; i < nb; ++i) {
+          const int s = i % C::kStages;
+          if (!wait_or_abort(smem_u32(h->empty + s), (uint32_t)(i / C::kStages - 1) & 1u, abort_flag, &g_fp4_status,
+                             p.wait_ns))
+            break;
+          bring_w(i);
+          bring_x(i);
         }
         if (i < nb)  // gave up: let the copies in flight land
           for (int j = max(0, i - C::kStages); j < i; ++j)
@@ -326,6 +406,7 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
         dst[q] = C::kA + C::kB + (w * C::kGroups + r / 128) * 512 + (r % 32) * 16 + ((r % 128) / 32) * 4;
       }
       const int64_t step = (int64_t)C::kWords * p.x_rows;
+      grid_dependency_wait();
 #pragma unroll
       for (int j = 0; j < kPrefetch; ++j)
 #pragma unroll
@@ -362,46 +443,60 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
     bool ok = wait_or_abort(smem_u32(&h->acc), 0, abort_flag, &g_fp4_status, p.wait_ns);
     ok = __all_sync(0xFFFFFFFFu, ok);
     tc_fence_after();
+    grid_dependency_wait();
     const float alpha = (p.xg ? __ldg(p.xg) : 1.0f) * (p.wg ? __ldg(p.wg + expert) : 1.0f);
     const int r = 32 * warp + lane;  // weight row inside the tile
-    const int64_t col = (int64_t)tile * 128 + r;
+    const int64_t col0 = (int64_t)tile * 128;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
+    // from here the ring is free: the last MMA has read it
     if (p.split == 1) {
-      if (ok) {
+      const bool vec = p.vec && p.out_dtype != BLUT_F32 && col0 + 128 <= p.n;
+      uint8_t* stage = ring + warp * 2048;  // 32 tokens x 32 rows of 16 bits
+      uint16_t* y16 = static_cast<uint16_t*>(p.y) + (int64_t)row0 * p.ldy + col0 + 32 * warp;
 #pragma unroll 1
-        for (int c = 0; c < cnt; c += 16) {
-          uint32_t v[16];
-          tc_ld16(lane_base + c, v);
-          tc_wait_ld16(v);
-          if (col < p.n) {
+      for (int c = 0; c < cnt && ok; c += 32) {
+        uint32_t v[32];
+        tc_ld32(lane_base + c, v);
+        if (vec) {
+          // through shared memory, so that a store covers 32 rows of 8 tokens, 16 bytes a lane
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c + j < cnt) store_y(p.y, (row0 + c + j) * p.ldy + col, p.out_dtype, __uint_as_float(v[j]) * alpha);
+          for (int j = 0; j < 32; j += 2) {
+            const uint32_t w = pack2(__uint_as_float(v[j]) * alpha, __uint_as_float(v[j + 1]) * alpha, p.out_dtype);
+            *reinterpret_cast<uint16_t*>(stage + j * 64 + lane * 2) = (uint16_t)w;
+            *reinterpret_cast<uint16_t*>(stage + j * 64 + 64 + lane * 2) = (uint16_t)(w >> 16);
           }
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int t = 8 * j + (lane >> 2);
+            if (c + t < cnt)
+              *reinterpret_cast<uint4*>(y16 + (int64_t)(c + t) * p.ldy + (lane & 3) * 8) =
+                  *reinterpret_cast<const uint4*>(stage + t * 64 + (lane & 3) * 16);
+          }
+          __syncwarp();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < cnt) store1(p, row0 + c + j, col0 + r, __uint_as_float(v[j]) * alpha);
         }
       }
     } else {
-      // the ring is free: the last MMA has read it
       float* part = reinterpret_cast<float*>(ring);
-      if (ok) {
 #pragma unroll 1
-        for (int c = 0; c < cnt; c += 16) {
-          uint32_t v[16];
-          tc_ld16(lane_base + c, v);
-          tc_wait_ld16(v);
+      for (int c = 0; c < cnt && ok; c += 32) {
+        uint32_t v[32];
+        tc_ld32(lane_base + c, v);
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c + j < NT) part[(c + j) * 128 + r] = __uint_as_float(v[j]);
-        }
+        for (int j = 0; j < 32; ++j) part[(c + j) * 128 + r] = __uint_as_float(v[j]);
       }
       cluster_sync();
       if (ok) {
-        for (int c = rank; c < cnt; c += p.split) {
-          const uint32_t a = smem_u32(part + c * 128 + r);
-          float sum = 0.0f;
-          for (int q = 0; q < p.split; ++q) sum += ld_peer(a, q);
-          if (col < p.n) store_y(p.y, (row0 + c) * p.ldy + col, p.out_dtype, sum * alpha);
-        }
+        if (p.split == 2)
+          reduce_cluster<2>(p, part, rank, cnt, row0, col0, alpha);
+        else if (p.split == 4)
+          reduce_cluster<4>(p, part, rank, cnt, row0, col0, alpha);
+        else
+          reduce_cluster<8>(p, part, rank, cnt, row0, col0, alpha);
       }
       cluster_sync();  // no CTA leaves while another still reads its partial tile
     }
@@ -412,8 +507,10 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols));
 }
 
+// early: the launch may begin while the kernel before it, which writes x, is
+// still running (it waits in grid_dependency_wait before it reads x).
 template <bool kMX, int NT>
-int launch(const Fp4Params& p, int row_tiles, int64_t token_tiles, cudaStream_t stream) {
+int launch(const Fp4Params& p, int row_tiles, int64_t token_tiles, bool early, cudaStream_t stream) {
   using C = Fp4Cfg<kMX, NT>;
   auto kern = fp4_mm_kernel<kMX, NT>;
   static std::atomic<bool> set[kMaxDevices];
@@ -429,19 +526,24 @@ int launch(const Fp4Params& p, int row_tiles, int64_t token_tiles, cudaStream_t 
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
   if (p.split > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.split;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)p.split;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (early) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
   }
   return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH;
 }
 
 template <bool kMX>
-int dispatch(Fp4Params& p, int64_t m, cudaStream_t stream) {
+int dispatch(Fp4Params& p, int64_t m, bool early, cudaStream_t stream) {
   const int row_tiles = (p.n + 127) / 128;
   // tokens per matrix: their number for one matrix, the mean for runs
   const int64_t mean = p.experts ? (m + p.experts - 1) / p.experts : m;
@@ -451,23 +553,16 @@ int dispatch(Fp4Params& p, int64_t m, cudaStream_t stream) {
   if (tiles > 65535) return BLUT_ERR_UNSUPPORTED;
   p.split = 1;
   if (nt <= 128)
-    while (p.split < 8 && tiles * row_tiles * p.split * 2 <= 296 && p.kblocks >= 4 * p.split) p.split *= 2;
+    while (p.split < 8 && tiles * row_tiles * p.split * 2 <= (nt <= 64 ? 444 : 296) && p.kblocks >= 4 * p.split) p.split *= 2;
   switch (nt) {
-    case 32: return launch<kMX, 32>(p, row_tiles, tiles, stream);
-    case 64: return launch<kMX, 64>(p, row_tiles, tiles, stream);
-    case 128: return launch<kMX, 128>(p, row_tiles, tiles, stream);
-    default: return launch<kMX, 192>(p, row_tiles, tiles, stream);
+    case 32: return launch<kMX, 32>(p, row_tiles, tiles, early, stream);
+    case 64: return launch<kMX, 64>(p, row_tiles, tiles, early, stream);
+    case 128: return launch<kMX, 128>(p, row_tiles, tiles, early, stream);
+    default: return launch<kMX, 192>(p, row_tiles, tiles, early, stream);
   }
 }
 
-}  // namespace
-}  // namespace blut
-
-using namespace blut;
-
-extern "C" {
-
-int blut_fp4_matmul(const blut_fp4_mm_args* a, void* stream) {
+int fp4_check(const blut_fp4_mm_args* a) {
   if (!a || !fp4_valid(a->w) || !a->w_tiled || !a->x_codes || !a->x_scales || !a->y) return BLUT_ERR_INVALID;
   if (a->x_rows <= 0 || a->x_rows > kMaxSlots || a->y_ld < a->w.rows) return BLUT_ERR_INVALID;
   if (a->num_experts < 0 || a->num_experts > kMaxExperts || (a->num_experts && !a->offsets)) return BLUT_ERR_INVALID;
@@ -475,6 +570,12 @@ int blut_fp4_matmul(const blut_fp4_mm_args* a, void* stream) {
   if (((uintptr_t)a->w_tiled | (uintptr_t)a->x_codes | (uintptr_t)a->x_scales) % 16 != 0) return BLUT_ERR_INVALID;
   if (a->out_dtype != BLUT_F16 && a->out_dtype != BLUT_BF16 && a->out_dtype != BLUT_F32) return BLUT_ERR_UNSUPPORTED;
   if ((uintptr_t)a->y % (a->out_dtype == BLUT_F32 ? 4 : 2) != 0) return BLUT_ERR_INVALID;
+  return BLUT_OK;
+}
+
+int fp4_product(const blut_fp4_mm_args* a, bool early, cudaStream_t s) {
+  const int rc = fp4_check(a);
+  if (rc != BLUT_OK) return rc;
   Fp4Params p = {};
   p.w = static_cast<const uint8_t*>(a->w_tiled);
   p.wstride = a->w_stride;
@@ -490,9 +591,66 @@ int blut_fp4_matmul(const blut_fp4_mm_args* a, void* stream) {
   p.y = a->y;
   p.ldy = a->y_ld;
   p.out_dtype = a->out_dtype;
+  p.vec = ((uintptr_t)a->y | (uintptr_t)(a->y_ld * (a->out_dtype == BLUT_F32 ? 4 : 2))) % 16 == 0;
   p.wait_ns = wait_limit_ns();
+  return a->w.kind == BLUT_FP4_MX ? dispatch<true>(p, a->x_rows, early, s) : dispatch<false>(p, a->x_rows, early, s);
+}
+
+// Workspace of blut_fp4_linear: x in 4-bit form, then its g.
+struct LinearWs {
+  int64_t scales, g, total;
+};
+LinearWs linear_ws(const blut_fp4_desc& w, int64_t m) {
+  blut_fp4_desc d = w;
+  d.rows = m;
+  LinearWs l;
+  l.scales = align256(blut_fp4_codes_bytes(&d));
+  l.g = l.scales + align256(blut_fp4_scales_bytes(&d));
+  l.total = l.g + 256;
+  return l;
+}
+
+}  // namespace
+}  // namespace blut
+
+using namespace blut;
+
+extern "C" {
+
+int blut_fp4_matmul(const blut_fp4_mm_args* a, void* stream) {
+  return fp4_product(a, false, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t blut_fp4_linear_workspace_size(const blut_fp4_desc* w, int64_t x_rows) {
+  if (!w || !fp4_valid(*w) || x_rows <= 0 || x_rows > kMaxSlots) return 0;
+  return (size_t)linear_ws(*w, x_rows).total;
+}
+
+int blut_fp4_linear(const blut_fp4_mm_args* args, const void* x, int32_t x_dtype, int64_t x_ld, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  if (!args || !fp4_valid(args->w) || !x || !workspace || (uintptr_t)workspace % 16) return BLUT_ERR_INVALID;
+  if (args->x_rows <= 0 || args->x_rows > kMaxSlots || args->num_experts) return BLUT_ERR_INVALID;
+  const LinearWs ws = linear_ws(args->w, args->x_rows);
+  if (workspace_bytes < (size_t)ws.total) return BLUT_ERR_WORKSPACE;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  blut_fp4_mm_args a = *args;
+  a.x_codes = base;
+  a.x_scales = base + ws.scales;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return a->w.kind == BLUT_FP4_MX ? dispatch<true>(p, a->x_rows, s) : dispatch<false>(p, a->x_rows, s);
+  int rc = fp4_check(&a);
+  if (rc != BLUT_OK) return rc;
+  if (a.w.kind == BLUT_FP4_NV && !a.x_scale) {
+    float* g = reinterpret_cast<float*>(base + ws.g);
+    rc = blut_fp4_global_scale(x, x_dtype, a.x_rows, a.w.cols, x_ld, 0, g, stream);
+    if (rc != BLUT_OK) return rc;
+    a.x_scale = g;
+  } else if (a.w.kind == BLUT_FP4_MX) {
+    a.x_scale = nullptr;
+  }
+  blut_fp4_desc d = a.w;
+  d.rows = a.x_rows;
+  rc = fp4_quantize_for_product(d, x, x_dtype, x_ld, a.x_scale, base, base + ws.scales, s);
+  return rc == BLUT_OK ? fp4_product(&a, true, s) : rc;
 }
 
 int blut_fp4_check_status(void* stream) {
