@@ -117,27 +117,45 @@ __device__ __forceinline__ float4 ld_peer4(uint32_t addr, uint32_t rank) {
 // launch that may begin before that, see launch()); otherwise does nothing.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// One lane of a converged warp; the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Low word of the no-swizzle K-major descriptor (tc_desc) of a shared
+// address, whose bits from 18 up may name the CTA in its cluster; the high
+// word is constant.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) {
+  return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);
+}
+constexpr uint32_t kDescHi = (128u >> 4) | (1u << 14);  // 128 bytes between 8-row groups, version 1
+
 // 32 rows x 16 bytes of shared memory to 4 columns of all four lane quarters.
-__device__ __forceinline__ void cp_scales(uint32_t taddr, uint32_t saddr) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(tc_desc(saddr, 512, 128))
-               : "memory");
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint32_t lo) {
+  asm volatile(
+      "{\n\t.reg .b64 s;\n\tmov.b64 s, {%1, %2};\n\ttcgen05.cp.cta_group::1.32x128b.warpx4 [%0], s;\n\t}" ::"r"(taddr),
+      "r"(lo), "n"(kDescHi)
+      : "memory");
 }
 
 template <bool kMX>
-__device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+__device__ __forceinline__ void mma_fp4(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                         uint32_t acc) {
   if constexpr (kMX) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc), "n"(kDescHi)
         : "memory");
   } else {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::
-            "r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 a, {%1, %7};\n\tmov.b64 b, {%2, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], a, b, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc), "n"(kDescHi)
         : "memory");
   }
 }
@@ -349,40 +367,55 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
       }
     } else if (warp == 1) {
       // --------------------------------------------------------------- MMA --
-      if (lane == 0) {
-        const int n = (cnt + 15) & ~15;
-        bool ok = true;
-        int i = 0;
-        for (; i < nb; ++i) {
-          const int s = i % C::kStages;
-          const uint32_t ph = (uint32_t)(i / C::kStages) & 1u;
-          ok = wait_or_abort(smem_u32(h->wfull + s), ph, abort_flag, &g_fp4_status, p.wait_ns) &&
-               wait_or_abort(smem_u32(h->sfull + s), ph, abort_flag, &g_fp4_status, p.wait_ns);
-          if (C::kSlots < C::kStages && ok && i >= C::kSlots) {
+      // The whole warp runs the loop, so that addresses and descriptors are
+      // uniform values, and one lane issues; run by a single lane, the same
+      // instructions took 75 cycles each to issue.  The barriers of a block
+      // are polled by a lane each.
+      const uint32_t n = (uint32_t)__shfl_sync(0xFFFFFFFFu, (cnt + 15) & ~15, 0);
+      const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+      const int blocks = __shfl_sync(0xFFFFFFFFu, nb, 0);
+      const uint32_t ring_addr = smem_u32(ring);
+      const bool leader = elect_one();
+      bool ok = true;
+      int i = 0;
+      for (; i < blocks; ++i) {
+        const int s = i % C::kStages;
+        {
+          const uint64_t* bar = lane == 1 ? h->sfull + s : h->wfull + s;
+          uint32_t ph = (uint32_t)(i / C::kStages) & 1u;
+          if (C::kSlots < C::kStages && lane == 2 && i >= C::kSlots) {
             // the MMAs that read this slot of scales are done
             const int j = i - C::kSlots;
-            ok = wait_or_abort(smem_u32(h->empty + j % C::kStages), (uint32_t)(j / C::kStages) & 1u, abort_flag,
-                               &g_fp4_status, p.wait_ns);
+            bar = h->empty + j % C::kStages;
+            ph = (uint32_t)(j / C::kStages) & 1u;
           }
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t st = smem_u32(ring + s * C::kStage);
-          const uint32_t slot = tmem + NT + (i % C::kSlots) * C::kSlotCols;
+          ok = __all_sync(0xFFFFFFFFu, wait_or_abort(smem_u32(bar), ph, abort_flag, &g_fp4_status, p.wait_ns));
+        }
+        if (!ok) break;
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t st = ring_addr + s * C::kStage;
+        const uint32_t slot = tm + NT + (i % C::kSlots) * C::kSlotCols;
+        if (leader) {
 #pragma unroll
           for (int w = 0; w < C::kWords; ++w) {
-            cp_scales(slot + w * C::kWordCols, st + kFp4UnitCodes + 512 * w);
+            cp_scales(slot + w * C::kWordCols, desc_lo(st + kFp4UnitCodes + 512 * w, 512));
 #pragma unroll
             for (int g = 0; g < C::kGroups; ++g)
-              cp_scales(slot + w * C::kWordCols + 4 + 4 * g, st + C::kA + C::kB + 512 * (w * C::kGroups + g));
+              cp_scales(slot + w * C::kWordCols + 4 + 4 * g,
+                        desc_lo(st + C::kA + C::kB + 512 * (w * C::kGroups + g), 512));
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const uint32_t sc = slot + (kMX ? 0 : k * C::kWordCols);
-            mma_fp4<kMX>(tmem, tc_desc(st + k * 4096, 2048, 128), tc_desc(st + C::kA + k * 2 * NT * 16, NT * 16, 128),
+            mma_fp4<kMX>(tm, desc_lo(st + k * 4096, 2048), desc_lo(st + C::kA + k * 2 * NT * 16, NT * 16),
                          idesc_fp4<kMX>(n, k), sc, sc + 4, (uint32_t)(i | k));
           }
           tc_commit(smem_u32(h->empty + s));
         }
+        __syncwarp();
+      }
+      if (leader) {
         if (ok) {
           tc_commit(smem_u32(&h->acc));
         } else if (i > 0) {  // gave up: let the MMAs issued so far finish
