@@ -4,25 +4,27 @@
 //
 //   y[t][n] = g_x g_w sum_k (q s)_w[n][k] (q s)_x[t][k],  float32 sums
 //
-// A CTA computes one tile of 128 weight rows x NT tokens over a K range
-// (D^T: weight rows are tensor-memory lanes, tokens are columns, so that a
-// few tokens cost a narrow MMA and not a padded one).  Per 128 columns:
+// A work item is a tile of 128 weight rows x NT tokens (D^T: weight rows are
+// tensor-memory lanes, tokens are columns, so that a few tokens cost a narrow
+// MMA and not a padded one).  A CTA takes items in turn, or shares one with
+// the CTAs of its cluster (split K).  Per 128 columns of K:
 //
-//  * warp 0 (one lane) fetches the tile's unit - 8 KB of codes and the scales
-//    of 128 rows, contiguous - with one bulk copy, and the tokens' codes with
-//    four (a run of rows is contiguous per 32 columns);
+//  * warp 0 fetches the tile's unit - 8 KB of codes and the scales of 128
+//    rows, contiguous - with one bulk copy, and the tokens' codes with four
+//    (a run of rows is contiguous per 32 columns);
 //  * warps 2, 3 bring the tokens' scales into the order that tcgen05.cp reads:
 //    they are the one operand whose position in a tile depends on where the
 //    run of rows starts;
-//  * warp 1 (one lane) copies both scales to tensor memory (tcgen05.cp,
-//    32x128b, replicated to the four lane quarters) and issues two
-//    tcgen05.mma of K = 64, kind::mxf4nvf4 (a scale per 16) or kind::mxf4 (a
-//    scale per 32), M = 128, N = the tile's tokens rounded to 16.
+//  * warp 1 copies both scales to tensor memory (tcgen05.cp, 32x128b,
+//    replicated to the four lane quarters) and issues two tcgen05.mma of
+//    K = 64, kind::mxf4nvf4 (a scale per 16) or kind::mxf4 (a scale per 32),
+//    M = 128, N = the tile's tokens rounded to 16;
+//  * warps 4 .. 7 turn a finished accumulator into rows of y, a lane quarter
+//    each, while the others run ahead into the next item.
 //
-// Then all four warps read the accumulator, one lane quarter each.  Where
-// there are few tiles, a cluster of 2, 4 or 8 CTAs splits K: each leaves its
-// partial tile in its shared memory and sums a share of the tokens over the
-// cluster in rank order, so the result is the same in every run and no
+// Where there are few tiles, a cluster of 2, 4 or 8 CTAs splits K: each leaves
+// its partial tile in its shared memory and sums a share of the tokens over
+// the cluster in rank order, so the result is the same in every run and no
 // workspace is needed.
 //
 // Every wait is bounded; one that runs out raises the CTA's abort flag and
@@ -42,8 +44,10 @@ namespace {
 
 __device__ int g_fp4_status;
 
-constexpr int kThreads = 128;
-constexpr int kHeader = 1024;  // barriers and flags before the ring
+constexpr int kThreads = 256;
+constexpr int kEpiWarp0 = 4;   // first of the four epilogue warps
+constexpr int kEpiStage = 2048;  // bytes an epilogue warp transposes in: 32 tokens x 32 rows of 16 bits
+constexpr int kHeader = 1024;  // barriers and flags
 constexpr int kPrefetch = 4;   // blocks of token scales held in registers
 
 template <bool kMX, int NT>
@@ -57,8 +61,9 @@ struct Fp4Cfg {
   // Two CTAs per SM (three for few tokens) keep copies in flight while one of
   // them starts or stores.
   static constexpr int kCtas = NT <= 64 ? 3 : 2;
-  static constexpr int kStages = (kCtas == 3 ? 74 * 1024 : 111 * 1024) / kStage;
-  static constexpr int kSmem = kHeader + kStages * kStage;
+  static constexpr int kFixed = kHeader + 4 * kEpiStage;
+  static constexpr int kStages = ((kCtas == 3 ? 73 * 1024 : 111 * 1024) - kFixed) / kStage;
+  static constexpr int kSmem = kFixed + kStages * kStage;  // and the table of runs, launch()
   // Tensor memory: NT accumulator columns, then slots of scales; a slot holds
   // one block, 4 columns per word for the weights and for each token group.
   static constexpr int kCols = NT <= 64 ? 128 : 256;
@@ -80,7 +85,9 @@ struct Fp4Params {
   int64_t x_rows;
   int n;        // weight rows
   int kblocks;  // 128-column blocks
-  int split;    // CTAs of a cluster along K
+  int row_tiles;
+  int token_tiles;  // one matrix: their number
+  int split_log;    // log2 of the CTAs of a cluster along K
   void* y;
   int64_t ldy;
   int out_dtype;
@@ -89,10 +96,16 @@ struct Fp4Params {
 };
 
 struct Fp4Header {
-  uint64_t wfull[8], sfull[8], empty[8], acc, fin;
+  uint64_t wfull[8], sfull[8], empty[8], acc_full, acc_empty, fin;
   uint32_t tmem;
   int abort_flag;
-  int expert, row0, cnt;
+  int items;
+};
+static_assert(sizeof(Fp4Header) <= kHeader, "header");
+
+// One work item: tokens row0 .. row0 + cnt - 1 of x, weight rows 128 tile ..
+struct Fp4Item {
+  int expert, row0, cnt, tile;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -169,11 +182,12 @@ __device__ __forceinline__ uint32_t idesc_fp4(int n, int step) {
          (id << 29);
 }
 
-// Which run tile `tile` of the token tiles belongs to (one warp): runs are
-// cut into ceil(rows / NT) tiles, in order.  Offsets are clamped to
-// [0, x_rows], so no offset leads out of the buffers.
+// The runs' first rows and the number of token tiles before each run, tab[e]
+// and tab[E + 1 + e], e = 0 .. E, by one warp; returns the number of tiles.  A
+// run is cut into ceil(rows / NT) tiles.  Offsets are clamped to [0, x_rows],
+// so none leads out of the buffers.
 template <int NT>
-__device__ void find_tile(const Fp4Params& p, int tile, int lane, Fp4Header* h) {
+__device__ int table_of_runs(const Fp4Params& p, int lane, int* tab) {
   int before = 0;
   for (int e0 = 0; e0 < p.experts; e0 += 128) {  // four runs per lane
     int o[5], tiles = 0;
@@ -190,28 +204,55 @@ __device__ void find_tile(const Fp4Params& p, int tile, int lane, Fp4Header* h) 
       const int v = __shfl_up_sync(0xFFFFFFFFu, incl, d);
       if (lane >= d) incl += v;
     }
-    int t = tile - before - (incl - tiles);  // tile index within this lane's runs
-    if (t >= 0 && t < tiles) {
+    int t = before + incl - tiles;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int cnt = max(o[j + 1] - o[j], 0), nt = (cnt + NT - 1) / NT;
-        if (t >= 0 && t < nt) {
-          h->expert = e0 + 4 * lane + j;
-          h->row0 = o[j] + t * NT;
-          h->cnt = min(NT, cnt - t * NT);
-        }
-        t -= nt;
+    for (int j = 0; j < 4; ++j) {
+      const int e = e0 + 4 * lane + j;
+      if (e < p.experts) {
+        tab[e] = o[j];
+        tab[p.experts + 1 + e] = t;
+        t += (max(o[j + 1] - o[j], 0) + NT - 1) / NT;
+        if (e == p.experts - 1) tab[p.experts] = o[j + 1], tab[2 * p.experts + 1] = t;
       }
     }
     before += __shfl_sync(0xFFFFFFFFu, incl, 31);
-    if (before > tile) break;
   }
+  return before;
 }
 
-// Two values in the output's 16-bit type, the first in the low half.
-__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
-  return dtype == BLUT_BF16 ? (uint32_t)f32_to_act<true>(a) | ((uint32_t)f32_to_act<true>(b) << 16)
-                            : (uint32_t)f32_to_act<false>(a) | ((uint32_t)f32_to_act<false>(b) << 16);
+// Item `i`, by a converged warp: row tiles of one token tile follow each other.
+template <int NT>
+__device__ __forceinline__ Fp4Item item_of(const Fp4Params& p, int i, int lane, const int* tab) {
+  Fp4Item t;
+  const int y = i / p.row_tiles;
+  t.tile = i - y * p.row_tiles;
+  if (p.experts) {
+    const int* first = tab + p.experts + 1;
+    int e = -1;  // the last run that starts at or before tile y has it: runs without tiles start where the next does
+    for (int e0 = 0; e0 < p.experts; e0 += 32)
+      e += __popc(__ballot_sync(0xFFFFFFFFu, e0 + lane < p.experts && first[min(e0 + lane, p.experts)] <= y));
+    t.expert = e;
+    const int in = (y - first[e]) * NT, cnt = tab[e + 1] - tab[e];
+    t.row0 = tab[e] + in;
+    t.cnt = min(NT, cnt - in);
+  } else {
+    t.expert = 0;
+    t.row0 = y * NT;
+    t.cnt = (int)min((int64_t)NT, p.x_rows - t.row0);
+  }
+  return t;
+}
+
+// Two values in a 16-bit type, the first in the low half.
+template <int kOut>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (kOut == BLUT_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
 }
 __device__ __forceinline__ void store1(const Fp4Params& p, int64_t token, int64_t row, float v) {
   if (row >= p.n) return;
@@ -229,12 +270,68 @@ __device__ __forceinline__ void store4(const Fp4Params& p, int64_t token, int64_
       *reinterpret_cast<float4*>(static_cast<float*>(p.y) + i) = v;
     else
       *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + i) =
-          make_uint2(pack2(v.x, v.y, p.out_dtype), pack2(v.z, v.w, p.out_dtype));
+          p.out_dtype == BLUT_BF16 ? make_uint2(pack2<BLUT_BF16>(v.x, v.y), pack2<BLUT_BF16>(v.z, v.w))
+                                   : make_uint2(pack2<BLUT_F16>(v.x, v.y), pack2<BLUT_F16>(v.z, v.w));
   } else {
     store1(p, token, row, v.x);
     store1(p, token, row + 1, v.y);
     store1(p, token, row + 2, v.z);
     store1(p, token, row + 3, v.w);
+  }
+}
+
+// 16 lanes (from the address's lane) x 32 columns of 32 bits, in the layout
+// of an mma accumulator: register 4c + 2h + j of a thread is lane
+// l / 4 + 8 h, column 8 c + 2 (l % 4) + j.
+__device__ __forceinline__ void tc_ld_16x32(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// An epilogue warp's 32 weight rows x cnt tokens as 16-bit rows of y: pairs
+// of tokens are packed as an mma accumulator holds them, stmatrix transposes
+// 8 x 8 of them at a time, and a store then covers 32 rows of 8 tokens, 16
+// bytes a lane.  y: token 0, the warp's first row.
+template <int kOut>
+__device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha, uint8_t* stage, uint16_t* y,
+                                             int64_t ldy, int lane) {
+  const uint32_t saddr = smem_u32(stage);
+#pragma unroll 1
+  for (int c = 0; c < cnt; c += 32) {
+    uint32_t v[2][16];
+    tc_ld_16x32(tcol + c, v[0]);
+    tc_ld_16x32(tcol + c + (16u << 16), v[1]);
+    tc_wait_ld16(v[0]);
+    tc_wait_ld16(v[1]);
+#pragma unroll
+    for (int tg = 0; tg < 4; ++tg) {  // 8 tokens x 32 rows: four 8 x 8 matrices
+      uint32_t w[4];
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg)
+        w[rg] = pack2<kOut>(__uint_as_float(v[rg >> 1][4 * tg + 2 * (rg & 1)]) * alpha,
+                            __uint_as_float(v[rg >> 1][4 * tg + 2 * (rg & 1) + 1]) * alpha);
+      // lane 8 rg + i gives the address of token i, rows 8 rg .. 8 rg + 7; the
+      // 16-byte pieces of a token are swapped about against bank conflicts
+      const int t = 8 * tg + (lane & 7), piece = (lane >> 3) ^ ((t >> 1) & 3);
+      asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(saddr + t * 64 +
+                                                                                                 piece * 16),
+                   "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   : "memory");
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = 8 * j + (lane >> 2);
+      if (c + t < cnt)
+        *reinterpret_cast<uint4*>(y + (int64_t)(c + t) * ldy + (lane & 3) * 8) =
+            *reinterpret_cast<const uint4*>(stage + t * 64 + ((lane & 3) ^ ((t >> 1) & 3)) * 16);
+    }
+    __syncwarp();
   }
 }
 
@@ -257,50 +354,33 @@ __device__ __forceinline__ void reduce_cluster(const Fp4Params& p, const float* 
   }
 }
 
-// 32 consecutive tensor-memory columns of this thread's lane.
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr)
-      : "memory");
-}
-
 template <bool kMX, int NT>
 __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kernel(const Fp4Params p) {
   using C = Fp4Cfg<kMX, NT>;
   extern __shared__ __align__(1024) uint8_t fp4_smem[];
-  uint8_t* smem = fp4_smem;
-  Fp4Header* h = reinterpret_cast<Fp4Header*>(smem);
-  uint8_t* ring = smem + kHeader;
+  Fp4Header* h = reinterpret_cast<Fp4Header*>(fp4_smem);
+  uint8_t* ring = fp4_smem + kHeader;
+  uint8_t* epi = ring + C::kStages * C::kStage;
+  int* tab = reinterpret_cast<int*>(epi + 4 * kEpiStage);
   volatile int* abort_flag = &h->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = p.split > 1 ? (int)cluster_rank() : 0;
-  const int tile = blockIdx.x / p.split;  // 128-row tile of W
+  const int split = 1 << p.split_log;
+  const int rank = split > 1 ? (int)cluster_rank() : 0;
+  const int first = blockIdx.x >> p.split_log, step = gridDim.x >> p.split_log;
+  const int b0 = p.kblocks * rank >> p.split_log;  // this CTA's K range
+  const int nb = (p.kblocks * (rank + 1) >> p.split_log) - b0;
 
-  // Warp 0 finds the tile, sets the barriers up and starts the first weight
+  // Warp 0 sets the barriers up, lists the runs, and starts the first weight
   // copies at once, beside the tensor-memory allocation of warp 1.
-  const uint8_t* wsrc = nullptr;
-  int nb = 0, b0 = 0, cnt = 0, row0 = 0, expert = 0, started = 0;
-  const auto bring_w = [&](int i) {
-    const int s = i % C::kStages;
+  const auto bring_w = [&](const Fp4Item& t, int b, int it) {
+    const int s = it % C::kStages;
     const uint32_t bar = smem_u32(h->wfull + s);
-    mbar_expect_tx(bar, C::kA + 4 * (uint32_t)cnt * 16);
-    bulk_g2s(smem_u32(ring + s * C::kStage), wsrc + (int64_t)i * C::kA, C::kA, bar);
+    mbar_expect_tx(bar, C::kA + 4 * (uint32_t)t.cnt * 16);
+    bulk_g2s(smem_u32(ring + s * C::kStage), p.w + t.expert * p.wstride + ((int64_t)t.tile * p.kblocks + b0 + b) * C::kA,
+             C::kA, bar);
   };
-  const auto my_range = [&]() {
-    // this CTA's K range; every rank of a cluster has the same tile, so all
-    // or none of them have work
-    cnt = h->cnt, row0 = h->row0, expert = cnt > 0 ? h->expert : 0;
-    b0 = (int)((int64_t)p.kblocks * rank / p.split);
-    const int b1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
-    nb = cnt > 0 ? b1 - b0 : 0;
-  };
+  Fp4Item t0 = {0, 0, 0, 0};
+  int started = 0;
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < C::kStages; ++s) {
@@ -308,24 +388,20 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
         mbar_init(smem_u32(h->sfull + s), 2);
         mbar_init(smem_u32(h->empty + s), 1);
       }
-      mbar_init(smem_u32(&h->acc), 1);
+      mbar_init(smem_u32(&h->acc_full), 1);
+      mbar_init(smem_u32(&h->acc_empty), 4);
       mbar_init(smem_u32(&h->fin), 1);
       h->abort_flag = 0;
       fence_mbar_init();
-      h->cnt = 0;
-      if (!p.experts) {
-        h->expert = 0;
-        h->row0 = blockIdx.y * NT;
-        h->cnt = (int)min((int64_t)NT, p.x_rows - h->row0);
-      }
     }
+    const int tiles = p.experts ? table_of_runs<NT>(p, lane, tab) : p.token_tiles;
+    if (lane == 0) h->items = tiles * p.row_tiles;
     __syncwarp();
-    if (p.experts) find_tile<NT>(p, blockIdx.y, lane, h);
-    __syncwarp();
-    if (lane == 0) {
-      my_range();
-      wsrc = p.w + expert * p.wstride + ((int64_t)tile * p.kblocks + b0) * C::kA;
-      for (; started < min(nb, C::kStages); ++started) bring_w(started);
+    if (first < tiles * p.row_tiles) {
+      t0 = item_of<NT>(p, first, lane, tab);
+      started = min(nb, C::kStages);
+      if (lane == 0)
+        for (int b = 0; b < started; ++b) bring_w(t0, b, b);
     }
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&h->tmem)),
@@ -336,58 +412,72 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = h->tmem;
-  my_range();
+  const int items = h->items;
 
-  if (cnt > 0) {
-    if (warp == 0) {
-      // ---------------------------------------------------------- producer --
-      if (lane == 0) {
-        const uint8_t* xsrc = p.xc + ((int64_t)b0 * 4 * p.x_rows + row0) * 16;
-        const auto bring_x = [&](int i) {
-          const int s = i % C::kStages;
-          const uint32_t bar = smem_u32(h->wfull + s), dst = smem_u32(ring + s * C::kStage + C::kA);
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer --
+    if (first < items) {
+      const auto bring_x = [&](const Fp4Item& t, int b, int it) {
+        const int s = it % C::kStages;
+        const uint32_t bar = smem_u32(h->wfull + s), dst = smem_u32(ring + s * C::kStage + C::kA);
+        const uint8_t* src = p.xc + ((int64_t)(b0 + b) * 4 * p.x_rows + t.row0) * 16;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            bulk_g2s(dst + c * NT * 16, xsrc + ((int64_t)i * 4 + c) * p.x_rows * 16, (uint32_t)cnt * 16, bar);
-        };
-        grid_dependency_wait();  // x may still be in the making; the weights are not
-        int i = 0;
-        for (; i < started; ++i) bring_x(i);
-        for (; i < nb; ++i) {
-          const int s = i % C::kStages;
-          if (!wait_or_abort(smem_u32(h->empty + s), (uint32_t)(i / C::kStages - 1) & 1u, abort_flag, &g_fp4_status,
-                             p.wait_ns))
-            break;
-          bring_w(i);
-          bring_x(i);
-        }
-        if (i < nb)  // gave up: let the copies in flight land
-          for (int j = max(0, i - C::kStages); j < i; ++j)
-            wait_drain(smem_u32(h->wfull + j % C::kStages), (uint32_t)(j / C::kStages) & 1u);
-      }
-    } else if (warp == 1) {
-      // --------------------------------------------------------------- MMA --
-      // The whole warp runs the loop, so that addresses and descriptors are
-      // uniform values, and one lane issues; run by a single lane, the same
-      // instructions took 75 cycles each to issue.  The barriers of a block
-      // are polled by a lane each.
-      const uint32_t n = (uint32_t)__shfl_sync(0xFFFFFFFFu, (cnt + 15) & ~15, 0);
-      const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-      const int blocks = __shfl_sync(0xFFFFFFFFu, nb, 0);
-      const uint32_t ring_addr = smem_u32(ring);
-      const bool leader = elect_one();
+        for (int c = 0; c < 4; ++c)
+          bulk_g2s(dst + c * NT * 16, src + (int64_t)c * p.x_rows * 16, (uint32_t)t.cnt * 16, bar);
+      };
+      grid_dependency_wait();  // x may still be in the making; the weights are not
+      int it = 0;              // blocks over all items: the ring goes on from one to the next
       bool ok = true;
-      int i = 0;
-      for (; i < blocks; ++i) {
-        const int s = i % C::kStages;
+      for (int i = first; i < items && ok; i += step) {
+        const Fp4Item t = i == first ? t0 : item_of<NT>(p, i, lane, tab);
+        if (lane == 0) {
+          for (int b = 0; b < nb; ++b, ++it) {
+            if (it >= started) {
+              const int s = it % C::kStages;
+              if (it >= C::kStages && !wait_or_abort(smem_u32(h->empty + s), (uint32_t)(it / C::kStages - 1) & 1u,
+                                                     abort_flag, &g_fp4_status, p.wait_ns)) {
+                ok = false;
+                break;
+              }
+              bring_w(t, b, it);
+            }
+            bring_x(t, b, it);
+          }
+        }
+        ok = __all_sync(0xFFFFFFFFu, ok);
+      }
+      if (lane == 0)  // whatever the other roles do, no copy is in flight when the CTA ends
+        for (int j = max(0, it - C::kStages); j < it; ++j)
+          wait_drain(smem_u32(h->wfull + j % C::kStages), (uint32_t)(j / C::kStages) & 1u);
+      __syncwarp();
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA --
+    // The whole warp runs the loop, so that addresses and descriptors are
+    // uniform values, and one lane issues; run by a single lane, the same
+    // instructions took 75 cycles each to issue.  The barriers of a block
+    // are polled by a lane each.
+    const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+    const uint32_t ring_addr = smem_u32(ring);
+    const bool leader = elect_one();
+    bool ok = true;
+    int it = 0, acc = 0;
+    for (int i = first; i < items && ok; i += step, ++acc) {
+      const uint32_t n = (uint32_t)__shfl_sync(0xFFFFFFFFu, (item_of<NT>(p, i, lane, tab).cnt + 15) & ~15, 0);
+      for (int b = 0; b < nb; ++b, ++it) {
+        const int s = it % C::kStages;
         {
           const uint64_t* bar = lane == 1 ? h->sfull + s : h->wfull + s;
-          uint32_t ph = (uint32_t)(i / C::kStages) & 1u;
-          if (C::kSlots < C::kStages && lane == 2 && i >= C::kSlots) {
+          uint32_t ph = (uint32_t)(it / C::kStages) & 1u;
+          if (C::kSlots < C::kStages && lane == 2 && it >= C::kSlots) {
             // the MMAs that read this slot of scales are done
-            const int j = i - C::kSlots;
+            const int j = it - C::kSlots;
             bar = h->empty + j % C::kStages;
             ph = (uint32_t)(j / C::kStages) & 1u;
+          }
+          if (lane == 3 && b == 0 && acc > 0) {  // the accumulator has been read
+            bar = &h->acc_empty;
+            ph = (uint32_t)(acc - 1) & 1u;
           }
           ok = __all_sync(0xFFFFFFFFu, wait_or_abort(smem_u32(bar), ph, abort_flag, &g_fp4_status, p.wait_ns));
         }
@@ -395,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
         __syncwarp();
         tc_fence_after();
         const uint32_t st = ring_addr + s * C::kStage;
-        const uint32_t slot = tm + NT + (i % C::kSlots) * C::kSlotCols;
+        const uint32_t slot = tm + NT + (it % C::kSlots) * C::kSlotCols;
         if (leader) {
 #pragma unroll
           for (int w = 0; w < C::kWords; ++w) {
@@ -409,49 +499,51 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
           for (int k = 0; k < 2; ++k) {
             const uint32_t sc = slot + (kMX ? 0 : k * C::kWordCols);
             mma_fp4<kMX>(tm, desc_lo(st + k * 4096, 2048), desc_lo(st + C::kA + k * 2 * NT * 16, NT * 16),
-                         idesc_fp4<kMX>(n, k), sc, sc + 4, (uint32_t)(i | k));
+                         idesc_fp4<kMX>(n, k), sc, sc + 4, (uint32_t)(b | k));
           }
           tc_commit(smem_u32(h->empty + s));
+          if (b == nb - 1) tc_commit(smem_u32(&h->acc_full));
         }
         __syncwarp();
       }
-      if (leader) {
-        if (ok) {
-          tc_commit(smem_u32(&h->acc));
-        } else if (i > 0) {  // gave up: let the MMAs issued so far finish
-          tc_commit(smem_u32(&h->fin));
-          wait_drain(smem_u32(&h->fin), 0);
-        }
-      }
-    } else {
-      // ------------------------------------------------------ token scales --
-      constexpr int kWordsAll = C::kWords * NT;
-      constexpr int kIt = (kWordsAll + 63) / 64;
-      const int t = threadIdx.x - 64;
+    }
+    if (!ok && it > 0 && leader) {  // gave up: let the MMAs issued so far finish
+      tc_commit(smem_u32(&h->fin));
+      wait_drain(smem_u32(&h->fin), 0);
+    }
+    __syncwarp();
+  } else if (warp < kEpiWarp0) {
+    // -------------------------------------------------------- token scales --
+    constexpr int kWordsAll = C::kWords * NT;
+    constexpr int kIt = (kWordsAll + 63) / 64;
+    const int t64 = threadIdx.x - 64;
+    const int64_t words = (int64_t)C::kWords * p.x_rows;
+    bool ok = true;
+    int it = 0;
+    grid_dependency_wait();
+    for (int i = first; i < items && ok; i += step) {
+      const Fp4Item t = item_of<NT>(p, i, lane, tab);
       const uint32_t* src[kIt];
       uint32_t dst[kIt], buf[kPrefetch][kIt];
       bool on[kIt];
 #pragma unroll
       for (int q = 0; q < kIt; ++q) {
-        const int idx = t + 64 * q, r = idx % NT, w = idx / NT;
-        on[q] = idx < kWordsAll && r < cnt;
-        src[q] = p.xs + ((int64_t)b0 * C::kWords + w) * p.x_rows + row0 + r;
+        const int idx = t64 + 64 * q, r = idx % NT, w = idx / NT;
+        on[q] = idx < kWordsAll && r < t.cnt;
+        src[q] = p.xs + ((int64_t)b0 * C::kWords + w) * p.x_rows + t.row0 + r;
         dst[q] = C::kA + C::kB + (w * C::kGroups + r / 128) * 512 + (r % 32) * 16 + ((r % 128) / 32) * 4;
       }
-      const int64_t step = (int64_t)C::kWords * p.x_rows;
-      grid_dependency_wait();
 #pragma unroll
       for (int j = 0; j < kPrefetch; ++j)
 #pragma unroll
-        for (int q = 0; q < kIt; ++q) buf[j][q] = j < nb && on[q] ? __ldg(src[q] + j * step) : 0u;
-      bool ok = true;
-      for (int i0 = 0; i0 < nb && ok; i0 += kPrefetch) {
+        for (int q = 0; q < kIt; ++q) buf[j][q] = j < nb && on[q] ? __ldg(src[q] + j * words) : 0u;
+      for (int c = 0; c < nb && ok; c += kPrefetch) {
 #pragma unroll
         for (int j = 0; j < kPrefetch; ++j) {
-          const int i = i0 + j, s = i % C::kStages;
-          if (i < nb && ok) {
-            if (i >= C::kStages) {
-              ok = wait_or_abort(smem_u32(h->empty + s), (uint32_t)(i / C::kStages - 1) & 1u, abort_flag, &g_fp4_status,
+          const int b = c + j, s = it % C::kStages;
+          if (b < nb && ok) {
+            if (it >= C::kStages) {
+              ok = wait_or_abort(smem_u32(h->empty + s), (uint32_t)(it / C::kStages - 1) & 1u, abort_flag, &g_fp4_status,
                                  p.wait_ns);
               ok = __all_sync(0xFFFFFFFFu, ok);
             }
@@ -464,75 +556,81 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
               if (lane == 0) mbar_arrive(smem_u32(h->sfull + s));
 #pragma unroll
               for (int q = 0; q < kIt; ++q)
-                if (i + kPrefetch < nb && on[q]) buf[j][q] = __ldg(src[q] + (i + kPrefetch) * step);
+                if (b + kPrefetch < nb && on[q]) buf[j][q] = __ldg(src[q] + (b + kPrefetch) * words);
             }
+            ++it;
           }
         }
       }
     }
-    __syncwarp();
-
+  } else if (split == 1) {
     // ------------------------------------------------------------ epilogue --
-    bool ok = wait_or_abort(smem_u32(&h->acc), 0, abort_flag, &g_fp4_status, p.wait_ns);
-    ok = __all_sync(0xFFFFFFFFu, ok);
-    tc_fence_after();
+    const int q = warp - kEpiWarp0;
+    uint8_t* stage = epi + q * kEpiStage;
+    const uint32_t tcol = tmem + ((uint32_t)(32 * q) << 16);
     grid_dependency_wait();
-    const float alpha = (p.xg ? __ldg(p.xg) : 1.0f) * (p.wg ? __ldg(p.wg + expert) : 1.0f);
-    const int r = 32 * warp + lane;  // weight row inside the tile
-    const int64_t col0 = (int64_t)tile * 128;
-    const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
-    // from here the ring is free: the last MMA has read it
-    if (p.split == 1) {
-      const bool vec = p.vec && p.out_dtype != BLUT_F32 && col0 + 128 <= p.n;
-      uint8_t* stage = ring + warp * 2048;  // 32 tokens x 32 rows of 16 bits
-      uint16_t* y16 = static_cast<uint16_t*>(p.y) + (int64_t)row0 * p.ldy + col0 + 32 * warp;
+    const float gx = p.xg ? __ldg(p.xg) : 1.0f;
+    int acc = 0;
+    for (int i = first; i < items; i += step, ++acc) {
+      const Fp4Item t = item_of<NT>(p, i, lane, tab);
+      const float alpha = gx * (p.wg ? __ldg(p.wg + t.expert) : 1.0f);
+      const int64_t row = (int64_t)t.tile * 128 + 32 * q;
+      if (!__all_sync(0xFFFFFFFFu, wait_or_abort(smem_u32(&h->acc_full), (uint32_t)acc & 1u, abort_flag, &g_fp4_status,
+                                                 p.wait_ns)))
+        break;
+      tc_fence_after();
+      if (p.vec && p.out_dtype != BLUT_F32 && row + 32 <= p.n) {
+        uint16_t* y = static_cast<uint16_t*>(p.y) + (int64_t)t.row0 * p.ldy + row;
+        if (p.out_dtype == BLUT_BF16)
+          store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, lane);
+        else
+          store_tile16<BLUT_F16>(tcol, t.cnt, alpha, stage, y, p.ldy, lane);
+      } else {
 #pragma unroll 1
-      for (int c = 0; c < cnt && ok; c += 32) {
-        uint32_t v[32];
-        tc_ld32(lane_base + c, v);
-        if (vec) {
-          // through shared memory, so that a store covers 32 rows of 8 tokens, 16 bytes a lane
+        for (int c = 0; c < t.cnt; c += 16) {
+          uint32_t v[16];
+          tc_ld16(tcol + c, v);
+          tc_wait_ld16(v);
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const uint32_t w = pack2(__uint_as_float(v[j]) * alpha, __uint_as_float(v[j + 1]) * alpha, p.out_dtype);
-            *reinterpret_cast<uint16_t*>(stage + j * 64 + lane * 2) = (uint16_t)w;
-            *reinterpret_cast<uint16_t*>(stage + j * 64 + 64 + lane * 2) = (uint16_t)(w >> 16);
-          }
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int t = 8 * j + (lane >> 2);
-            if (c + t < cnt)
-              *reinterpret_cast<uint4*>(y16 + (int64_t)(c + t) * p.ldy + (lane & 3) * 8) =
-                  *reinterpret_cast<const uint4*>(stage + t * 64 + (lane & 3) * 16);
-          }
-          __syncwarp();
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < cnt) store1(p, row0 + c + j, col0 + r, __uint_as_float(v[j]) * alpha);
+          for (int j = 0; j < 16; ++j)
+            if (c + j < t.cnt) store1(p, t.row0 + c + j, row + lane, __uint_as_float(v[j]) * alpha);
         }
       }
-    } else {
-      float* part = reinterpret_cast<float*>(ring);
-#pragma unroll 1
-      for (int c = 0; c < cnt && ok; c += 32) {
-        uint32_t v[32];
-        tc_ld32(lane_base + c, v);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) part[(c + j) * 128 + r] = __uint_as_float(v[j]);
-      }
-      cluster_sync();
-      if (ok) {
-        if (p.split == 2)
-          reduce_cluster<2>(p, part, rank, cnt, row0, col0, alpha);
-        else if (p.split == 4)
-          reduce_cluster<4>(p, part, rank, cnt, row0, col0, alpha);
-        else
-          reduce_cluster<8>(p, part, rank, cnt, row0, col0, alpha);
-      }
-      cluster_sync();  // no CTA leaves while another still reads its partial tile
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&h->acc_empty));
     }
+  }
+
+  if (split > 1 && first < items) {
+    // ----------------------------------- one item, K split over the cluster --
+    const Fp4Item t = item_of<NT>(p, first, lane, tab);
+    float* part = reinterpret_cast<float*>(ring);  // free: the last MMA has read it
+    bool ok = __all_sync(0xFFFFFFFFu, wait_or_abort(smem_u32(&h->acc_full), 0, abort_flag, &g_fp4_status, p.wait_ns));
+    tc_fence_after();
+    if (warp >= kEpiWarp0 && ok) {
+      const int q = warp - kEpiWarp0;
+#pragma unroll 1
+      for (int c = 0; c < t.cnt; c += 16) {
+        uint32_t v[16];
+        tc_ld16(tmem + ((uint32_t)(32 * q) << 16) + c, v);
+        tc_wait_ld16(v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c + j) * 128 + 32 * q + lane] = __uint_as_float(v[j]);
+      }
+    }
+    cluster_sync();
+    grid_dependency_wait();
+    const float alpha = (p.xg ? __ldg(p.xg) : 1.0f) * (p.wg ? __ldg(p.wg + t.expert) : 1.0f);
+    if (ok) {
+      if (split == 2)
+        reduce_cluster<2>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
+      else if (split == 4)
+        reduce_cluster<4>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
+      else
+        reduce_cluster<8>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
+    }
+    cluster_sync();  // no CTA leaves while another still reads its partial tile
   }
   tc_fence_before();
   __syncthreads();
@@ -543,27 +641,34 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
 // early: the launch may begin while the kernel before it, which writes x, is
 // still running (it waits in grid_dependency_wait before it reads x).
 template <bool kMX, int NT>
-int launch(const Fp4Params& p, int row_tiles, int64_t token_tiles, bool early, cudaStream_t stream) {
+int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
   using C = Fp4Cfg<kMX, NT>;
   auto kern = fp4_mm_kernel<kMX, NT>;
-  static std::atomic<bool> set[kMaxDevices];
+  constexpr int kMaxSmem = C::kSmem + (2 * kMaxExperts + 2) * 4;
+  static std::atomic<int> sms_of[kMaxDevices];  // 0: not set up yet
   const int dev = cache_device();
-  if (dev < 0 || !set[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess ||
+  int sms = dev < 0 ? 0 : sms_of[dev].load(std::memory_order_acquire);
+  if (sms == 0) {
+    int d = 0;
+    if (cudaGetDevice(&d) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess ||
         cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
       return BLUT_ERR_CUDA;
-    if (dev >= 0) set[dev].store(true, std::memory_order_release);
+    if (dev >= 0) sms_of[dev].store(sms, std::memory_order_release);
   }
+  const int split = 1 << p.split_log;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(row_tiles * p.split), (unsigned)token_tiles);
+  // one CTA (cluster) per item where K is split, else as many as run at once
+  cfg.gridDim = dim3((unsigned)(split > 1 ? items * split : std::min<int64_t>(items, (int64_t)sms * C::kCtas)));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.dynamicSmemBytes = C::kSmem + (p.experts ? (2 * p.experts + 2) * 4 : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  if (p.split > 1) {
+  if (split > 1) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)p.split;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)split;
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
@@ -572,26 +677,29 @@ int launch(const Fp4Params& p, int row_tiles, int64_t token_tiles, bool early, c
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kern, (const Fp4Params)p) == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH;
 }
 
 template <bool kMX>
 int dispatch(Fp4Params& p, int64_t m, bool early, cudaStream_t stream) {
-  const int row_tiles = (p.n + 127) / 128;
+  p.row_tiles = (p.n + 127) / 128;
   // tokens per matrix: their number for one matrix, the mean for runs
   const int64_t mean = p.experts ? (m + p.experts - 1) / p.experts : m;
   const int nt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 192;
   // bound on the token tiles: every run may end in a partial one
   const int64_t tiles = p.experts ? m / nt + std::min<int64_t>(p.experts, m) : (m + nt - 1) / nt;
-  if (tiles > 65535) return BLUT_ERR_UNSUPPORTED;
-  p.split = 1;
+  const int64_t items = tiles * p.row_tiles;
+  if (items * 8 > INT32_MAX) return BLUT_ERR_UNSUPPORTED;
+  p.token_tiles = (int)tiles;
+  p.split_log = 0;
   if (nt <= 128)
-    while (p.split < 8 && tiles * row_tiles * p.split * 2 <= (nt <= 64 ? 444 : 296) && p.kblocks >= 4 * p.split) p.split *= 2;
+    while (p.split_log < 3 && (items << p.split_log) * 2 <= (nt <= 64 ? 444 : 296) && p.kblocks >= 4 << p.split_log)
+      ++p.split_log;
   switch (nt) {
-    case 32: return launch<kMX, 32>(p, row_tiles, tiles, early, stream);
-    case 64: return launch<kMX, 64>(p, row_tiles, tiles, early, stream);
-    case 128: return launch<kMX, 128>(p, row_tiles, tiles, early, stream);
-    default: return launch<kMX, 192>(p, row_tiles, tiles, early, stream);
+    case 32: return launch<kMX, 32>(p, items, early, stream);
+    case 64: return launch<kMX, 64>(p, items, early, stream);
+    case 128: return launch<kMX, 128>(p, items, early, stream);
+    default: return launch<kMX, 192>(p, items, early, stream);
   }
 }
 
