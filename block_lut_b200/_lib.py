@@ -124,7 +124,7 @@ SIGNATURES = [
     ("blut_fp4_export", C.c_int, [C.POINTER(FP4Desc), _VP, _VP, _VP, _VP, _VP]),
     ("blut_fp4_pack_tiled", C.c_int, [C.POINTER(FP4Desc), _VP, _VP, _VP, _VP]),
     ("blut_fp4_matmul", C.c_int, [C.POINTER(FP4MMArgs), _VP]),
-    ("blut_fp4_linear_workspace_size", C.c_size_t, [C.POINTER(FP4Desc), _I64]),
+    ("blut_fp4_linear_workspace_size", C.c_int64, [C.POINTER(FP4Desc), _I64, _I32]),
     ("blut_fp4_linear", C.c_int, [C.POINTER(FP4MMArgs), _VP, _I32, _I64, _VP, C.c_size_t, _VP]),
     ("blut_fp4_check_status", C.c_int, [_VP]),
 ]

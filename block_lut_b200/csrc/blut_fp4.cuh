@@ -3,6 +3,9 @@
 // product share.
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
 #include "blut_common.cuh"
 #include "blut_internal.h"
 
@@ -79,6 +82,189 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* v) {
       : "=r"(d)
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return d;
+}
+
+constexpr float kSiluWin = 0x1p-17f;  // twice the error of a float32 silu(gate) * up / (s g)
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<BLUT_F16> {
+  using T = uint16_t;
+  static __device__ __forceinline__ float f(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+  static __device__ __forceinline__ uint16_t from(float v) { return __half_as_ushort(__float2half_rn(v)); }
+};
+template <>
+struct Elem<BLUT_BF16> {
+  using T = uint16_t;
+  static __device__ __forceinline__ float f(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+  static __device__ __forceinline__ uint16_t from(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+};
+template <>
+struct Elem<BLUT_F32> {
+  using T = float;
+  static __device__ __forceinline__ float f(float v) { return v; }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+
+// 16 consecutive values of a row, zeros past the n valid ones.
+template <int DT>
+__device__ __forceinline__ void load16(const typename Elem<DT>::T* p, int n, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = i < n ? Elem<DT>::f(p[i]) : 0.0f;
+}
+
+// 16 values of a row as they are in memory.  kVec: the boundary in bytes that
+// every such run starts on (32 or 16), or 0 for any other.
+template <int DT>
+struct Raw {
+  static constexpr int kN = DT == BLUT_F32 ? 4 : 2;
+  uint4 w[kN];
+};
+template <int DT, int kVec>
+__device__ __forceinline__ void raw_load(const typename Elem<DT>::T* p, Raw<DT>& r) {
+  if constexpr (kVec == 16) {
+#pragma unroll
+    for (int i = 0; i < Raw<DT>::kN; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Raw<DT>::kN; i += 2)
+      asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+          : "=r"(r.w[i].x), "=r"(r.w[i].y), "=r"(r.w[i].z), "=r"(r.w[i].w), "=r"(r.w[i + 1].x), "=r"(r.w[i + 1].y),
+            "=r"(r.w[i + 1].z), "=r"(r.w[i + 1].w)
+          : "l"(reinterpret_cast<const uint4*>(p) + i));
+  }
+}
+template <int DT>
+__device__ __forceinline__ void raw_unpack(const Raw<DT>& r, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < Raw<DT>::kN; ++i) {
+    const uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == BLUT_F32) {
+        v[4 * i + j] = __uint_as_float(w[j]);
+      } else if constexpr (DT == BLUT_BF16) {
+        v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+        v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[8 * i + 2 * j] = f.x;
+        v[8 * i + 2 * j + 1] = f.y;
+      }
+    }
+  }
+}
+
+// max(a, |b|, |c|); NaN if one of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
+}
+
+// Border between e2m1 codes c and c + 1 (c = 0 .. 6).
+__device__ __forceinline__ float e2m1_border(uint32_t c) {
+  return c < 4 ? 0.25f + 0.5f * (float)c : c == 4 ? 2.5f : c == 5 ? 3.5f : 5.0f;
+}
+// Code of |x| between the neighbours lo and lo + 1, by the exact quotient.
+__device__ __forceinline__ uint32_t e2m1_decide(double ax, double unit, uint32_t lo) {
+  const double border = (double)e2m1_border(lo) * unit;
+  return ax > border || (ax == border && (lo & 1)) ? lo + 1 : lo;
+}
+__device__ __forceinline__ uint32_t e4m3x2_sat(float hi, float lo) {
+  uint16_t d;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// e4m3(a / (6 g)) by the exact quotient; t is that quotient up to 2^-21.
+__device__ __forceinline__ uint32_t e4m3_scale(double a, float g, float t) {
+  const uint32_t both = e4m3x2_sat(t * (1.0f + 0x1p-20f), t * (1.0f - 0x1p-20f));
+  uint32_t lo = both & 0xFFu;
+  const uint32_t hi = both >> 8;
+  if (lo != hi) {
+    const double border = 0.5 * ((double)e4m3_f32(lo) + (double)e4m3_f32(hi)) * (6.0 * (double)g);
+    if (a > border || (a == border && (lo & 1))) lo = hi;
+  }
+  return lo;
+}
+
+// The scale byte and the 16 codes of this lane's columns.  A block is one
+// lane (nvfp4) or two neighbouring lanes (mxfp4).  v: the values; kSilu:
+// float32 approximations, and `unsure` is raised for a block that a more
+// exact form could change.
+template <bool kMX, bool kSilu>
+__device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool& unsure, uint32_t& sbyte) {
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) most = max3_abs(most, v[i], v[i + 1]);
+  uint32_t top = __float_as_uint(most) & 0x7FFFFFFFu;  // bits of non-negative floats order as integers, NaN last
+  if (kMX) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  const bool bad = top >= 0x7F800000u;  // an infinity or a NaN: the block has no scale
+  const float a = __uint_as_float(top);
+  float r, unit = 0.0f;
+  if constexpr (kMX) {
+    const int e = (int)(top >> 23);
+    sbyte = e > 2 ? (uint32_t)(e - 2) : 0u;
+    r = __uint_as_float((254u - sbyte) << 23);
+    if (kSilu) {  // near a power of two, or where float32 has lost digits
+      unsure |= (__float_as_uint(a * (1.0f + kSiluWin)) >> 23) != (__float_as_uint(a * (1.0f - kSiluWin)) >> 23);
+      unsure |= a < 0x1p-100f && top != 0;
+    }
+  } else {
+    const float t = a * __frcp_rn(6.0f * g);
+    if (kSilu) {
+      const uint32_t both = e4m3x2_sat(t * (1.0f + kSiluWin), t * (1.0f - kSiluWin));
+      sbyte = both & 0xFFu;
+      unsure |= sbyte != both >> 8;
+    } else {
+      sbyte = e4m3_scale((double)a, g, t);
+    }
+    unit = e4m3_f32(sbyte);
+    r = unit > 0.0f ? __frcp_rn(unit * g) : 0.0f;
+  }
+  uint2 c;
+  if constexpr (kMX && !kSilu) {
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = v[i] * r;
+    c = make_uint2(e2m1x8(w), e2m1x8(w + 8));
+  } else {
+    constexpr float kWin = kSilu ? kSiluWin : 0x1p-21f;
+    const float ru = r * (1.0f + kWin), rd = r * (1.0f - kWin);
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = v[i] * rd;
+    c = make_uint2(e2m1x8(w), e2m1x8(w + 8));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = v[i] * ru;
+    uint32_t d0 = c.x ^ e2m1x8(w), d1 = c.y ^ e2m1x8(w + 8);
+    if constexpr (!kSilu) {
+      if (d0 | d1) {
+        const double un = (double)unit * (double)g;  // 4 + 24 bits: exact
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          uint32_t& cw = i < 8 ? c.x : c.y;
+          const int sh = 4 * (i & 7);
+          if (((i < 8 ? d0 : d1) >> sh) & 15u) {
+            const uint32_t lo = (cw >> sh) & 7u;
+            cw += (e2m1_decide((double)fabsf(v[i]), un, lo) - lo) << sh;
+          }
+        }
+      }
+    } else {
+      unsure |= (d0 | d1) != 0;
+    }
+  }
+  if (kSilu) {
+    unsure = unsure && !bad;
+    if (kMX) unsure |= __shfl_xor_sync(0xFFFFFFFFu, unsure ? 1 : 0, 1) != 0;
+  }
+  if (bad) {
+    sbyte = kMX ? 0xFFu : 0x7Fu;
+    c = make_uint2(0, 0);
+  }
+  return c;
 }
 
 }  // namespace blut

@@ -49,6 +49,7 @@ constexpr int kEpiWarp0 = 4;   // first of the four epilogue warps
 constexpr int kEpiStage = 2048;  // bytes an epilogue warp transposes in: 32 tokens x 32 rows of 16 bits
 constexpr int kHeader = 1024;  // barriers and flags
 constexpr int kPrefetch = 4;   // blocks of token scales held in registers
+constexpr int kFuseRows = 8;   // most rows that the product quantises itself
 
 template <bool kMX, int NT>
 struct Fp4Cfg {
@@ -83,6 +84,9 @@ struct Fp4Params {
   const uint32_t* xs;
   const float* xg;
   int64_t x_rows;
+  const void* x;    // kFuse: x before quantisation, its row pitch in elements,
+  int64_t x_ld;     // columns, and whether its rows start on 16-byte boundaries
+  int cols, x_vec;
   int n;        // weight rows
   int kblocks;  // 128-column blocks
   int row_tiles;
@@ -354,7 +358,10 @@ __device__ __forceinline__ void reduce_cluster(const Fp4Params& p, const float* 
   }
 }
 
-template <bool kMX, int NT>
+// kFuse: 0, x comes in 4-bit form; 1 + dtype, warps 2, 3 quantise its (at
+// most 8) rows themselves, 16 columns a lane and block: a launch and a pass
+// through memory less, where a call is little else.
+template <bool kMX, int NT, int kFuse>
 __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kernel(const Fp4Params p) {
   using C = Fp4Cfg<kMX, NT>;
   extern __shared__ __align__(1024) uint8_t fp4_smem[];
@@ -375,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
   const auto bring_w = [&](const Fp4Item& t, int b, int it) {
     const int s = it % C::kStages;
     const uint32_t bar = smem_u32(h->wfull + s);
-    mbar_expect_tx(bar, C::kA + 4 * (uint32_t)t.cnt * 16);
+    mbar_expect_tx(bar, C::kA + (kFuse ? 0u : 4 * (uint32_t)t.cnt * 16));
     bulk_g2s(smem_u32(ring + s * C::kStage), p.w + t.expert * p.wstride + ((int64_t)t.tile * p.kblocks + b0 + b) * C::kA,
              C::kA, bar);
   };
@@ -425,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
         for (int c = 0; c < 4; ++c)
           bulk_g2s(dst + c * NT * 16, src + (int64_t)c * p.x_rows * 16, (uint32_t)t.cnt * 16, bar);
       };
-      grid_dependency_wait();  // x may still be in the making; the weights are not
+      if (!kFuse) grid_dependency_wait();  // x may still be in the making; the weights are not
       int it = 0;              // blocks over all items: the ring goes on from one to the next
       bool ok = true;
       for (int i = first; i < items && ok; i += step) {
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
               }
               bring_w(t, b, it);
             }
-            bring_x(t, b, it);
+            if (!kFuse) bring_x(t, b, it);
           }
         }
         ok = __all_sync(0xFFFFFFFFu, ok);
@@ -512,6 +519,64 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
       wait_drain(smem_u32(&h->fin), 0);
     }
     __syncwarp();
+  } else if (kFuse && warp < kEpiWarp0) {
+    // ------------------------------------------------------ x to 4-bit form --
+    if constexpr (kFuse != 0) {
+      constexpr int DT = kFuse - 1;
+      constexpr int kAhead = DT == BLUT_F32 ? 2 : 4;  // blocks of x in registers
+      using T = typename Elem<DT>::T;
+      const int t64 = threadIdx.x - 64, r = t64 >> 3, u = t64 & 7;  // row, and 16 columns of the block's 128
+      grid_dependency_wait();
+      const float g = kMX ? 1.0f : __ldg(p.xg);
+      const uint32_t cdst = C::kA + (u >> 1) * NT * 16 + r * 16 + (u & 1) * 8;
+      const uint32_t sdst = C::kA + C::kB + r * 16 + (kMX ? u >> 1 : (u >> 2) * 512 + (u & 3));
+      bool ok = true;
+      int it = 0;
+      for (int i = first; i < items && ok; i += step) {
+        const Fp4Item t = item_of<NT>(p, i, lane, tab);
+        const bool in = r < t.cnt;
+        const T* src = static_cast<const T*>(p.x) + (int64_t)(t.row0 + (in ? r : 0)) * p.x_ld;
+        Raw<DT> raw[kAhead];
+        const auto fetch = [&](int b, Raw<DT>& w) {
+          const int col = (b0 + b) * 128 + 16 * u;
+          if (p.x_vec && in && b < nb && col + 16 <= p.cols) raw_load<DT, 16>(src + col, w);
+        };
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) fetch(j, raw[j]);
+        for (int c = 0; c < nb && ok; c += kAhead) {
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            const int b = c + j, s = it % C::kStages;
+            if (b < nb && ok) {
+              const int col = (b0 + b) * 128 + 16 * u, n = in ? min(16, max(0, p.cols - col)) : 0;
+              float v[16];
+              if (p.x_vec && n == 16)
+                raw_unpack<DT>(raw[j], v);
+              else
+                load16<DT>(src + col, n, v);
+              fetch(b + kAhead, raw[j]);
+              uint32_t sbyte;
+              bool unsure = false;
+              const uint2 code = encode16<kMX, false>(v, g, unsure, sbyte);
+              if (it >= C::kStages) {
+                ok = wait_or_abort(smem_u32(h->empty + s), (uint32_t)(it / C::kStages - 1) & 1u, abort_flag,
+                                   &g_fp4_status, p.wait_ns);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+              }
+              if (ok) {
+                uint8_t* st = ring + s * C::kStage;
+                *reinterpret_cast<uint2*>(st + cdst) = code;
+                if (!kMX || (u & 1) == 0) st[sdst] = (uint8_t)sbyte;
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(h->sfull + s));
+              }
+              ++it;
+            }
+          }
+        }
+      }
+    }
   } else if (warp < kEpiWarp0) {
     // -------------------------------------------------------- token scales --
     constexpr int kWordsAll = C::kWords * NT;
@@ -640,10 +705,10 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
 
 // early: the launch may begin while the kernel before it, which writes x, is
 // still running (it waits in grid_dependency_wait before it reads x).
-template <bool kMX, int NT>
+template <bool kMX, int NT, int kFuse = 0>
 int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
   using C = Fp4Cfg<kMX, NT>;
-  auto kern = fp4_mm_kernel<kMX, NT>;
+  auto kern = fp4_mm_kernel<kMX, NT, kFuse>;
   constexpr int kMaxSmem = C::kSmem + (2 * kMaxExperts + 2) * 4;
   static std::atomic<int> sms_of[kMaxDevices];  // 0: not set up yet
   const int dev = cache_device();
@@ -681,7 +746,7 @@ int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
 }
 
 template <bool kMX>
-int dispatch(Fp4Params& p, int64_t m, bool early, cudaStream_t stream) {
+int dispatch(Fp4Params& p, int64_t m, int fuse, bool early, cudaStream_t stream) {
   p.row_tiles = (p.n + 127) / 128;
   // tokens per matrix: their number for one matrix, the mean for runs
   const int64_t mean = p.experts ? (m + p.experts - 1) / p.experts : m;
@@ -695,6 +760,11 @@ int dispatch(Fp4Params& p, int64_t m, bool early, cudaStream_t stream) {
   if (nt <= 128)
     while (p.split_log < 3 && (items << p.split_log) * 2 <= (nt <= 64 ? 444 : 296) && p.kblocks >= 4 << p.split_log)
       ++p.split_log;
+  switch (fuse) {
+    case 1 + BLUT_F16: return launch<kMX, 32, 1 + BLUT_F16>(p, items, early, stream);
+    case 1 + BLUT_BF16: return launch<kMX, 32, 1 + BLUT_BF16>(p, items, early, stream);
+    case 1 + BLUT_F32: return launch<kMX, 32, 1 + BLUT_F32>(p, items, early, stream);
+  }
   switch (nt) {
     case 32: return launch<kMX, 32>(p, items, early, stream);
     case 64: return launch<kMX, 64>(p, items, early, stream);
@@ -714,7 +784,8 @@ int fp4_check(const blut_fp4_mm_args* a) {
   return BLUT_OK;
 }
 
-int fp4_product(const blut_fp4_mm_args* a, bool early, cudaStream_t s) {
+// x not null: x's rows are quantised by the product (at most kFuseRows of them).
+int fp4_product(const blut_fp4_mm_args* a, bool early, const void* x, int x_dtype, int64_t x_ld, cudaStream_t s) {
   const int rc = fp4_check(a);
   if (rc != BLUT_OK) return rc;
   Fp4Params p = {};
@@ -734,20 +805,31 @@ int fp4_product(const blut_fp4_mm_args* a, bool early, cudaStream_t s) {
   p.out_dtype = a->out_dtype;
   p.vec = ((uintptr_t)a->y | (uintptr_t)(a->y_ld * (a->out_dtype == BLUT_F32 ? 4 : 2))) % 16 == 0;
   p.wait_ns = wait_limit_ns();
-  return a->w.kind == BLUT_FP4_MX ? dispatch<true>(p, a->x_rows, early, s) : dispatch<false>(p, a->x_rows, early, s);
+  const int fuse = x ? 1 + x_dtype : 0;
+  if (x) {
+    p.x = x;
+    p.x_ld = x_ld;
+    p.cols = (int)a->w.cols;
+    p.x_vec = ((uintptr_t)x | (uintptr_t)(x_ld * (x_dtype == BLUT_F32 ? 4 : 2))) % 16 == 0;
+  }
+  return a->w.kind == BLUT_FP4_MX ? dispatch<true>(p, a->x_rows, fuse, early, s)
+                                  : dispatch<false>(p, a->x_rows, fuse, early, s);
 }
 
-// Workspace of blut_fp4_linear: x in 4-bit form, then its g.
+// Workspace of blut_fp4_linear: x in 4-bit form (unless the product quantises
+// it), then its g (unless it is given or there is none).
 struct LinearWs {
   int64_t scales, g, total;
 };
-LinearWs linear_ws(const blut_fp4_desc& w, int64_t m) {
+LinearWs linear_ws(const blut_fp4_desc& w, int64_t m, bool given) {
   blut_fp4_desc d = w;
   d.rows = m;
-  LinearWs l;
-  l.scales = align256(blut_fp4_codes_bytes(&d));
-  l.g = l.scales + align256(blut_fp4_scales_bytes(&d));
-  l.total = l.g + 256;
+  LinearWs l = {};
+  if (m > kFuseRows) {
+    l.scales = align256(blut_fp4_codes_bytes(&d));
+    l.g = l.scales + align256(blut_fp4_scales_bytes(&d));
+  }
+  l.total = l.g + (w.kind == BLUT_FP4_NV && !given ? 256 : 0);
   return l;
 }
 
@@ -759,24 +841,28 @@ using namespace blut;
 extern "C" {
 
 int blut_fp4_matmul(const blut_fp4_mm_args* a, void* stream) {
-  return fp4_product(a, false, reinterpret_cast<cudaStream_t>(stream));
+  return fp4_product(a, false, nullptr, 0, 0, reinterpret_cast<cudaStream_t>(stream));
 }
 
-size_t blut_fp4_linear_workspace_size(const blut_fp4_desc* w, int64_t x_rows) {
-  if (!w || !fp4_valid(*w) || x_rows <= 0 || x_rows > kMaxSlots) return 0;
-  return (size_t)linear_ws(*w, x_rows).total;
+int64_t blut_fp4_linear_workspace_size(const blut_fp4_desc* w, int64_t x_rows, int32_t scale_given) {
+  if (!w || !fp4_valid(*w) || x_rows <= 0 || x_rows > kMaxSlots) return BLUT_ERR_INVALID;
+  return linear_ws(*w, x_rows, scale_given != 0).total;
 }
 
 int blut_fp4_linear(const blut_fp4_mm_args* args, const void* x, int32_t x_dtype, int64_t x_ld, void* workspace,
                     size_t workspace_bytes, void* stream) {
-  if (!args || !fp4_valid(args->w) || !x || !workspace || (uintptr_t)workspace % 16) return BLUT_ERR_INVALID;
-  if (args->x_rows <= 0 || args->x_rows > kMaxSlots || args->num_experts) return BLUT_ERR_INVALID;
-  const LinearWs ws = linear_ws(args->w, args->x_rows);
-  if (workspace_bytes < (size_t)ws.total) return BLUT_ERR_WORKSPACE;
-  uint8_t* base = static_cast<uint8_t*>(workspace);
+  if (!args || !fp4_valid(args->w) || !x || (uintptr_t)workspace % 16) return BLUT_ERR_INVALID;
+  if (args->x_rows <= 0 || args->x_rows > kMaxSlots || args->num_experts || x_ld < args->w.cols) return BLUT_ERR_INVALID;
+  if (x_dtype != BLUT_F16 && x_dtype != BLUT_BF16 && x_dtype != BLUT_F32) return BLUT_ERR_UNSUPPORTED;
+  if ((uintptr_t)x % (x_dtype == BLUT_F32 ? 4 : 2)) return BLUT_ERR_INVALID;
   blut_fp4_mm_args a = *args;
-  a.x_codes = base;
-  a.x_scales = base + ws.scales;
+  if (a.w.kind == BLUT_FP4_MX) a.x_scale = nullptr;
+  const LinearWs ws = linear_ws(a.w, a.x_rows, a.x_scale != nullptr);
+  if (ws.total && (!workspace || workspace_bytes < (size_t)ws.total)) return BLUT_ERR_WORKSPACE;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  const bool fuse = a.x_rows <= kFuseRows;
+  a.x_codes = fuse ? a.w_tiled : base;  // not read where the product quantises x
+  a.x_scales = fuse ? a.w_tiled : base + ws.scales;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int rc = fp4_check(&a);
   if (rc != BLUT_OK) return rc;
@@ -785,13 +871,12 @@ int blut_fp4_linear(const blut_fp4_mm_args* args, const void* x, int32_t x_dtype
     rc = blut_fp4_global_scale(x, x_dtype, a.x_rows, a.w.cols, x_ld, 0, g, stream);
     if (rc != BLUT_OK) return rc;
     a.x_scale = g;
-  } else if (a.w.kind == BLUT_FP4_MX) {
-    a.x_scale = nullptr;
   }
+  if (fuse) return fp4_product(&a, false, x, x_dtype, x_ld, s);
   blut_fp4_desc d = a.w;
   d.rows = a.x_rows;
   rc = fp4_quantize_for_product(d, x, x_dtype, x_ld, a.x_scale, base, base + ws.scales, s);
-  return rc == BLUT_OK ? fp4_product(&a, true, s) : rc;
+  return rc == BLUT_OK ? fp4_product(&a, true, nullptr, 0, 0, s) : rc;
 }
 
 int blut_fp4_check_status(void* stream) {

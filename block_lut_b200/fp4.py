@@ -460,14 +460,15 @@ class FP4Linear:
             lib = _lib.lib()
             need = self._ws.get(m)
             if need is None:
-                need = self._ws[m] = int(lib.blut_fp4_linear_workspace_size(C.byref(_desc(w.kind, w.rows, w.cols)), m))
-                if need == 0:
-                    raise ValueError(f"at most {MAX_ROWS} rows in one product")
+                need = self._ws[m] = int(lib.blut_fp4_linear_workspace_size(C.byref(_desc(w.kind, w.rows, w.cols)), m,
+                                                                            int(self.act_scale is not None)))
+            if need < 0:
+                raise ValueError(f"at most {MAX_ROWS} rows in one product")
             a = _lib.FP4MMArgs.from_buffer_copy(self._args)  # calls from several host threads never share one
             a.x_rows, a.y, a.y_ld, a.out_dtype = m, y.data_ptr(), _pitch(y), _DT[y.dtype]
-            ws = torch.empty(need, dtype=torch.uint8, device=x2.device)
+            ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
             with _lib.on_device(x2):
-                _lib.check(lib.blut_fp4_linear(C.byref(a), x2.data_ptr(), _DT[x2.dtype], _pitch(x2), ws.data_ptr(), need,
+                _lib.check(lib.blut_fp4_linear(C.byref(a), x2.data_ptr(), _DT[x2.dtype], _pitch(x2), _p(ws), need,
                                                _lib.stream_ptr(stream)), "fp4_linear")
         if out is not None:
             return out

@@ -530,13 +530,16 @@ typedef struct {
  * float32 accumulation on the tensor cores, one launch, no workspace; the
  * result does not depend on timing. */
 BLUT_API int blut_fp4_matmul(const blut_fp4_mm_args* args, void* stream);
-/* y = x W^T for 16- or 32-bit x [x_rows][cols] (pitch x_ld): blut_fp4_quantize
- * and the product in one call; the product's weight copies start while x is
- * still being quantised.  args as for one matrix; x_codes and x_scales are
- * ignored, x_scale NULL (NV) takes x's own maximum (blut_fp4_global_scale).
- * The workspace (16-byte aligned) holds x in 4-bit form; calls that can
- * overlap need one each. */
-BLUT_API size_t blut_fp4_linear_workspace_size(const blut_fp4_desc* w, int64_t x_rows);
+/* y = x W^T for 16- or 32-bit x [x_rows][cols] (pitch x_ld), the result of
+ * blut_fp4_quantize and blut_fp4_matmul in one call: up to 8 rows are
+ * quantised inside the product, more before it, with the product's weight
+ * copies starting meanwhile.  args as for one matrix; x_codes and x_scales
+ * are ignored, x_scale NULL (NV) takes x's own maximum
+ * (blut_fp4_global_scale).  The workspace (16-byte aligned;
+ * blut_fp4_linear_workspace_size bytes, which may be 0: NULL then, < 0 for
+ * invalid arguments; scale_given: x_scale is not NULL) is free again when
+ * the work is done; calls that can overlap need one each. */
+BLUT_API int64_t blut_fp4_linear_workspace_size(const blut_fp4_desc* w, int64_t x_rows, int32_t scale_given);
 BLUT_API int blut_fp4_linear(const blut_fp4_mm_args* args, const void* x, int32_t x_dtype, int64_t x_ld,
                              void* workspace, size_t workspace_bytes, void* stream);
 /* Reads and clears the device status of this device's blut_fp4_matmul calls:

@@ -51,6 +51,35 @@ def test_matmul(kind, m, n, k):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k", [(3, 60000, 640), (40, 50000, 384), (100, 30000, 1408), (700, 20000, 640), (1500, 9000, 2048)])
+def test_matmul_many_items(kind, m, n, k):
+    """More tiles than CTAs run at once: the rings and the accumulator go on from one to the next."""
+    F = fp4()
+    xq, x = operand(m, k, kind, 1)
+    wq, w = operand(n, k, kind, 2, 0.05)
+    W = F.FP4Weight.from_quantized(wq)
+    check(F.fp4_matmul(xq, W, out_dtype=torch.float32), x, w, "float32")
+    check(F.fp4_matmul(xq, W), x, w, "bfloat16")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,k", [(200, 500), (1000, 4096), (60000, 1408), (129, 33)])
+def test_linear_is_quantize_then_matmul(kind, dtype, n, k):
+    """Bit for bit, on both sides of the number of rows that the product quantises itself, for any row pitch."""
+    F = fp4()
+    W = F.FP4Weight.quantize(torch.randn(n, k, generator=gen(5), device="cuda") * 0.05, kind)
+    for scale in (None, 0.0025) if kind == "nvfp4" else (None,):
+        lin = F.FP4Linear(W, scale)
+        for m in (1, 2, 7, 8, 9, 33):
+            big = torch.randn(m, k + 11, generator=gen(m), device="cuda").to(dtype)
+            for x in (big[:, :k].contiguous(), big[:, 3:3 + k]):
+                want = F.fp4_matmul(F.quantize_fp4(x, kind, scale), W, out_dtype=dtype)
+                assert torch.equal(lin(x), want), (m, scale)
+    F.fp4_check_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_every_element_has_its_place(kind):
     """One nonzero weight column and one nonzero token at a time would take long; a rank-one pattern of distinct
     powers shows a swapped row, token, block or half just as well."""
