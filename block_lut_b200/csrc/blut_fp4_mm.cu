@@ -300,10 +300,12 @@ __device__ __forceinline__ void tc_ld_16x32(uint32_t taddr, uint32_t (&v)[16]) {
 // An epilogue warp's 32 weight rows x cnt tokens as 16-bit rows of y: pairs
 // of tokens are packed as an mma accumulator holds them, stmatrix transposes
 // 8 x 8 of them at a time, and a store then covers 32 rows of 8 tokens, 16
-// bytes a lane.  y: token 0, the warp's first row.
+// bytes a lane.  y: token 0, the warp's first row, of which `left` are rows
+// of the matrix; vec: rows of y start on 16-byte boundaries.
 template <int kOut>
 __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha, uint8_t* stage, uint16_t* y,
-                                             int64_t ldy, int lane) {
+                                             int64_t ldy, int left, bool vec, int lane) {
+  const int mine = min(8, left - (lane & 3) * 8);  // rows of this lane's piece
   const uint32_t saddr = smem_u32(stage);
 #pragma unroll 1
   for (int c = 0; c < cnt; c += 32) {
@@ -331,9 +333,17 @@ __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int t = 8 * j + (lane >> 2);
-      if (c + t < cnt)
-        *reinterpret_cast<uint4*>(y + (int64_t)(c + t) * ldy + (lane & 3) * 8) =
-            *reinterpret_cast<const uint4*>(stage + t * 64 + ((lane & 3) ^ ((t >> 1) & 3)) * 16);
+      if (c + t >= cnt) continue;
+      const uint4 w = *reinterpret_cast<const uint4*>(stage + t * 64 + ((lane & 3) ^ ((t >> 1) & 3)) * 16);
+      uint16_t* dst = y + (int64_t)(c + t) * ldy + (lane & 3) * 8;
+      if (vec && mine == 8) {
+        *reinterpret_cast<uint4*>(dst) = w;
+      } else {
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < mine) dst[k] = (uint16_t)(words[k >> 1] >> (16 * (k & 1)));
+      }
     }
     __syncwarp();
   }
@@ -644,12 +654,14 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
                                                  p.wait_ns)))
         break;
       tc_fence_after();
-      if (p.vec && p.out_dtype != BLUT_F32 && row + 32 <= p.n) {
+      const int left = (int)min((int64_t)32, p.n - row);  // rows of the matrix among this warp's
+      if (left <= 0) {
+      } else if (p.out_dtype != BLUT_F32) {
         uint16_t* y = static_cast<uint16_t*>(p.y) + (int64_t)t.row0 * p.ldy + row;
         if (p.out_dtype == BLUT_BF16)
-          store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, lane);
+          store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane);
         else
-          store_tile16<BLUT_F16>(tcol, t.cnt, alpha, stage, y, p.ldy, lane);
+          store_tile16<BLUT_F16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane);
       } else {
 #pragma unroll 1
         for (int c = 0; c < t.cnt; c += 16) {
