@@ -47,6 +47,18 @@ def _desc(kind: str, rows: int, cols: int) -> _lib.FP4Desc:
     return _lib.FP4Desc(_KIND[kind], 0, int(rows), int(cols))
 
 
+def _launch(what: str, t: torch.Tensor, stream, *args) -> None:
+    """The library's ``blut_<what>`` on t's device and the given (default: current) stream."""
+    fn = getattr(_lib.lib(), "blut_" + what)
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.stream_ptr(stream))
+    _lib.check(rc, what)
+
+
 def _rows2d(x: torch.Tensor, what: str) -> torch.Tensor:
     """x as a CUDA matrix with contiguous rows (any row pitch), copied only when its rows are not."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
@@ -55,7 +67,7 @@ def _rows2d(x: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError(f"{what} must be float16, bfloat16 or float32, not {x.dtype}")
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"{what} must be a matrix [rows, columns] with at least one column")
-    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:  # transposed, expanded, overlapping rows
+    if not x.is_contiguous() and (x.stride(1) != 1 or x.stride(0) < x.shape[1]):  # transposed, expanded, overlapping
         x = x.contiguous()
     return x
 
@@ -135,10 +147,7 @@ class FP4Matrix:
         scales = torch.empty(self.rows, nb, dtype=torch.uint8, device=self.data.device)
         if self.rows:
             d = _desc(self.kind, self.rows, self.cols)
-            with _lib.on_device(codes):
-                _lib.check(_lib.lib().blut_fp4_export(C.byref(d), *self._ptrs(),
-                                                      codes.data_ptr(), scales.data_ptr(), _lib.stream_ptr(stream)),
-                           "fp4_export")
+            _launch("fp4_export", codes, stream, C.byref(d), *self._ptrs(), codes.data_ptr(), scales.data_ptr())
         return codes, scales
 
 
@@ -157,9 +166,7 @@ def _import(kind, codes, scales, cols, global_scale, stream=None) -> FP4Matrix:
     g = _given_scale(kind, global_scale, codes.device)
     m = FP4Matrix.empty(kind, rows, cols, codes.device, g)
     if rows:
-        with _lib.on_device(codes):
-            _lib.check(_lib.lib().blut_fp4_import(C.byref(d), codes.data_ptr(), scales.data_ptr(), *m._ptrs(),
-                                                  _lib.stream_ptr(stream)), "fp4_import")
+        _launch("fp4_import", codes, stream, C.byref(d), codes.data_ptr(), scales.data_ptr(), *m._ptrs())
     return m
 
 
@@ -180,10 +187,8 @@ def fp4_global_scale(x: torch.Tensor, silu_mul: bool = False, stream=None) -> to
     buf = torch.empty(4, dtype=torch.float32, device=x.device)
     if x.shape[0] == 0:
         return buf.fill_(MIN_GLOBAL_SCALE)[:1]
-    with _lib.on_device(x):
-        _lib.check(_lib.lib().blut_fp4_global_scale(x.data_ptr(), _DT[x.dtype], x.shape[0], cols, _pitch(x),
-                                                    int(silu_mul), buf.data_ptr(), _lib.stream_ptr(stream)),
-                   "fp4_global_scale")
+    _launch("fp4_global_scale", x, stream, x.data_ptr(), _DT[x.dtype], x.shape[0], cols, _pitch(x), int(silu_mul),
+            buf.data_ptr())
     return buf[:1]
 
 
@@ -224,10 +229,8 @@ def quantize_fp4(x: torch.Tensor, kind: str = "nvfp4", global_scale: Scale = Non
         return m
     if x.shape[0] == 0:
         raise ValueError("row_index into an x without rows")
-    with _lib.on_device(x):
-        _lib.check(_lib.lib().blut_fp4_quantize(C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(row_index),
-                                                x.shape[0], _p(g), *m._ptrs(), _lib.stream_ptr(stream)),
-                   "fp4_quantize")
+    _launch("fp4_quantize", x, stream, C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(row_index), x.shape[0], _p(g),
+            *m._ptrs())
     return m
 
 
@@ -243,10 +246,7 @@ def silu_mul_quantize_fp4(gate_up: torch.Tensor, kind: str = "nvfp4", global_sca
     m = FP4Matrix.empty(kind, x.shape[0], cols, x.device, g)
     if x.shape[0] == 0:
         return m
-    with _lib.on_device(x):
-        _lib.check(_lib.lib().blut_fp4_silu_mul_quantize(C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(g),
-                                                         *m._ptrs(), _lib.stream_ptr(stream)),
-                   "fp4_silu_mul_quantize")
+    _launch("fp4_silu_mul_quantize", x, stream, C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(g), *m._ptrs())
     return m
 
 
@@ -259,9 +259,7 @@ def dequantize_fp4(q: FP4Matrix, dtype: torch.dtype = torch.bfloat16, stream=Non
     if q.rows == 0:
         return out
     d = _desc(q.kind, q.rows, q.cols)
-    with _lib.on_device(out):
-        _lib.check(_lib.lib().blut_fp4_dequantize(C.byref(d), *q._ptrs(), _p(q.global_scale), out.data_ptr(),
-                                                  _DT[dtype], q.cols, _lib.stream_ptr(stream)), "fp4_dequantize")
+    _launch("fp4_dequantize", out, stream, C.byref(d), *q._ptrs(), _p(q.global_scale), out.data_ptr(), _DT[dtype], q.cols)
     return out
 
 
@@ -317,10 +315,8 @@ def _pack(mats, stream=None) -> FP4Weight:
         raise ValueError(f"no 4-bit weight layout for [{m0.rows}, {m0.cols}]")
     dev = m0.data.device
     tiled = torch.empty(len(mats) * stride, dtype=torch.uint8, device=dev)
-    with _lib.on_device(tiled):
-        for i, m in enumerate(mats):
-            _lib.check(_lib.lib().blut_fp4_pack_tiled(C.byref(d), *m._ptrs(), tiled.data_ptr() + i * stride,
-                                                      _lib.stream_ptr(stream)), "fp4_pack_tiled")
+    for i, m in enumerate(mats):
+        _launch("fp4_pack_tiled", tiled, stream, C.byref(d), *m._ptrs(), tiled.data_ptr() + i * stride)
     g = None if m0.kind == "mxfp4" else torch.cat([m.global_scale.reshape(1) for m in mats])
     return FP4Weight(m0.kind, m0.rows, m0.cols, None if single else len(mats), tiled, stride, g)
 
@@ -384,8 +380,7 @@ def _product(x: FP4Matrix, w: FP4Weight, offsets, out, out_dtype, stream) -> tor
     a.x_codes, a.x_scales = x._ptrs()
     a.x_scale = _p(x.global_scale)
     a.x_rows, a.y, a.y_ld = x.rows, out.data_ptr(), _pitch(out)
-    with _lib.on_device(out):
-        _lib.check(_lib.lib().blut_fp4_matmul(C.byref(a), _lib.stream_ptr(stream)), "fp4_matmul")
+    _launch("fp4_matmul", out, stream, C.byref(a))
     return out
 
 
@@ -454,22 +449,20 @@ class FP4Linear:
             y = out if out.dim() == 2 else out.view(-1, self.rows)
             _check_out(y, m, w, out_dtype)
         else:
+            if out_dtype is not None and out_dtype not in _DT:
+                raise ValueError("the output is float16, bfloat16 or float32")
             y = torch.empty((m, self.rows), dtype=out_dtype or x2.dtype, device=x2.device)
-            _check_out(y, m, w, out_dtype)
         if m:
-            lib = _lib.lib()
             need = self._ws.get(m)
             if need is None:
-                need = self._ws[m] = int(lib.blut_fp4_linear_workspace_size(C.byref(_desc(w.kind, w.rows, w.cols)), m,
-                                                                            int(self.act_scale is not None)))
+                need = self._ws[m] = int(_lib.lib().blut_fp4_linear_workspace_size(
+                    C.byref(_desc(w.kind, w.rows, w.cols)), m, int(self.act_scale is not None)))
             if need < 0:
                 raise ValueError(f"at most {MAX_ROWS} rows in one product")
             a = _lib.FP4MMArgs.from_buffer_copy(self._args)  # calls from several host threads never share one
             a.x_rows, a.y, a.y_ld, a.out_dtype = m, y.data_ptr(), _pitch(y), _DT[y.dtype]
             ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
-            with _lib.on_device(x2):
-                _lib.check(lib.blut_fp4_linear(C.byref(a), x2.data_ptr(), _DT[x2.dtype], _pitch(x2), _p(ws), need,
-                                               _lib.stream_ptr(stream)), "fp4_linear")
+            _launch("fp4_linear", x2, stream, C.byref(a), x2.data_ptr(), _DT[x2.dtype], _pitch(x2), _p(ws), need)
         if out is not None:
             return out
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.rows)
