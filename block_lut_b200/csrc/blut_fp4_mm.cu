@@ -433,37 +433,46 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer --
+    // Converged, like the MMA warp below, with one lane issuing: a copy issued
+    // by a lone lane costs as much as the data it brings takes.
     if (first < items) {
-      const auto bring_x = [&](const Fp4Item& t, int b, int it) {
-        const int s = it % C::kStages;
-        const uint32_t bar = smem_u32(h->wfull + s), dst = smem_u32(ring + s * C::kStage + C::kA);
-        const uint8_t* src = p.xc + ((int64_t)(b0 + b) * 4 * p.x_rows + t.row0) * 16;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          bulk_g2s(dst + c * NT * 16, src + (int64_t)c * p.x_rows * 16, (uint32_t)t.cnt * 16, bar);
-      };
       if (!kFuse) grid_dependency_wait();  // x may still be in the making; the weights are not
-      int it = 0;              // blocks over all items: the ring goes on from one to the next
+      const uint32_t ring_addr = smem_u32(ring), full_addr = smem_u32(h->wfull);
+      const int64_t xstep = p.x_rows * 16;
+      const bool leader = elect_one();
+      int it = 0;  // blocks over all items: the ring goes on from one to the next
       bool ok = true;
       for (int i = first; i < items && ok; i += step) {
         const Fp4Item t = i == first ? t0 : item_of<NT>(p, i, lane, tab);
-        if (lane == 0) {
-          for (int b = 0; b < nb; ++b, ++it) {
-            if (it >= started) {
-              const int s = it % C::kStages;
-              if (it >= C::kStages && !wait_or_abort(smem_u32(h->empty + s), (uint32_t)(it / C::kStages - 1) & 1u,
-                                                     abort_flag, &g_fp4_status, p.wait_ns)) {
-                ok = false;
-                break;
-              }
-              bring_w(t, b, it);
-            }
-            if (!kFuse) bring_x(t, b, it);
+        const uint8_t* wsrc = p.w + t.expert * p.wstride + ((int64_t)t.tile * p.kblocks + b0) * C::kA;
+        const uint8_t* xsrc = p.xc + ((int64_t)b0 * 4 * p.x_rows + t.row0) * 16;
+        const uint32_t xbytes = (uint32_t)t.cnt * 16;
+        for (int b = 0; b < nb; ++b, ++it, wsrc += C::kA) {
+          const int s = it % C::kStages;
+          if (it >= C::kStages) {
+            ok = __all_sync(0xFFFFFFFFu, wait_or_abort(smem_u32(h->empty + s), (uint32_t)(it / C::kStages - 1) & 1u,
+                                                       abort_flag, &g_fp4_status, p.wait_ns));
+            if (!ok) break;
           }
+          const uint32_t bar = full_addr + 8 * s, dst = ring_addr + s * C::kStage;
+          if (leader) {
+            if (it >= started) {
+              mbar_expect_tx(bar, C::kA + (kFuse ? 0u : 4 * xbytes));
+              bulk_g2s(dst, wsrc, C::kA, bar);
+            }
+            if (!kFuse) {
+              bulk_g2s(dst + C::kA, xsrc, xbytes, bar);
+              bulk_g2s(dst + C::kA + NT * 16, xsrc + xstep, xbytes, bar);
+              bulk_g2s(dst + C::kA + 2 * NT * 16, xsrc + 2 * xstep, xbytes, bar);
+              bulk_g2s(dst + C::kA + 3 * NT * 16, xsrc + 3 * xstep, xbytes, bar);
+            }
+          }
+          __syncwarp();
+          xsrc += 4 * xstep;
         }
-        ok = __all_sync(0xFFFFFFFFu, ok);
       }
-      if (lane == 0)  // whatever the other roles do, no copy is in flight when the CTA ends
+      // whatever the other roles do, no copy is in flight when the CTA ends
+      if (lane == 0)
         for (int j = max(0, it - C::kStages); j < it; ++j)
           wait_drain(smem_u32(h->wfull + j % C::kStages), (uint32_t)(j / C::kStages) & 1u);
       __syncwarp();
