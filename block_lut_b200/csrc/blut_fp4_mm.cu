@@ -19,8 +19,8 @@
 //    replicated to the four lane quarters) and issues two tcgen05.mma of
 //    K = 64, kind::mxf4nvf4 (a scale per 16) or kind::mxf4 (a scale per 32),
 //    M = 128, N = the tile's tokens rounded to 16;
-//  * warps 4 .. 7 turn a finished accumulator into rows of y, a lane quarter
-//    each, while the others run ahead into the next item.
+//  * the warps from 4 on turn a finished accumulator into rows of y, a lane
+//    quarter each, while the others run ahead into the next item.
 //
 // Where there are few tiles, a cluster of 2, 4 or 8 CTAs splits K: each leaves
 // its partial tile in its shared memory and sums a share of the tokens over
@@ -44,8 +44,7 @@ namespace {
 
 __device__ int g_fp4_status;
 
-constexpr int kThreads = 256;
-constexpr int kEpiWarp0 = 4;   // first of the four epilogue warps
+constexpr int kEpiWarp0 = 4;   // first epilogue warp
 constexpr int kEpiStage = 2048;  // bytes an epilogue warp transposes in: 32 tokens x 32 rows of 16 bits
 constexpr int kHeader = 1024;  // barriers and flags
 constexpr int kPrefetch = 4;   // blocks of token scales held in registers
@@ -62,8 +61,12 @@ struct Fp4Cfg {
   // Two CTAs per SM (three for few tokens) keep copies in flight while one of
   // them starts or stores.
   static constexpr int kCtas = NT <= 64 ? 3 : 2;
-  static constexpr int kFixed = kHeader + 4 * kEpiStage;
-  static constexpr int kStages = ((kCtas == 3 ? 73 * 1024 : 111 * 1024) - kFixed) / kStage;
+  // Epilogue warps per lane quarter: two where an item has many tokens, since
+  // the accumulator is not free for the next item before it is read.
+  static constexpr int kEpi = NT > 128 ? 2 : 1;
+  static constexpr int kThreads = 32 * (kEpiWarp0 + 4 * kEpi);
+  static constexpr int kFixed = kHeader + 4 * kEpi * kEpiStage;
+  static constexpr int kStages = ((kCtas == 3 ? 73 * 1024 : 112 * 1024) - kFixed) / kStage;
   static constexpr int kSmem = kFixed + kStages * kStage;  // and the table of runs, launch()
   // Tensor memory: NT accumulator columns, then slots of scales; a slot holds
   // one block, 4 columns per word for the weights and for each token group.
@@ -301,14 +304,15 @@ __device__ __forceinline__ void tc_ld_16x32(uint32_t taddr, uint32_t (&v)[16]) {
 // of tokens are packed as an mma accumulator holds them, stmatrix transposes
 // 8 x 8 of them at a time, and a store then covers 32 rows of 8 tokens, 16
 // bytes a lane.  y: token 0, the warp's first row, of which `left` are rows
-// of the matrix; vec: rows of y start on 16-byte boundaries.
+// of the matrix; vec: rows of y start on 16-byte boundaries; c0, cstep: the
+// warp's stretches of 32 tokens.
 template <int kOut>
 __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha, uint8_t* stage, uint16_t* y,
-                                             int64_t ldy, int left, bool vec, int lane) {
+                                             int64_t ldy, int left, bool vec, int lane, int c0, int cstep) {
   const int mine = min(8, left - (lane & 3) * 8);  // rows of this lane's piece
   const uint32_t saddr = smem_u32(stage);
 #pragma unroll 1
-  for (int c = 0; c < cnt; c += 32) {
+  for (int c = c0; c < cnt; c += cstep) {
     uint32_t v[2][16];
     tc_ld_16x32(tcol + c, v[0]);
     tc_ld_16x32(tcol + c + (16u << 16), v[1]);
@@ -352,7 +356,7 @@ __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha
 // This CTA's share of the tokens, summed over the cluster's partial tiles in
 // rank order.  A thread takes 4 rows of a token; its loads are in flight
 // together.
-template <int S>
+template <int S, int kThreads>
 __device__ __forceinline__ void reduce_cluster(const Fp4Params& p, const float* part, int rank, int cnt, int64_t row0,
                                                int64_t col0, float alpha) {
   const int quad = 4 * (threadIdx.x & 31);
@@ -372,13 +376,13 @@ __device__ __forceinline__ void reduce_cluster(const Fp4Params& p, const float* 
 // most 8) rows themselves, 16 columns a lane and block: a launch and a pass
 // through memory less, where a call is little else.
 template <bool kMX, int NT, int kFuse>
-__global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kernel(const Fp4Params p) {
+__global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kernel(const Fp4Params p) {
   using C = Fp4Cfg<kMX, NT>;
   extern __shared__ __align__(1024) uint8_t fp4_smem[];
   Fp4Header* h = reinterpret_cast<Fp4Header*>(fp4_smem);
   uint8_t* ring = fp4_smem + kHeader;
   uint8_t* epi = ring + C::kStages * C::kStage;
-  int* tab = reinterpret_cast<int*>(epi + 4 * kEpiStage);
+  int* tab = reinterpret_cast<int*>(epi + 4 * C::kEpi * kEpiStage);
   volatile int* abort_flag = &h->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = 1 << p.split_log;
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
         mbar_init(smem_u32(h->empty + s), 1);
       }
       mbar_init(smem_u32(&h->acc_full), 1);
-      mbar_init(smem_u32(&h->acc_empty), 4);
+      mbar_init(smem_u32(&h->acc_empty), 4 * C::kEpi);
       mbar_init(smem_u32(&h->fin), 1);
       h->abort_flag = 0;
       fence_mbar_init();
@@ -649,8 +653,8 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
     }
   } else if (split == 1) {
     // ------------------------------------------------------------ epilogue --
-    const int q = warp - kEpiWarp0;
-    uint8_t* stage = epi + q * kEpiStage;
+    const int q = warp & 3, part = (warp - kEpiWarp0) >> 2;  // lane quarter (a warp may read its own only), share
+    uint8_t* stage = epi + (warp - kEpiWarp0) * kEpiStage;
     const uint32_t tcol = tmem + ((uint32_t)(32 * q) << 16);
     grid_dependency_wait();
     const float gx = p.xg ? __ldg(p.xg) : 1.0f;
@@ -668,12 +672,12 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
       } else if (p.out_dtype != BLUT_F32) {
         uint16_t* y = static_cast<uint16_t*>(p.y) + (int64_t)t.row0 * p.ldy + row;
         if (p.out_dtype == BLUT_BF16)
-          store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane);
+          store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi);
         else
-          store_tile16<BLUT_F16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane);
+          store_tile16<BLUT_F16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi);
       } else {
 #pragma unroll 1
-        for (int c = 0; c < t.cnt; c += 16) {
+        for (int c = 16 * part; c < t.cnt; c += 16 * C::kEpi) {
           uint32_t v[16];
           tc_ld16(tcol + c, v);
           tc_wait_ld16(v);
@@ -694,8 +698,8 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
     float* part = reinterpret_cast<float*>(ring);  // free: the last MMA has read it
     bool ok = __all_sync(0xFFFFFFFFu, wait_or_abort(smem_u32(&h->acc_full), 0, abort_flag, &g_fp4_status, p.wait_ns));
     tc_fence_after();
-    if (warp >= kEpiWarp0 && ok) {
-      const int q = warp - kEpiWarp0;
+    if (warp >= kEpiWarp0 && ok) {  // (K is split for NT <= 128 only: four warps)
+      const int q = warp & 3;
 #pragma unroll 1
       for (int c = 0; c < t.cnt; c += 16) {
         uint32_t v[16];
@@ -710,11 +714,11 @@ __global__ void __launch_bounds__(kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kerne
     const float alpha = (p.xg ? __ldg(p.xg) : 1.0f) * (p.wg ? __ldg(p.wg + t.expert) : 1.0f);
     if (ok) {
       if (split == 2)
-        reduce_cluster<2>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
+        reduce_cluster<2, C::kThreads>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
       else if (split == 4)
-        reduce_cluster<4>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
+        reduce_cluster<4, C::kThreads>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
       else
-        reduce_cluster<8>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
+        reduce_cluster<8, C::kThreads>(p, part, rank, t.cnt, t.row0, (int64_t)t.tile * 128, alpha);
     }
     cluster_sync();  // no CTA leaves while another still reads its partial tile
   }
@@ -747,7 +751,7 @@ int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   // one CTA (cluster) per item where K is split, else as many as run at once
   cfg.gridDim = dim3((unsigned)(split > 1 ? items * split : std::min<int64_t>(items, (int64_t)sms * C::kCtas)));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem + (p.experts ? (2 * p.experts + 2) * 4 : 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
