@@ -11,9 +11,10 @@
 // computed from x * (1 / (s g)) twice, with the reciprocal moved up and down
 // by 2^-21, more than its error; where both give the same code, no border
 // lies between them and the code is right.  Where they differ, the border is
-// compared with x in float64, in which border * s * g (2 + 4 + 24 bits) is
-// exact.  Borders are met often when g is a power of two (0.8 % of bf16
-// values are ties) and cost a few instructions each.  silu(gate) * up is
+// compared with x by one fused multiply-add, whose sign is exact (border * s
+// has 7 bits).  Borders are met often when g is a power of two or comes from
+// x's own maximum (0.8 % of bf16 values are ties) and cost a few instructions
+// each.  silu(gate) * up is
 // rounded once, to its code: it is computed in float32 from the hardware's
 // approximate exponential and reciprocal (relative error below 2^-18, window
 // 2^-17); a block with a value near a border is done again in float64, a
@@ -64,7 +65,7 @@ __device__ __noinline__ void encode_block_f64(const typename Elem<DT>::T* row, i
     s = m > 0.0 ? (uint32_t)(min(max(ilogb(m) - 2, -127), 127) + 127) : 0u;
     unit = ldexp(1.0, (int)s - 127);
   } else {
-    s = e4m3_scale(m, g, (float)(m / (6.0 * (double)g)));
+    s = e4m3_scale_f64(m, g);
     unit = (double)e4m3_f32(s) * (double)g;
   }
   uint32_t q = 0;
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(32 * kQWarps, kPer > 1 ? 4 : 1)
       }
     }
     uint32_t sbyte;
-    uint2 c = encode16<kMX, kSilu>(v, g, unsure, sbyte);
+    uint2 c = encode16<DT, kMX, kSilu>(v, g, unsure, sbyte);
     const int r = warp + kQWarps * i;
     if constexpr (kSilu) {
       for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, unsure); todo;) {

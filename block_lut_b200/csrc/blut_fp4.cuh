@@ -177,13 +177,30 @@ __device__ __forceinline__ uint32_t e4m3x2_sat(float hi, float lo) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
   return d;
 }
+// Neighbouring codes lo and hi (lo = hi: decided) for a quotient at border /
+// unit of them: hi where x is past the border, the even one on it.  A border
+// times its small factor (at most 7 bits) is exact, so the sign of the fused
+// difference is that of x - border * factor * g.
+__device__ __forceinline__ bool past_border(float x, float border, float g, uint32_t lo) {
+  const float d = fmaf(-border, g, x);
+  return d > 0.0f || (d == 0.0f && (lo & 1));
+}
 // e4m3(a / (6 g)) by the exact quotient; t is that quotient up to 2^-21.
-__device__ __forceinline__ uint32_t e4m3_scale(double a, float g, float t) {
+__device__ __forceinline__ uint32_t e4m3_scale(float a, float g, float t) {
+  const uint32_t both = e4m3x2_sat(t * (1.0f + 0x1p-20f), t * (1.0f - 0x1p-20f));
+  uint32_t lo = both & 0xFFu;
+  const uint32_t hi = both >> 8;
+  if (lo != hi && past_border(a, 3.0f * (e4m3_f32(lo) + e4m3_f32(hi)), g, lo)) lo = hi;
+  return lo;
+}
+// The same of a float64 value.
+__device__ __forceinline__ uint32_t e4m3_scale_f64(double a, float g) {
+  const float t = (float)(a / (6.0 * (double)g));
   const uint32_t both = e4m3x2_sat(t * (1.0f + 0x1p-20f), t * (1.0f - 0x1p-20f));
   uint32_t lo = both & 0xFFu;
   const uint32_t hi = both >> 8;
   if (lo != hi) {
-    const double border = 0.5 * ((double)e4m3_f32(lo) + (double)e4m3_f32(hi)) * (6.0 * (double)g);
+    const double border = 3.0 * ((double)e4m3_f32(lo) + (double)e4m3_f32(hi)) * (double)g;
     if (a > border || (a == border && (lo & 1))) lo = hi;
   }
   return lo;
@@ -193,7 +210,7 @@ __device__ __forceinline__ uint32_t e4m3_scale(double a, float g, float t) {
 // lane (nvfp4) or two neighbouring lanes (mxfp4).  v: the values; kSilu:
 // float32 approximations, and `unsure` is raised for a block that a more
 // exact form could change.
-template <bool kMX, bool kSilu>
+template <int DT, bool kMX, bool kSilu>
 __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool& unsure, uint32_t& sbyte) {
   float most = 0.0f;
 #pragma unroll
@@ -218,7 +235,7 @@ __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool& u
       sbyte = both & 0xFFu;
       unsure |= sbyte != both >> 8;
     } else {
-      sbyte = e4m3_scale((double)a, g, t);
+      sbyte = e4m3_scale(a, g, t);
     }
     unit = e4m3_f32(sbyte);
     r = unit > 0.0f ? __frcp_rn(unit * g) : 0.0f;
@@ -239,18 +256,33 @@ __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool& u
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = v[i] * ru;
     uint32_t d0 = c.x ^ e2m1x8(w), d1 = c.y ^ e2m1x8(w + 8);
-    if constexpr (!kSilu) {
+    if constexpr (!kSilu && DT == BLUT_F32) {
       if (d0 | d1) {
-        const double un = (double)unit * (double)g;  // 4 + 24 bits: exact
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           uint32_t& cw = i < 8 ? c.x : c.y;
           const int sh = 4 * (i & 7);
           if (((i < 8 ? d0 : d1) >> sh) & 15u) {
             const uint32_t lo = (cw >> sh) & 7u;
-            cw += (e2m1_decide((double)fabsf(v[i]), un, lo) - lo) << sh;
+            if (past_border(fabsf(v[i]), e2m1_border(lo) * unit, g, lo)) cw += 1u << sh;
           }
         }
+      }
+    } else if constexpr (!kSilu) {
+      // a 16-bit x this near to a border is the border rounded to x's type:
+      // the code alone tells which x it was
+      while (d0 | d1) {
+        const bool second = d0 == 0;
+        const uint32_t d = second ? d1 : d0;
+        const int sh = (__ffs(d) - 1) & 28;
+        const uint32_t lo = ((second ? c.y : c.x) >> sh) & 7u;
+        const float border = e2m1_border(lo) * unit;
+        const uint32_t up = past_border(Elem<DT>::f(Elem<DT>::from(border * g)), border, g, lo) ? 1u << sh : 0u;
+        const uint32_t left = d & ~(15u << sh);
+        if (second)
+          c.y += up, d1 = left;
+        else
+          c.x += up, d0 = left;
       }
     } else {
       unsure |= (d0 | d1) != 0;

@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
               fetch(b + kAhead, raw[j]);
               uint32_t sbyte;
               bool unsure = false;
-              const uint2 code = encode16<kMX, false>(v, g, unsure, sbyte);
+              const uint2 code = encode16<DT, kMX, false>(v, g, unsure, sbyte);
               if (it >= C::kStages) {
                 ok = wait_or_abort(smem_u32(h->empty + s), (uint32_t)(it / C::kStages - 1) & 1u, abort_flag,
                                    &g_fp4_status, p.wait_ns);
