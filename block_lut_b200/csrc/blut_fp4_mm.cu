@@ -94,6 +94,7 @@ struct Fp4Params {
   int kblocks;  // 128-column blocks
   int row_tiles;
   int token_tiles;  // one matrix: their number
+  int tn;           // tokens of an item, at most NT
   int split_log;    // log2 of the CTAs of a cluster along K
   void* y;
   int64_t ldy;
@@ -191,9 +192,8 @@ __device__ __forceinline__ uint32_t idesc_fp4(int n, int step) {
 
 // The runs' first rows and the number of token tiles before each run, tab[e]
 // and tab[E + 1 + e], e = 0 .. E, by one warp; returns the number of tiles.  A
-// run is cut into ceil(rows / NT) tiles.  Offsets are clamped to [0, x_rows],
+// run is cut into ceil(rows / tn) tiles.  Offsets are clamped to [0, x_rows],
 // so none leads out of the buffers.
-template <int NT>
 __device__ int table_of_runs(const Fp4Params& p, int lane, int* tab) {
   int before = 0;
   for (int e0 = 0; e0 < p.experts; e0 += 128) {  // four runs per lane
@@ -204,7 +204,7 @@ __device__ int table_of_runs(const Fp4Params& p, int lane, int* tab) {
       o[j] = (int)min((int64_t)max(p.offsets[e], 0), p.x_rows);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) tiles += (max(o[j + 1] - o[j], 0) + NT - 1) / NT;
+    for (int j = 0; j < 4; ++j) tiles += (max(o[j + 1] - o[j], 0) + p.tn - 1) / p.tn;
     int incl = tiles;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -218,7 +218,7 @@ __device__ int table_of_runs(const Fp4Params& p, int lane, int* tab) {
       if (e < p.experts) {
         tab[e] = o[j];
         tab[p.experts + 1 + e] = t;
-        t += (max(o[j + 1] - o[j], 0) + NT - 1) / NT;
+        t += (max(o[j + 1] - o[j], 0) + p.tn - 1) / p.tn;
         if (e == p.experts - 1) tab[p.experts] = o[j + 1], tab[2 * p.experts + 1] = t;
       }
     }
@@ -228,7 +228,6 @@ __device__ int table_of_runs(const Fp4Params& p, int lane, int* tab) {
 }
 
 // Item `i`, by a converged warp: row tiles of one token tile follow each other.
-template <int NT>
 __device__ __forceinline__ Fp4Item item_of(const Fp4Params& p, int i, int lane, const int* tab) {
   Fp4Item t;
   const int y = i / p.row_tiles;
@@ -239,13 +238,13 @@ __device__ __forceinline__ Fp4Item item_of(const Fp4Params& p, int i, int lane, 
     for (int e0 = 0; e0 < p.experts; e0 += 32)
       e += __popc(__ballot_sync(0xFFFFFFFFu, e0 + lane < p.experts && first[min(e0 + lane, p.experts)] <= y));
     t.expert = e;
-    const int in = (y - first[e]) * NT, cnt = tab[e + 1] - tab[e];
+    const int in = (y - first[e]) * p.tn, cnt = tab[e + 1] - tab[e];
     t.row0 = tab[e] + in;
-    t.cnt = min(NT, cnt - in);
+    t.cnt = min(p.tn, cnt - in);
   } else {
     t.expert = 0;
-    t.row0 = y * NT;
-    t.cnt = (int)min((int64_t)NT, p.x_rows - t.row0);
+    t.row0 = y * p.tn;
+    t.cnt = (int)min((int64_t)p.tn, p.x_rows - t.row0);
   }
   return t;
 }
@@ -415,11 +414,11 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
       h->abort_flag = 0;
       fence_mbar_init();
     }
-    const int tiles = p.experts ? table_of_runs<NT>(p, lane, tab) : p.token_tiles;
+    const int tiles = p.experts ? table_of_runs(p, lane, tab) : p.token_tiles;
     if (lane == 0) h->items = tiles * p.row_tiles;
     __syncwarp();
     if (first < tiles * p.row_tiles) {
-      t0 = item_of<NT>(p, first, lane, tab);
+      t0 = item_of(p, first, lane, tab);
       started = min(nb, C::kStages);
       if (lane == 0)
         for (int b = 0; b < started; ++b) bring_w(t0, b, b);
@@ -447,7 +446,7 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
       int it = 0;  // blocks over all items: the ring goes on from one to the next
       bool ok = true;
       for (int i = first; i < items && ok; i += step) {
-        const Fp4Item t = i == first ? t0 : item_of<NT>(p, i, lane, tab);
+        const Fp4Item t = i == first ? t0 : item_of(p, i, lane, tab);
         const uint8_t* wsrc = p.w + t.expert * p.wstride + ((int64_t)t.tile * p.kblocks + b0) * C::kA;
         const uint8_t* xsrc = p.xc + ((int64_t)b0 * 4 * p.x_rows + t.row0) * 16;
         const uint32_t xbytes = (uint32_t)t.cnt * 16;
@@ -493,7 +492,7 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
     bool ok = true;
     int it = 0, acc = 0;
     for (int i = first; i < items && ok; i += step, ++acc) {
-      const uint32_t n = (uint32_t)__shfl_sync(0xFFFFFFFFu, (item_of<NT>(p, i, lane, tab).cnt + 15) & ~15, 0);
+      const uint32_t n = (uint32_t)__shfl_sync(0xFFFFFFFFu, (item_of(p, i, lane, tab).cnt + 15) & ~15, 0);
       for (int b = 0; b < nb; ++b, ++it) {
         const int s = it % C::kStages;
         {
@@ -556,7 +555,7 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
       bool ok = true;
       int it = 0;
       for (int i = first; i < items && ok; i += step) {
-        const Fp4Item t = item_of<NT>(p, i, lane, tab);
+        const Fp4Item t = item_of(p, i, lane, tab);
         const bool in = r < t.cnt;
         const T* src = static_cast<const T*>(p.x) + (int64_t)(t.row0 + (in ? r : 0)) * p.x_ld;
         Raw<DT> raw[kAhead];
@@ -610,7 +609,7 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
     int it = 0;
     grid_dependency_wait();
     for (int i = first; i < items && ok; i += step) {
-      const Fp4Item t = item_of<NT>(p, i, lane, tab);
+      const Fp4Item t = item_of(p, i, lane, tab);
       const uint32_t* src[kIt];
       uint32_t dst[kIt], buf[kPrefetch][kIt];
       bool on[kIt];
@@ -660,7 +659,7 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
     const float gx = p.xg ? __ldg(p.xg) : 1.0f;
     int acc = 0;
     for (int i = first; i < items; i += step, ++acc) {
-      const Fp4Item t = item_of<NT>(p, i, lane, tab);
+      const Fp4Item t = item_of(p, i, lane, tab);
       const float alpha = gx * (p.wg ? __ldg(p.wg + t.expert) : 1.0f);
       const int64_t row = (int64_t)t.tile * 128 + 32 * q;
       if (!__all_sync(0xFFFFFFFFu, wait_or_abort(smem_u32(&h->acc_full), (uint32_t)acc & 1u, abort_flag, &g_fp4_status,
@@ -694,7 +693,7 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
 
   if (split > 1 && first < items) {
     // ----------------------------------- one item, K split over the cluster --
-    const Fp4Item t = item_of<NT>(p, first, lane, tab);
+    const Fp4Item t = item_of(p, first, lane, tab);
     float* part = reinterpret_cast<float*>(ring);  // free: the last MMA has read it
     bool ok = __all_sync(0xFFFFFFFFu, wait_or_abort(smem_u32(&h->acc_full), 0, abort_flag, &g_fp4_status, p.wait_ns));
     tc_fence_after();
@@ -770,14 +769,35 @@ int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kern, (const Fp4Params)p) == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH;
 }
 
+// Tokens of an item for one matrix and more than 128 tokens: the number of
+// token tiles that makes the least of rounds over the GPU's CTAs x the cost of
+// an item.  The cost follows the bytes that shared memory takes in and gives
+// out per block, which bound the loop (17 KB for the weights, 136 B a token),
+// and about four blocks' worth of time to fill and drain.  Against tiles of
+// 192: 256 x 11264 x 2048 12.8 -> 12.0 us, 1999 x 5000 x 1400 18.0 -> 17.3,
+// 4096 x 11264 x 2048 65.5 -> 63.1.
+int tokens_per_item(int64_t m, int row_tiles, int kblocks) {
+  int best = 192;
+  double least = 1e300;
+  const int64_t t0 = (m + 191) / 192;
+  for (int64_t t = t0; t <= 2 * t0 && t <= t0 + 64; ++t) {
+    const int tn = (int)(((m + t - 1) / t + 15) / 16 * 16);
+    const int64_t items = (m + tn - 1) / tn * row_tiles;
+    const double cost = (double)((items + 295) / 296) * (kblocks + 4) * (17000.0 + 136.0 * tn);
+    if (cost < least) least = cost, best = tn;
+  }
+  return best;
+}
+
 template <bool kMX>
 int dispatch(Fp4Params& p, int64_t m, int fuse, bool early, cudaStream_t stream) {
   p.row_tiles = (p.n + 127) / 128;
   // tokens per matrix: their number for one matrix, the mean for runs
   const int64_t mean = p.experts ? (m + p.experts - 1) / p.experts : m;
   const int nt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 192;
+  p.tn = nt == 192 && !p.experts ? tokens_per_item(m, p.row_tiles, p.kblocks) : nt;
   // bound on the token tiles: every run may end in a partial one
-  const int64_t tiles = p.experts ? m / nt + std::min<int64_t>(p.experts, m) : (m + nt - 1) / nt;
+  const int64_t tiles = p.experts ? m / nt + std::min<int64_t>(p.experts, m) : (m + p.tn - 1) / p.tn;
   const int64_t items = tiles * p.row_tiles;
   if (items * 8 > INT32_MAX) return BLUT_ERR_UNSUPPORTED;
   p.token_tiles = (int)tiles;

@@ -448,6 +448,8 @@ class FP4Linear:
                 raise ValueError(f"out must be {list(x.shape[:-1]) + [self.rows]}")
             y = out if out.dim() == 2 else out.view(-1, self.rows)
             _check_out(y, m, w, out_dtype)
+            if out.untyped_storage().data_ptr() == x2.untyped_storage().data_ptr():
+                x2 = x2.clone()  # y is written while other parts of the product still read x
         else:
             if out_dtype is not None and out_dtype not in _DT:
                 raise ValueError("the output is float16, bfloat16 or float32")

@@ -149,3 +149,30 @@ def test_restatement(kind):
     best = (t[..., None] - R.LEVELS).abs().min(-1).values
     got = (R.values(c, s, kind, x.shape[1], g) / unit).abs()
     assert torch.allclose((t - got).abs(), best, rtol=0, atol=1e-12)
+
+
+def test_linear_refusals():
+    L = _lib.lib()
+    d = desc(1, 256, 128)
+    size = L.blut_fp4_linear_workspace_size
+    assert size(C.byref(d), 8, 1) == 0 and size(C.byref(d), 8, 0) == 256 and size(C.byref(d), 9, 1) > 9 * 72
+    assert size(C.byref(desc(2, 256, 128)), 3, 0) == 0
+    assert size(C.byref(d), 0, 1) < 0 and size(C.byref(d), (1 << 22) + 1, 1) < 0 and size(None, 1, 1) < 0
+    f = L.blut_fp4_linear
+    a = mm_args()
+    assert f(None, 256, 1, 128, 256, 1 << 20, None) == -1
+    assert f(C.byref(a), None, 1, 128, 256, 1 << 20, None) == -1
+    assert f(C.byref(a), 256, 1, 127, 256, 1 << 20, None) == -1  # pitch
+    assert f(C.byref(a), 257, 1, 128, 256, 1 << 20, None) == -1  # alignment
+    assert f(C.byref(a), 256, 4, 128, 256, 1 << 20, None) == -2
+    assert f(C.byref(a), 256, 1, 128, None, 0, None) == -3  # g has no place
+    assert f(C.byref(mm_args(x_rows=9, x_scale=256)), 256, 1, 128, 256, 64, None) == -3
+    assert f(C.byref(mm_args(num_experts=2)), 256, 1, 128, 256, 1 << 20, None) == -1
+    assert f(C.byref(mm_args(y=None, x_scale=256)), 256, 1, 128, None, 0, None) == -1
+    w = F.FP4Weight("nvfp4", 128, 64, None, torch.zeros(9216, dtype=torch.uint8), 9216, torch.ones(1))
+    lin = F.FP4Linear(w)
+    for x in (torch.zeros(4, 63), torch.zeros(())):
+        with pytest.raises(ValueError, match="x must be"):
+            lin(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        lin(torch.zeros(4, 64))

@@ -282,3 +282,73 @@ def test_expert_layer(kind):
     # noise of a 4-bit value: at most a quarter of it between two levels, in rms about 0.1; five such factors
     # (x twice through the product of gate and up, two weights, h) stay below 0.5 of the result in the 2-norm
     assert float((y.double() - full).norm() / full.norm()) < 0.5
+
+
+def test_linear_in_place():
+    """An output that overlaps the input is written from the input as it was."""
+    F = fp4()
+    W = F.FP4Weight.quantize(torch.randn(1024, 1024, generator=gen(1), device="cuda") * 0.05)
+    lin = F.FP4Linear(W, 0.002)
+    for m in (3, 20):
+        x = torch.randn(m, 1024, generator=gen(2), device="cuda").bfloat16()
+        want = lin(x)
+        assert lin(x, out=x) is x and torch.equal(x, want)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 256, 2048), (40, 256, 2048), (500, 3000, 2048)])
+def test_a_wait_that_runs_out_is_reported(m, n, k):
+    """With a limit of 1 ns the kernels' waits give up: the call ends, the status says so once, the next call is right."""
+    from block_lut_b200 import _lib
+    F = fp4()
+    xq, x = operand(m, k, "nvfp4", 1)
+    wq, w = operand(n, k, "nvfp4", 2)
+    W = F.FP4Weight.from_quantized(wq)
+    F.fp4_check_status()
+    _lib.lib().blut_debug_set_wait_limit(1)
+    try:
+        F.fp4_matmul(xq, W)
+        torch.cuda.synchronize()
+    finally:
+        _lib.lib().blut_debug_set_wait_limit(0)
+    with pytest.raises(RuntimeError, match="timed out"):
+        F.fp4_check_status()
+    F.fp4_check_status()
+    check(F.fp4_matmul(xq, W), x, w)
+    F.fp4_check_status()
+
+
+def test_first_call_in_a_capture():
+    """A process whose first product is captured: the launch set-up works inside a capture."""
+    import subprocess
+    import sys
+    code = (
+        "import torch\n"
+        "from block_lut_b200 import fp4 as F\n"
+        "w = torch.randn(256, 512, device='cuda'); x = torch.randn(20, 512, device='cuda').bfloat16()\n"
+        "W = F.FP4Weight.quantize(w); lin = F.FP4Linear(W)\n"
+        "torch.cuda.synchronize(); g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g): y = lin(x); z = lin(x[:2])\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "assert torch.equal(y, lin(x)) and torch.equal(z, lin(x[:2]))\n"
+        "print('captured')\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_large_codes_offset(kind):
+    """Rows and columns whose codes pass 2^31 bytes, and an output past 2^31 elements: spot checks on both ends."""
+    F = fp4()
+    m, k, n = 1 << 21, 2304, 1152
+    x = torch.zeros(m, k, device="cuda", dtype=torch.bfloat16)
+    at = [0, 1, m // 2, m - 2, m - 1]
+    x[at] = torch.randn(5, k, generator=gen(1), device="cuda").bfloat16()
+    g = None if kind == "mxfp4" else 0.002
+    xq = F.quantize_fp4(x, kind, g)
+    wq, w = operand(n, k, kind, 2, 0.05)
+    y = F.fp4_matmul(xq, F.FP4Weight.from_quantized(wq))
+    gv = 1.0 if g is None else torch.tensor([g], device="cuda")
+    check(y[at], R.values(*R.quantize(x[at], kind, gv), kind, k, gv), w)
+    assert int(y.count_nonzero()) <= 5 * n and m * n > 2 ** 31 and xq.codes.numel() > 2 ** 31
+    d = F.dequantize_fp4(xq)
+    assert torch.equal(d[at], R.values(*R.quantize(x[at], kind, gv), kind, k, gv).float().bfloat16())
