@@ -146,10 +146,12 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // Low word of the no-swizzle K-major descriptor (tc_desc) of a shared
-// address, whose bits from 18 up may name the CTA in its cluster; the high
-// word is constant.
-__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) {
-  return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);
+// address, whose bits from 18 up may name the CTA in its cluster, in two
+// parts: the stage's, and what an operand inside it adds; the high word is
+// constant.
+__device__ __forceinline__ uint32_t desc_base(uint32_t saddr) { return (saddr >> 4) & 0x3FFFu; }
+__device__ __forceinline__ constexpr uint32_t desc_add(uint32_t offset, uint32_t lbo) {
+  return (offset >> 4) + ((lbo >> 4) << 16);
 }
 constexpr uint32_t kDescHi = (128u >> 4) | (1u << 14);  // 128 bytes between 8-row groups, version 1
 
@@ -487,12 +489,13 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
     // instructions took 75 cycles each to issue.  The barriers of a block
     // are polled by a lane each.
     const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-    const uint32_t ring_addr = smem_u32(ring);
+    const uint32_t ring_desc = desc_base(smem_u32(ring));
     const bool leader = elect_one();
     bool ok = true;
     int it = 0, acc = 0;
     for (int i = first; i < items && ok; i += step, ++acc) {
       const uint32_t n = (uint32_t)__shfl_sync(0xFFFFFFFFu, (item_of(p, i, lane, tab).cnt + 15) & ~15, 0);
+      const uint32_t idesc0 = idesc_fp4<kMX>(n, 0), idesc1 = idesc_fp4<kMX>(n, 1);
       for (int b = 0; b < nb; ++b, ++it) {
         const int s = it % C::kStages;
         {
@@ -513,22 +516,22 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
         if (!ok) break;
         __syncwarp();
         tc_fence_after();
-        const uint32_t st = ring_addr + s * C::kStage;
+        const uint32_t st = ring_desc + s * (C::kStage >> 4);
         const uint32_t slot = tm + NT + (it % C::kSlots) * C::kSlotCols;
         if (leader) {
 #pragma unroll
           for (int w = 0; w < C::kWords; ++w) {
-            cp_scales(slot + w * C::kWordCols, desc_lo(st + kFp4UnitCodes + 512 * w, 512));
+            cp_scales(slot + w * C::kWordCols, st + desc_add(kFp4UnitCodes + 512 * w, 512));
 #pragma unroll
             for (int g = 0; g < C::kGroups; ++g)
               cp_scales(slot + w * C::kWordCols + 4 + 4 * g,
-                        desc_lo(st + C::kA + C::kB + 512 * (w * C::kGroups + g), 512));
+                        st + desc_add(C::kA + C::kB + 512 * (w * C::kGroups + g), 512));
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const uint32_t sc = slot + (kMX ? 0 : k * C::kWordCols);
-            mma_fp4<kMX>(tm, desc_lo(st + k * 4096, 2048), desc_lo(st + C::kA + k * 2 * NT * 16, NT * 16),
-                         idesc_fp4<kMX>(n, k), sc, sc + 4, (uint32_t)(b | k));
+            mma_fp4<kMX>(tm, st + desc_add(k * 4096, 2048), st + desc_add(C::kA + k * 2 * NT * 16, NT * 16),
+                         k ? idesc1 : idesc0, sc, sc + 4, (uint32_t)(b | k));
           }
           tc_commit(smem_u32(h->empty + s));
           if (b == nb - 1) tc_commit(smem_u32(&h->acc_full));

@@ -49,14 +49,15 @@ def _desc(kind: str, rows: int, cols: int) -> _lib.FP4Desc:
 
 def _launch(what: str, t: torch.Tensor, stream, *args) -> None:
     """The library's ``blut_<what>`` on t's device and the given (default: current) stream."""
-    fn = getattr(_lib.lib(), "blut_" + what)
+    fn = getattr(_lib.lib(), what)
     dev = t.get_device()
     if dev == torch.cuda.current_device():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream)
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _lib.stream_ptr(stream))
-    _lib.check(rc, what)
+    if rc:
+        _lib.check(rc, what[5:])
 
 
 def _rows2d(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -147,7 +148,7 @@ class FP4Matrix:
         scales = torch.empty(self.rows, nb, dtype=torch.uint8, device=self.data.device)
         if self.rows:
             d = _desc(self.kind, self.rows, self.cols)
-            _launch("fp4_export", codes, stream, C.byref(d), *self._ptrs(), codes.data_ptr(), scales.data_ptr())
+            _launch("blut_fp4_export", codes, stream, C.byref(d), *self._ptrs(), codes.data_ptr(), scales.data_ptr())
         return codes, scales
 
 
@@ -166,7 +167,7 @@ def _import(kind, codes, scales, cols, global_scale, stream=None) -> FP4Matrix:
     g = _given_scale(kind, global_scale, codes.device)
     m = FP4Matrix.empty(kind, rows, cols, codes.device, g)
     if rows:
-        _launch("fp4_import", codes, stream, C.byref(d), codes.data_ptr(), scales.data_ptr(), *m._ptrs())
+        _launch("blut_fp4_import", codes, stream, C.byref(d), codes.data_ptr(), scales.data_ptr(), *m._ptrs())
     return m
 
 
@@ -187,7 +188,7 @@ def fp4_global_scale(x: torch.Tensor, silu_mul: bool = False, stream=None) -> to
     buf = torch.empty(4, dtype=torch.float32, device=x.device)
     if x.shape[0] == 0:
         return buf.fill_(MIN_GLOBAL_SCALE)[:1]
-    _launch("fp4_global_scale", x, stream, x.data_ptr(), _DT[x.dtype], x.shape[0], cols, _pitch(x), int(silu_mul),
+    _launch("blut_fp4_global_scale", x, stream, x.data_ptr(), _DT[x.dtype], x.shape[0], cols, _pitch(x), int(silu_mul),
             buf.data_ptr())
     return buf[:1]
 
@@ -198,9 +199,9 @@ def _gate_cols(x: torch.Tensor) -> int:
     return x.shape[1] // 2
 
 
-def _row_scale(kind: str, g: Scale, x: torch.Tensor, silu_mul: bool, stream) -> Optional[torch.Tensor]:
-    if kind == "nvfp4" and g is None:
-        return fp4_global_scale(x, silu_mul, stream=stream)
+def _row_scale(kind: str, g: Scale, x: torch.Tensor, silu_mul: bool) -> Optional[torch.Tensor]:
+    if g is None:
+        return fp4_global_scale(x, silu_mul) if kind == "nvfp4" else None
     return _given_scale(kind, g, x.device)
 
 
@@ -223,13 +224,13 @@ def quantize_fp4(x: torch.Tensor, kind: str = "nvfp4", global_scale: Scale = Non
         row_index = row_index.contiguous()
         n = row_index.shape[0]
     d = _desc(kind, n, x.shape[1])
-    g = _row_scale(kind, global_scale, x, False, stream)
+    g = _row_scale(kind, global_scale, x, False)
     m = FP4Matrix.empty(kind, n, x.shape[1], x.device, g)
     if n == 0:
         return m
     if x.shape[0] == 0:
         raise ValueError("row_index into an x without rows")
-    _launch("fp4_quantize", x, stream, C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(row_index), x.shape[0], _p(g),
+    _launch("blut_fp4_quantize", x, stream, C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(row_index), x.shape[0], _p(g),
             *m._ptrs())
     return m
 
@@ -242,11 +243,11 @@ def silu_mul_quantize_fp4(gate_up: torch.Tensor, kind: str = "nvfp4", global_sca
     x = _rows2d(gate_up, "gate_up")
     cols = _gate_cols(x)
     d = _desc(kind, x.shape[0], cols)
-    g = _row_scale(kind, global_scale, x, True, stream)
+    g = _row_scale(kind, global_scale, x, True)
     m = FP4Matrix.empty(kind, x.shape[0], cols, x.device, g)
     if x.shape[0] == 0:
         return m
-    _launch("fp4_silu_mul_quantize", x, stream, C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(g), *m._ptrs())
+    _launch("blut_fp4_silu_mul_quantize", x, stream, C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(g), *m._ptrs())
     return m
 
 
@@ -255,11 +256,11 @@ def dequantize_fp4(q: FP4Matrix, dtype: torch.dtype = torch.bfloat16, stream=Non
     """The values q stands for, [rows, cols] in ``dtype`` (float32 products, rounded once to 16 bits)."""
     if dtype not in _DT:
         raise ValueError(f"dtype must be float16, bfloat16 or float32, not {dtype}")
-    out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.data.device)
+    out = q.data.new_empty((q.rows, q.cols), dtype=dtype)
     if q.rows == 0:
         return out
     d = _desc(q.kind, q.rows, q.cols)
-    _launch("fp4_dequantize", out, stream, C.byref(d), *q._ptrs(), _p(q.global_scale), out.data_ptr(), _DT[dtype], q.cols)
+    _launch("blut_fp4_dequantize", out, stream, C.byref(d), *q._ptrs(), _p(q.global_scale), out.data_ptr(), _DT[dtype], q.cols)
     return out
 
 
@@ -316,7 +317,7 @@ def _pack(mats, stream=None) -> FP4Weight:
     dev = m0.data.device
     tiled = torch.empty(len(mats) * stride, dtype=torch.uint8, device=dev)
     for i, m in enumerate(mats):
-        _launch("fp4_pack_tiled", tiled, stream, C.byref(d), *m._ptrs(), tiled.data_ptr() + i * stride)
+        _launch("blut_fp4_pack_tiled", tiled, stream, C.byref(d), *m._ptrs(), tiled.data_ptr() + i * stride)
     g = None if m0.kind == "mxfp4" else torch.cat([m.global_scale.reshape(1) for m in mats])
     return FP4Weight(m0.kind, m0.rows, m0.cols, None if single else len(mats), tiled, stride, g)
 
@@ -369,7 +370,7 @@ def _product(x: FP4Matrix, w: FP4Weight, offsets, out, out_dtype, stream) -> tor
     if x.rows > MAX_ROWS:
         raise ValueError(f"at most {MAX_ROWS} rows in one product")
     if out is None:
-        out = torch.empty((x.rows, w.rows), dtype=out_dtype or torch.bfloat16, device=x.data.device)
+        out = x.data.new_empty((x.rows, w.rows), dtype=out_dtype or torch.bfloat16)
     _check_out(out, x.rows, w, out_dtype)
     if x.rows == 0:
         return out
@@ -380,7 +381,7 @@ def _product(x: FP4Matrix, w: FP4Weight, offsets, out, out_dtype, stream) -> tor
     a.x_codes, a.x_scales = x._ptrs()
     a.x_scale = _p(x.global_scale)
     a.x_rows, a.y, a.y_ld = x.rows, out.data_ptr(), _pitch(out)
-    _launch("fp4_matmul", out, stream, C.byref(a))
+    _launch("blut_fp4_matmul", out, stream, C.byref(a))
     return out
 
 
@@ -453,7 +454,7 @@ class FP4Linear:
         else:
             if out_dtype is not None and out_dtype not in _DT:
                 raise ValueError("the output is float16, bfloat16 or float32")
-            y = torch.empty((m, self.rows), dtype=out_dtype or x2.dtype, device=x2.device)
+            y = x2.new_empty((m, self.rows), dtype=out_dtype or x2.dtype)
         if m:
             need = self._ws.get(m)
             if need is None:
@@ -463,8 +464,8 @@ class FP4Linear:
                 raise ValueError(f"at most {MAX_ROWS} rows in one product")
             a = _lib.FP4MMArgs.from_buffer_copy(self._args)  # calls from several host threads never share one
             a.x_rows, a.y, a.y_ld, a.out_dtype = m, y.data_ptr(), _pitch(y), _DT[y.dtype]
-            ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
-            _launch("fp4_linear", x2, stream, C.byref(a), x2.data_ptr(), _DT[x2.dtype], _pitch(x2), _p(ws), need)
+            ws = x2.new_empty(need, dtype=torch.uint8) if need else None
+            _launch("blut_fp4_linear", x2, stream, C.byref(a), x2.data_ptr(), _DT[x2.dtype], _pitch(x2), _p(ws), need)
         if out is not None:
             return out
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.rows)
