@@ -30,6 +30,7 @@
 // Every wait is bounded; one that runs out raises the CTA's abort flag and
 // the device status, and every role then leaves its loop, lets what it has in
 // flight land, and frees the tensor memory.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -100,6 +101,7 @@ struct Fp4Params {
   int64_t ldy;
   int out_dtype;
   int vec;      // rows of y start on 16-byte boundaries
+  int tma;      // y is described by the kernel's tensor map
   uint64_t wait_ns;
 };
 
@@ -301,50 +303,79 @@ __device__ __forceinline__ void tc_ld_16x32(uint32_t taddr, uint32_t (&v)[16]) {
       : "memory");
 }
 
+// Bulk tensor store of a warp's stage, 32 tokens x 32 rows, to y at (row,
+// token); what lies outside y is not written.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t saddr, int row, int token) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n\t"
+               "cp.async.bulk.commit_group;" ::"l"(map),
+               "r"(row), "r"(token), "r"(saddr)
+               : "memory");
+}
+
 // An epilogue warp's 32 weight rows x cnt tokens as 16-bit rows of y: pairs
-// of tokens are packed as an mma accumulator holds them, stmatrix transposes
-// 8 x 8 of them at a time, and a store then covers 32 rows of 8 tokens, 16
-// bytes a lane.  y: token 0, the warp's first row, of which `left` are rows
-// of the matrix; vec: rows of y start on 16-byte boundaries; c0, cstep: the
-// warp's stretches of 32 tokens.
-template <int kOut>
+// of tokens are packed as an mma accumulator holds them and stmatrix
+// transposes 8 x 8 of them at a time into rows of 64 bytes per token, whose
+// 16-byte pieces are swapped about against bank conflicts (and as a tensor
+// map with 64-byte swizzle expects them).  From there a full stretch of 32
+// tokens leaves as one bulk tensor store (map not null); a stretch that ends
+// inside, or a y without a map, as stores of 32 rows of 8 tokens, 16 bytes a
+// lane.  Plain stores alone kept the accumulator for 4500 cycles of an item
+// of 16 000 (128 x 192, K = 2048).  y: token 0, the warp's first row `row`,
+// of which `left` are rows of the matrix; vec: rows of y start on 16-byte
+// boundaries; c0, cstep: the warp's stretches; read: called once the
+// accumulator has been read.
+template <int kOut, class Read>
 __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha, uint8_t* stage, uint16_t* y,
-                                             int64_t ldy, int left, bool vec, int lane, int c0, int cstep) {
+                                             int64_t ldy, int left, bool vec, int lane, int c0, int cstep,
+                                             const CUtensorMap* map, int row, int token0, int rows_in_y, Read read) {
   const int mine = min(8, left - (lane & 3) * 8);  // rows of this lane's piece
   const uint32_t saddr = smem_u32(stage);
+  if (c0 >= cnt) read();
 #pragma unroll 1
   for (int c = c0; c < cnt; c += cstep) {
-    uint32_t v[2][16];
+    uint32_t v[2][16], w[4][4];
     tc_ld_16x32(tcol + c, v[0]);
     tc_ld_16x32(tcol + c + (16u << 16), v[1]);
     tc_wait_ld16(v[0]);
     tc_wait_ld16(v[1]);
+    if (c + cstep >= cnt) read();
 #pragma unroll
-    for (int tg = 0; tg < 4; ++tg) {  // 8 tokens x 32 rows: four 8 x 8 matrices
-      uint32_t w[4];
+    for (int tg = 0; tg < 4; ++tg)  // 8 tokens x 32 rows: four 8 x 8 matrices
 #pragma unroll
       for (int rg = 0; rg < 4; ++rg)
-        w[rg] = pack2<kOut>(__uint_as_float(v[rg >> 1][4 * tg + 2 * (rg & 1)]) * alpha,
-                            __uint_as_float(v[rg >> 1][4 * tg + 2 * (rg & 1) + 1]) * alpha);
-      // lane 8 rg + i gives the address of token i, rows 8 rg .. 8 rg + 7; the
-      // 16-byte pieces of a token are swapped about against bank conflicts
+        w[tg][rg] = pack2<kOut>(__uint_as_float(v[rg >> 1][4 * tg + 2 * (rg & 1)]) * alpha,
+                                __uint_as_float(v[rg >> 1][4 * tg + 2 * (rg & 1) + 1]) * alpha);
+    if (map) {  // the stage's last store has read it
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+    }
+#pragma unroll
+    for (int tg = 0; tg < 4; ++tg) {
+      // lane 8 rg + i gives the address of token i, rows 8 rg .. 8 rg + 7
       const int t = 8 * tg + (lane & 7), piece = (lane >> 3) ^ ((t >> 1) & 3);
       asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(saddr + t * 64 +
                                                                                                  piece * 16),
-                   "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   "r"(w[tg][0]), "r"(w[tg][1]), "r"(w[tg][2]), "r"(w[tg][3])
                    : "memory");
+    }
+    // a box may reach past the item's tokens where y ends there too
+    if (map && (c + 32 <= cnt || token0 + cnt == rows_in_y)) {
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) store_box(map, saddr, row, token0 + c);
+      continue;
     }
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int t = 8 * j + (lane >> 2);
       if (c + t >= cnt) continue;
-      const uint4 w = *reinterpret_cast<const uint4*>(stage + t * 64 + ((lane & 3) ^ ((t >> 1) & 3)) * 16);
+      const uint4 u = *reinterpret_cast<const uint4*>(stage + t * 64 + ((lane & 3) ^ ((t >> 1) & 3)) * 16);
       uint16_t* dst = y + (int64_t)(c + t) * ldy + (lane & 3) * 8;
       if (vec && mine == 8) {
-        *reinterpret_cast<uint4*>(dst) = w;
+        *reinterpret_cast<uint4*>(dst) = u;
       } else {
-        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t words[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (k < mine) dst[k] = (uint16_t)(words[k >> 1] >> (16 * (k & 1)));
@@ -377,7 +408,8 @@ __device__ __forceinline__ void reduce_cluster(const Fp4Params& p, const float* 
 // most 8) rows themselves, 16 columns a lane and block: a launch and a pass
 // through memory less, where a call is little else.
 template <bool kMX, int NT, int kFuse>
-__global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kernel(const Fp4Params p) {
+__global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kernel(const __grid_constant__ Fp4Params p,
+                                                                                              const __grid_constant__ CUtensorMap ymap) {
   using C = Fp4Cfg<kMX, NT>;
   extern __shared__ __align__(1024) uint8_t fp4_smem[];
   Fp4Header* h = reinterpret_cast<Fp4Header*>(fp4_smem);
@@ -670,13 +702,22 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
         break;
       tc_fence_after();
       const int left = (int)min((int64_t)32, p.n - row);  // rows of the matrix among this warp's
+      const auto read = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&h->acc_empty));
+      };
       if (left <= 0) {
+        read();
       } else if (p.out_dtype != BLUT_F32) {
         uint16_t* y = static_cast<uint16_t*>(p.y) + (int64_t)t.row0 * p.ldy + row;
+        const CUtensorMap* map = p.tma ? &ymap : nullptr;
         if (p.out_dtype == BLUT_BF16)
-          store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi);
+          store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi, map,
+                                  (int)row, t.row0, (int)p.x_rows, read);
         else
-          store_tile16<BLUT_F16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi);
+          store_tile16<BLUT_F16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi, map,
+                                 (int)row, t.row0, (int)p.x_rows, read);
       } else {
 #pragma unroll 1
         for (int c = 16 * part; c < t.cnt; c += 16 * C::kEpi) {
@@ -687,11 +728,11 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
           for (int j = 0; j < 16; ++j)
             if (c + j < t.cnt) store1(p, t.row0 + c + j, row + lane, __uint_as_float(v[j]) * alpha);
         }
+        read();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&h->acc_empty));
     }
+    if (p.tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
 
   if (split > 1 && first < items) {
@@ -730,6 +771,28 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols));
 }
 
+// The map of a 16-bit y [x_rows][n] for boxes of 32 tokens x 32 rows.
+bool y_map(const Fp4Params& p, CUtensorMap* map) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> encode{nullptr};
+  Encode fn = encode.load(std::memory_order_acquire);
+  if (!fn) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      return false;
+    fn = reinterpret_cast<Encode>(f);
+    encode.store(fn, std::memory_order_release);
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)p.n, (cuuint64_t)p.x_rows}, pitch[1] = {(cuuint64_t)p.ldy * 2};
+  const cuuint32_t box[2] = {32, 32}, one[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, pitch, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // early: the launch may begin while the kernel before it, which writes x, is
 // still running (it waits in grid_dependency_wait before it reads x).
 template <bool kMX, int NT, int kFuse = 0>
@@ -750,6 +813,10 @@ int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
     if (dev >= 0) sms_of[dev].store(sms, std::memory_order_release);
   }
   const int split = 1 << p.split_log;
+  // large items leave by bulk tensor stores (the map costs the host under a
+  // microsecond, which the smallest calls would notice)
+  CUtensorMap map = {};
+  p.tma = NT >= 128 && split == 1 && p.vec && p.out_dtype != BLUT_F32 && y_map(p, &map);
   cudaLaunchConfig_t cfg = {};
   // one CTA (cluster) per item where K is split, else as many as run at once
   cfg.gridDim = dim3((unsigned)(split > 1 ? items * split : std::min<int64_t>(items, (int64_t)sms * C::kCtas)));
@@ -769,7 +836,7 @@ int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  return cudaLaunchKernelEx(&cfg, kern, (const Fp4Params)p) == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kern, (const Fp4Params)p, (const CUtensorMap)map) == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH;
 }
 
 // Tokens of an item for one matrix and more than 128 tokens: the number of
