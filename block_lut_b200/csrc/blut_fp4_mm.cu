@@ -48,7 +48,6 @@ __device__ int g_fp4_status;
 constexpr int kEpiWarp0 = 4;   // first epilogue warp
 constexpr int kEpiStage = 2048;  // bytes an epilogue warp transposes in: 32 tokens x 32 rows of 16 bits
 constexpr int kHeader = 1024;  // barriers and flags
-constexpr int kPrefetch = 4;   // blocks of token scales held in registers
 constexpr int kFuseRows = 8;   // most rows that the product quantises itself
 
 template <bool kMX, int NT>
@@ -636,17 +635,28 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
     }
   } else if (warp < kEpiWarp0) {
     // -------------------------------------------------------- token scales --
+    // Copied a word at a time, without registers in between.  Copies of up to
+    // kAhead blocks are in flight; before it waits for a free stage a warp
+    // hands over all it has, so nobody waits for what is already here.
     constexpr int kWordsAll = C::kWords * NT;
     constexpr int kIt = (kWordsAll + 63) / 64;
+    constexpr int kAhead = 3;
     const int t64 = threadIdx.x - 64;
     const int64_t words = (int64_t)C::kWords * p.x_rows;
+    const uint32_t ring_addr = smem_u32(ring);
     bool ok = true;
-    int it = 0;
+    int it = 0, given = 0;  // blocks copied, and handed over
+    const auto give = [&] {
+      fence_proxy_async();  // tcgen05.cp reads what was written here
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(h->sfull + given % C::kStages));
+      ++given;
+    };
     grid_dependency_wait();
     for (int i = first; i < items && ok; i += step) {
       const Fp4Item t = item_of(p, i, lane, tab);
       const uint32_t* src[kIt];
-      uint32_t dst[kIt], buf[kPrefetch][kIt];
+      uint32_t dst[kIt];
       bool on[kIt];
 #pragma unroll
       for (int q = 0; q < kIt; ++q) {
@@ -655,36 +665,33 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
         src[q] = p.xs + ((int64_t)b0 * C::kWords + w) * p.x_rows + t.row0 + r;
         dst[q] = C::kA + C::kB + (w * C::kGroups + r / 128) * 512 + (r % 32) * 16 + ((r % 128) / 32) * 4;
       }
-#pragma unroll
-      for (int j = 0; j < kPrefetch; ++j)
-#pragma unroll
-        for (int q = 0; q < kIt; ++q) buf[j][q] = j < nb && on[q] ? __ldg(src[q] + j * words) : 0u;
-      for (int c = 0; c < nb && ok; c += kPrefetch) {
-#pragma unroll
-        for (int j = 0; j < kPrefetch; ++j) {
-          const int b = c + j, s = it % C::kStages;
-          if (b < nb && ok) {
-            if (it >= C::kStages) {
-              ok = wait_or_abort(smem_u32(h->empty + s), (uint32_t)(it / C::kStages - 1) & 1u, abort_flag, &g_fp4_status,
-                                 p.wait_ns);
-              ok = __all_sync(0xFFFFFFFFu, ok);
-            }
-            if (ok) {
-#pragma unroll
-              for (int q = 0; q < kIt; ++q)
-                if (on[q]) *reinterpret_cast<uint32_t*>(ring + s * C::kStage + dst[q]) = buf[j][q];
-              fence_proxy_async();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(smem_u32(h->sfull + s));
-#pragma unroll
-              for (int q = 0; q < kIt; ++q)
-                if (b + kPrefetch < nb && on[q]) buf[j][q] = __ldg(src[q] + (b + kPrefetch) * words);
-            }
-            ++it;
+      for (int b = 0; b < nb; ++b) {
+        const int s = it % C::kStages;
+        if (it >= C::kStages) {
+          const uint32_t bar = smem_u32(h->empty + s), ph = (uint32_t)(it / C::kStages - 1) & 1u;
+          if (!__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, ph))) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            while (given < it) give();
+            ok = __all_sync(0xFFFFFFFFu, wait_or_abort(bar, ph, abort_flag, &g_fp4_status, p.wait_ns));
+            if (!ok) break;
           }
+        }
+#pragma unroll
+        for (int q = 0; q < kIt; ++q) {
+          if (on[q])
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ring_addr + s * C::kStage + dst[q]), "l"(src[q])
+                         : "memory");
+          src[q] += words;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (++it - given == kAhead) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+          give();
         }
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    while (ok && given < it) give();
   } else if (split == 1) {
     // ------------------------------------------------------------ epilogue --
     const int q = warp & 3, part = (warp - kEpiWarp0) >> 2;  // lane quarter (a warp may read its own only), share
