@@ -81,6 +81,21 @@ __device__ __noinline__ void encode_block_f64(const typename Elem<DT>::T* row, i
   if (kMX ? (lane | 1) == (owner | 1) : lane == owner) c = w, sbyte = s;
 }
 
+// 16 columns a lane of a row (null: zeros) with n columns left, any boundary.
+template <int DT>
+__device__ __forceinline__ void load_row(const typename Elem<DT>::T* p, int n, typename Elem<DT>::T* buf, float (&v)[16]) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int c = 32 * j + lane;
+    buf[c + (c >> 4)] = p && c < n ? p[c] : typename Elem<DT>::T(0);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = Elem<DT>::f(buf[17 * lane + j]);
+}
+
 // Bytes of a staged chunk: 16 more than its rows, against bank conflicts.
 __host__ __device__ constexpr int q_pitch(int rows) { return rows * 16 + 16; }
 
@@ -100,6 +115,7 @@ __global__ void __launch_bounds__(32 * kQWarps, kPer > 1 ? 4 : 1)
   constexpr int kWordCols = kMX ? 128 : 64, kWords = kQCols / kWordCols;
   __shared__ alignas(16) uint8_t sc[kQChunks * kPitch];
   __shared__ uint32_t ss[kWords * kRows];
+  __shared__ typename Elem<DT>::T sx[kVec ? 1 : kQWarps][kVec ? 1 : kQCols + kQCols / 16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * kRows;
   const int col0 = blockIdx.y * kQCols, col = col0 + 16 * lane;
@@ -107,14 +123,15 @@ __global__ void __launch_bounds__(32 * kQWarps, kPer > 1 ? 4 : 1)
   const float g = kMX ? 1.0f : __ldg(gptr);
   const typename Elem<DT>::T* p[kPer];  // null: no row, or no columns
   Raw<DT> raw[kPer], raw_up[kSilu ? kPer : 1];
+  const auto src_of = [&](int64_t row) -> int64_t {  // row of x, below 0 for none
+    if (row >= rows) return -1;
+    if (!row_index) return row;
+    const int64_t src = row_index[row];
+    return src < src_rows ? src : -1;
+  };
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int64_t row = row0 + warp + kQWarps * i;
-    int64_t src = row < rows ? row : -1;
-    if (row_index && src >= 0) {
-      src = row_index[row];
-      if (src >= src_rows) src = -1;
-    }
+    const int64_t src = src_of(row0 + warp + kQWarps * i);
     p[i] = src < 0 || n == 0 ? nullptr : x + src * ld + col;
     if (kVec && n == 16 && p[i]) {
       raw_load<DT, kVec>(p[i], raw[i]);
@@ -125,7 +142,22 @@ __global__ void __launch_bounds__(32 * kQWarps, kPer > 1 ? 4 : 1)
   for (int i = 0; i < kPer; ++i) {
     float v[16];
     bool unsure = false;
-    if (!p[i]) {
+    if constexpr (kVec == 0) {
+      // rows on any boundary: the warp reads them side by side and passes
+      // them on in shared memory (16 columns a lane, a gap after each)
+      const int64_t srow = src_of(row0 + warp + kQWarps * i);
+      load_row<DT>(srow < 0 ? nullptr : x + srow * ld + col0, cols - col0, sx[warp], v);
+      if constexpr (kSilu) {
+        float u[16], least = 0.0f;
+        load_row<DT>(srow < 0 ? nullptr : x + srow * ld + cols + col0, cols - col0, sx[warp], u);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          least = fminf(least, v[j]);
+          v[j] = silu_mul_f32(v[j], u[j]);
+        }
+        unsure = least < -80.0f;
+      }
+    } else if (!p[i]) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) v[j] = 0.0f;
     } else {
@@ -191,57 +223,88 @@ __global__ void __launch_bounds__(32 * kQWarps, kPer > 1 ? 4 : 1)
 template <int DT, bool kSilu, int kVec>
 __global__ void __launch_bounds__(256)
     fp4_global_scale_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t ld, int64_t rows, int cols,
-                            float* out) {
-  constexpr int kDepth = 2;  // stretches of 16 columns in flight
-  const int per_row = (cols + 15) / 16;
-  const int64_t stride = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t srow = stride / per_row;
-  const int scol = (int)(stride - srow * per_row);
-  int64_t row = first / per_row;
-  int c = (int)(first - row * per_row);
+                            const typename Elem<DT>::T* __restrict__ tail, int ntail, float* out) {
   uint32_t top = 0;
-  while (row < rows) {
-    Raw<DT> raw[kDepth], raw_up[kSilu ? kDepth : 1];
-    const typename Elem<DT>::T* p[kDepth];
-    int n[kDepth];
-#pragma unroll
-    for (int i = 0; i < kDepth; ++i) {
-      n[i] = row < rows ? min(16, cols - 16 * c) : 0;
-      p[i] = x + row * ld + 16 * c;
-      if (kVec && n[i] == 16) {
-        raw_load<DT, kVec>(p[i], raw[i]);
-        if constexpr (kSilu) raw_load<DT, kVec>(p[i] + cols, raw_up[i]);
-      }
-      row += srow, c += scol;
-      if (c >= per_row) c -= per_row, ++row;
+  if (blockIdx.x == 0)  // what a matrix read as one long row leaves over
+    for (int c = threadIdx.x; c < ntail; c += 256) {
+      const uint32_t b = __float_as_uint(Elem<DT>::f(tail[c])) & 0x7FFFFFFFu;
+      top = max(top, b < 0x7F800000u ? b : 0u);
     }
+  if constexpr (kVec == 0) {  // rows on any boundary: columns side by side
+    const int stretches = (cols + 2047) / 2048;
+    const int64_t drow = gridDim.x / stretches;
+    const int dst = gridDim.x % stretches;
+    int64_t row = blockIdx.x / stretches;
+    for (int st = blockIdx.x % stretches; row < rows;) {
+      const int c0 = st * 2048 + threadIdx.x;
+      const typename Elem<DT>::T* p = x + row * ld;
+      float v[8], u[8];
 #pragma unroll
-    for (int i = 0; i < kDepth; ++i) {
-      if (!n[i]) continue;
-      float v[16];
-      if (kVec && n[i] == 16)
-        raw_unpack<DT>(raw[i], v);
-      else
-        load16<DT>(p[i], n[i], v);
-      if constexpr (kSilu) {
-        float u[16];
-        if (kVec && n[i] == 16)
-          raw_unpack<DT>(raw_up[i], u);
-        else
-          load16<DT>(p[i] + cols, n[i], u);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = silu_mul_f32(v[j], u[j]);
+      for (int j = 0; j < 8; ++j) {
+        const int c = c0 + 256 * j;
+        v[j] = c < cols ? Elem<DT>::f(p[c]) : 0.0f;
+        if constexpr (kSilu) u[j] = c < cols ? Elem<DT>::f(p[cols + c]) : 0.0f;
       }
-      float most = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) most = max3_abs(most, v[j], v[j + 1]);
-      if (__float_as_uint(most) < 0x7F800000u) {
-        top = max(top, __float_as_uint(most));
-      } else {  // something is not finite: value by value
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (kSilu) v[j] = silu_mul_f32(v[j], u[j]);
+        const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+        top = max(top, b < 0x7F800000u ? b : 0u);
+      }
+      row += drow, st += dst;
+      if (st >= stretches) st -= stretches, ++row;
+    }
+  } else {
+    constexpr int kDepth = 2;  // stretches of 16 columns in flight
+    const int per_row = (cols + 15) / 16;
+    const int64_t stride = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t srow = stride / per_row;
+    const int scol = (int)(stride - srow * per_row);
+    int64_t row = first / per_row;
+    int c = (int)(first - row * per_row);
+    while (row < rows) {
+      Raw<DT> raw[kDepth], raw_up[kSilu ? kDepth : 1];
+      const typename Elem<DT>::T* p[kDepth];
+      int n[kDepth];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-          top = max(top, b < 0x7F800000u ? b : 0u);
+      for (int i = 0; i < kDepth; ++i) {
+        n[i] = row < rows ? min(16, cols - 16 * c) : 0;
+        p[i] = x + row * ld + 16 * c;
+        if (kVec && n[i] == 16) {
+          raw_load<DT, kVec>(p[i], raw[i]);
+          if constexpr (kSilu) raw_load<DT, kVec>(p[i] + cols, raw_up[i]);
+        }
+        row += srow, c += scol;
+        if (c >= per_row) c -= per_row, ++row;
+      }
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) {
+        if (!n[i]) continue;
+        float v[16];
+        if (kVec && n[i] == 16)
+          raw_unpack<DT>(raw[i], v);
+        else
+          load16<DT>(p[i], n[i], v);
+        if constexpr (kSilu) {
+          float u[16];
+          if (kVec && n[i] == 16)
+            raw_unpack<DT>(raw_up[i], u);
+          else
+            load16<DT>(p[i] + cols, n[i], u);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = silu_mul_f32(v[j], u[j]);
+        }
+        float most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) most = max3_abs(most, v[j], v[j + 1]);
+        if (__float_as_uint(most) < 0x7F800000u) {
+          top = max(top, __float_as_uint(most));
+        } else {  // something is not finite: value by value
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+            top = max(top, b < 0x7F800000u ? b : 0u);
+          }
         }
       }
     }
@@ -273,6 +336,7 @@ __global__ void __launch_bounds__(32 * kQWarps)
   constexpr int kWordCols = kMX ? 128 : 64, kWords = kQCols / kWordCols;
   __shared__ alignas(16) uint8_t sc[kQChunks * kPitch];
   __shared__ uint32_t ss[kWords * kRows];
+  __shared__ alignas(16) typename Elem<DT>::T sx[kVec ? 1 : kQWarps][kVec ? 8 : 256];
   const int64_t row0 = (int64_t)blockIdx.x * kRows;
   const int col0 = blockIdx.y * kQCols;
   const float g = kMX || !gptr ? 1.0f : __ldg(gptr);
@@ -308,7 +372,7 @@ __global__ void __launch_bounds__(32 * kQWarps)
 #pragma unroll
     for (int k = 0; k < kQCols / (32 * kCols); ++k) {
       const int c = k * 32 * kCols + lane * kCols, n = cols - col0 - c;  // column inside the 512
-      if (n <= 0) break;
+      if (kVec ? n <= 0 : cols - col0 - k * 32 * kCols <= 0) break;
       const int blk = c / (kMX ? 32 : 16);
       const float s = fp4_scale_f32<kMX>(s8[((blk >> 2) * kRows + r) * 4 + (blk & 3)]);
       uint32_t cw = *reinterpret_cast<const uint32_t*>(sc + (c >> 5) * kPitch + r * 16 + ((c & 31) >> 3) * 4);
@@ -337,17 +401,28 @@ __global__ void __launch_bounds__(32 * kQWarps)
           o[j] = *reinterpret_cast<const uint32_t*>(&b);
         }
       }
-      if (kVec && n >= kCols) {
-        *reinterpret_cast<uint4*>(p + c) = make_uint4(o[0], o[1], o[2], o[3]);
-      } else {
+      if constexpr (kVec) {
+        if (n >= kCols) {
+          *reinterpret_cast<uint4*>(p + c) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) {
-          if (j >= n) break;
-          if constexpr (DT == BLUT_F32)
-            p[c + j] = __uint_as_float(o[j]);
-          else
-            p[c + j] = (uint16_t)(o[j / 2] >> (16 * (j & 1)));
+          for (int j = 0; j < kCols; ++j) {
+            if (j >= n) break;
+            if constexpr (DT == BLUT_F32)
+              p[c + j] = __uint_as_float(o[j]);
+            else
+              p[c + j] = (uint16_t)(o[j / 2] >> (16 * (j & 1)));
+          }
         }
+      } else {  // rows on any boundary: a lane's values side by side first
+        typename Elem<DT>::T* buf = sx[warp];
+        __syncwarp();
+        *reinterpret_cast<uint4*>(buf + lane * kCols) = make_uint4(o[0], o[1], o[2], o[3]);
+        __syncwarp();
+        const int c1 = k * 32 * kCols, left1 = cols - col0 - c1;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+          if (32 * j + lane < left1) p[c1 + 32 * j + lane] = buf[32 * j + lane];
       }
     }
   }
@@ -476,11 +551,22 @@ template <int DT>
 int launch_global(const void* x, int64_t rows, int64_t cols, int64_t ld, bool silu, float* out, cudaStream_t stream) {
   using T = typename Elem<DT>::T;
   const int64_t es = sizeof(T);
-  const int vec = alignment(x, ld * es, silu ? cols * es : 0);
+  int vec = alignment(x, ld * es, silu ? cols * es : 0);
+  const T *p = static_cast<const T*>(x), *tail = p;
+  int ntail = 0;
+  if (!silu && vec == 0 && (rows == 1 || ld == cols) && (uintptr_t)x % 16 == 0 && rows * cols >= 4096) {
+    // rows without gaps: their boundaries do not matter to a maximum
+    const int64_t total = rows * cols;
+    rows = total / 4096;
+    cols = ld = 4096;
+    ntail = (int)(total - rows * 4096);
+    tail = p + rows * 4096;
+    vec = alignment(x, ld * es, 0);
+  }
   const int64_t ctas = (rows * ((cols + 15) / 16) + 255) / 256;
   const unsigned grid = (unsigned)(ctas < 148 * 8 ? ctas : 148 * 8);
-  const T* p = static_cast<const T*>(x);
-#define BLUT_G(SILU, VEC) fp4_global_scale_kernel<DT, SILU, VEC><<<grid, 256, 0, stream>>>(p, ld, rows, (int)cols, out)
+#define BLUT_G(SILU, VEC) \
+  fp4_global_scale_kernel<DT, SILU, VEC><<<grid, 256, 0, stream>>>(p, ld, rows, (int)cols, tail, ntail, out)
   if (silu) {
     if (vec == 32) BLUT_G(true, 32); else if (vec == 16) BLUT_G(true, 16); else BLUT_G(true, 0);
   } else {

@@ -12,9 +12,9 @@
 //  * warp 0 fetches the tile's unit - 8 KB of codes and the scales of 128
 //    rows, contiguous - with one bulk copy, and the tokens' codes with four
 //    (a run of rows is contiguous per 32 columns);
-//  * warps 2, 3 bring the tokens' scales into the order that tcgen05.cp reads:
-//    they are the one operand whose position in a tile depends on where the
-//    run of rows starts;
+//  * warps 2, 3 copy the tokens' scales, word by word, into the order that
+//    tcgen05.cp reads: they are the one operand whose position in a tile
+//    depends on where the run of rows starts;
 //  * warp 1 copies both scales to tensor memory (tcgen05.cp, 32x128b,
 //    replicated to the four lane quarters) and issues two tcgen05.mma of
 //    K = 64, kind::mxf4nvf4 (a scale per 16) or kind::mxf4 (a scale per 32),
@@ -327,7 +327,6 @@ template <int kOut, class Read>
 __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha, uint8_t* stage, uint16_t* y,
                                              int64_t ldy, int left, bool vec, int lane, int c0, int cstep,
                                              const CUtensorMap* map, int row, int token0, int rows_in_y, Read read) {
-  const int mine = min(8, left - (lane & 3) * 8);  // rows of this lane's piece
   const uint32_t saddr = smem_u32(stage);
   if (c0 >= cnt) read();
 #pragma unroll 1
@@ -365,20 +364,19 @@ __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha
       continue;
     }
     __syncwarp();
+    if (vec && left == 32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = 8 * j + (lane >> 2);
-      if (c + t >= cnt) continue;
-      const uint4 u = *reinterpret_cast<const uint4*>(stage + t * 64 + ((lane & 3) ^ ((t >> 1) & 3)) * 16);
-      uint16_t* dst = y + (int64_t)(c + t) * ldy + (lane & 3) * 8;
-      if (vec && mine == 8) {
-        *reinterpret_cast<uint4*>(dst) = u;
-      } else {
-        const uint32_t words[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < mine) dst[k] = (uint16_t)(words[k >> 1] >> (16 * (k & 1)));
+      for (int j = 0; j < 4; ++j) {
+        const int t = 8 * j + (lane >> 2);
+        if (c + t < cnt)
+          *reinterpret_cast<uint4*>(y + (int64_t)(c + t) * ldy + (lane & 3) * 8) =
+              *reinterpret_cast<const uint4*>(stage + t * 64 + ((lane & 3) ^ ((t >> 1) & 3)) * 16);
       }
+    } else if (lane < left) {  // a token's rows side by side, 2 bytes a lane
+#pragma unroll 8
+      for (int t = 0; t < min(32, cnt - c); ++t)
+        y[(int64_t)(c + t) * ldy + lane] =
+            *reinterpret_cast<const uint16_t*>(stage + t * 64 + ((lane >> 3) ^ ((t >> 1) & 3)) * 16 + (lane & 7) * 2);
     }
     __syncwarp();
   }

@@ -161,7 +161,7 @@ def test_quantize_strides_and_gather(kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", [(1, 7), (5, 2048), (300, 1400)])
+@pytest.mark.parametrize("rows,cols", [(1, 7), (5, 2048), (300, 1400), (77, 2319), (1, 9001)])
 def test_global_scale(dtype, rows, cols):
     F = fp4()
     x = rand(rows, cols, dtype, 11)
@@ -171,12 +171,19 @@ def test_global_scale(dtype, rows, cols):
     assert torch.equal(q.global_scale, want)
     assert_same_codes(q, R.quantize(x, "nvfp4", want))
     assert int(q.to_checkpoint()[1].max()) == 0x7E  # the largest block has the last scale
+    for at in ((0, 0), (rows - 1, cols - 1), (rows // 2, cols // 2), (rows - 1, 0)):  # found wherever it is, any row pitch
+        big = torch.zeros(rows, cols + 3, dtype=dtype, device="cuda")
+        for y in (big[:, :cols], big[:, 1:cols + 1], torch.zeros(rows, cols, dtype=dtype, device="cuda")):
+            y.zero_()
+            y[at] = -42.0
+            assert float(F.fp4_global_scale(y)) == float(torch.tensor(42 / 2688, dtype=torch.float32))
     zero = torch.zeros(rows, cols, dtype=dtype, device="cuda")
     assert float(F.fp4_global_scale(zero)) == 2.0 ** -100
     assert int(F.quantize_fp4(zero).codes.count_nonzero()) == 0
     if cols % 2 == 0:
         h = R.silu_mul(x).abs().max()
-        # expf, the quotient and two products: below 2^-20 of the value
+        # at the largest value the exponential is at most 1, its error counts half: with the quotient and the two
+        # products below 2^-20 (far from it, where the gate nears -80, 2^-18)
         assert abs(float(F.fp4_global_scale(x, silu_mul=True)) / float(h / 2688) - 1) < 2.0 ** -20
 
 
