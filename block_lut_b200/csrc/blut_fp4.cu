@@ -26,6 +26,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "blut_fp4.cuh"
 
 namespace blut {
@@ -564,7 +566,7 @@ int launch_global(const void* x, int64_t rows, int64_t cols, int64_t ld, bool si
     vec = alignment(x, ld * es, 0);
   }
   const int64_t ctas = (rows * ((cols + 15) / 16) + 255) / 256;
-  const unsigned grid = (unsigned)(ctas < 148 * 8 ? ctas : 148 * 8);
+  const unsigned grid = (unsigned)std::min<int64_t>(ctas, 148 * 5);  // one round of CTAs
 #define BLUT_G(SILU, VEC) \
   fp4_global_scale_kernel<DT, SILU, VEC><<<grid, 256, 0, stream>>>(p, ld, rows, (int)cols, tail, ntail, out)
   if (silu) {
