@@ -34,6 +34,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "blut_fp4.cuh"
@@ -302,8 +303,8 @@ __device__ __forceinline__ void tc_ld_16x32(uint32_t taddr, uint32_t (&v)[16]) {
       : "memory");
 }
 
-// Bulk tensor store of a warp's stage, 32 tokens x 32 rows, to y at (row,
-// token); what lies outside y is not written.
+// Bulk tensor store of a warp's stage, 32 tokens x 32 rows of the matrix, to
+// y at (row, token); tokens past y are not written.
 __device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t saddr, int row, int token) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n\t"
                "cp.async.bulk.commit_group;" ::"l"(map),
@@ -318,8 +319,9 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t saddr
 // map with 64-byte swizzle expects them).  From there a full stretch of 32
 // tokens leaves as one bulk tensor store (map not null); a stretch that ends
 // inside, or a y without a map, as stores of 32 rows of 8 tokens, 16 bytes a
-// lane.  Plain stores alone kept the accumulator for 4500 cycles of an item
-// of 16 000 (128 x 192, K = 2048).  y: token 0, the warp's first row `row`,
+// lane; rows on other boundaries, or a partial tile, 2 bytes a lane, a
+// token's rows side by side.  Plain stores alone kept the accumulator for
+// 4500 cycles of an item of 16 000 (128 x 192, K = 2048).  y: token 0, the warp's first row `row`,
 // of which `left` are rows of the matrix; vec: rows of y start on 16-byte
 // boundaries; c0, cstep: the warp's stretches; read: called once the
 // accumulator has been read.
@@ -405,8 +407,8 @@ __device__ __forceinline__ void reduce_cluster(const Fp4Params& p, const float* 
 // most 8) rows themselves, 16 columns a lane and block: a launch and a pass
 // through memory less, where a call is little else.
 template <bool kMX, int NT, int kFuse>
-__global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kCtas) fp4_mm_kernel(const __grid_constant__ Fp4Params p,
-                                                                                              const __grid_constant__ CUtensorMap ymap) {
+__global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kCtas)
+    fp4_mm_kernel(const __grid_constant__ Fp4Params p, const __grid_constant__ CUtensorMap ymap) {
   using C = Fp4Cfg<kMX, NT>;
   extern __shared__ __align__(1024) uint8_t fp4_smem[];
   Fp4Header* h = reinterpret_cast<Fp4Header*>(fp4_smem);
@@ -716,7 +718,8 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
         read();
       } else if (p.out_dtype != BLUT_F32) {
         uint16_t* y = static_cast<uint16_t*>(p.y) + (int64_t)t.row0 * p.ldy + row;
-        const CUtensorMap* map = p.tma ? &ymap : nullptr;
+        // (a box that y's last rows cut is written in 16-byte pieces, past them)
+        const CUtensorMap* map = p.tma && left == 32 ? &ymap : nullptr;
         if (p.out_dtype == BLUT_BF16)
           store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi, map,
                                   (int)row, t.row0, (int)p.x_rows, read);
@@ -841,27 +844,18 @@ int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  return cudaLaunchKernelEx(&cfg, kern, (const Fp4Params)p, (const CUtensorMap)map) == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kern, (const Fp4Params)p, (const CUtensorMap)map) == cudaSuccess ? BLUT_OK
+                                                                                                   : BLUT_ERR_LAUNCH;
 }
 
-// Tokens of an item for one matrix and more than 128 tokens: the number of
-// token tiles that makes the least of rounds over the GPU's CTAs x the cost of
-// an item.  The cost follows the bytes that shared memory takes in and gives
-// out per block, which bound the loop (17 KB for the weights, 136 B a token),
-// and about four blocks' worth of time to fill and drain.  Against tiles of
-// 192: 256 x 11264 x 2048 12.8 -> 12.0 us, 1999 x 5000 x 1400 18.0 -> 17.3,
-// 4096 x 11264 x 2048 65.5 -> 63.1.
-int tokens_per_item(int64_t m, int row_tiles, int kblocks) {
-  int best = 192;
-  double least = 1e300;
-  const int64_t t0 = (m + 191) / 192;
-  for (int64_t t = t0; t <= 2 * t0 && t <= t0 + 64; ++t) {
-    const int tn = (int)(((m + t - 1) / t + 15) / 16 * 16);
-    const int64_t items = (m + tn - 1) / tn * row_tiles;
-    const double cost = (double)((items + 295) / 296) * (kblocks + 4) * (17000.0 + 136.0 * tn);
-    if (cost < least) least = cost, best = tn;
-  }
-  return best;
+// Tokens of an item for one matrix and more than 128 tokens: as few tiles as
+// 192 allow, cut evenly.  Against tiles of 192: 256 x 11264 x 2048 10.8 ->
+// 10.3 us, 300 x 2816 x 2048 10.3 -> 9.8.  More and smaller tiles that fill
+// the last round of CTAs better do not pay (1999 x 5000 x 1400: 15.3 us with
+// 192, 16.1 with 144).
+int tokens_per_item(int64_t m) {
+  const int64_t tiles = (m + 191) / 192;
+  return (int)(((m + tiles - 1) / tiles + 15) / 16 * 16);
 }
 
 template <bool kMX>
@@ -870,7 +864,7 @@ int dispatch(Fp4Params& p, int64_t m, int fuse, bool early, cudaStream_t stream)
   // tokens per matrix: their number for one matrix, the mean for runs
   const int64_t mean = p.experts ? (m + p.experts - 1) / p.experts : m;
   const int nt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 192;
-  p.tn = nt == 192 && !p.experts ? tokens_per_item(m, p.row_tiles, p.kblocks) : nt;
+  p.tn = nt == 192 && !p.experts ? tokens_per_item(m) : nt;
   // bound on the token tiles: every run may end in a partial one
   const int64_t tiles = p.experts ? m / nt + std::min<int64_t>(p.experts, m) : (m + p.tn - 1) / p.tn;
   const int64_t items = tiles * p.row_tiles;

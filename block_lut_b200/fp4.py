@@ -21,7 +21,6 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
-import math
 from dataclasses import dataclass
 from typing import Optional, Sequence, Union
 
@@ -32,7 +31,7 @@ from . import _lib
 _KIND = {"nvfp4": _lib.FP4_NV, "mxfp4": _lib.FP4_MX}
 _BLOCK = {"nvfp4": 16, "mxfp4": 32}
 _DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
-MIN_GLOBAL_SCALE = 2.0 ** -100
+MIN_GLOBAL_SCALE, MAX_GLOBAL_SCALE = 2.0 ** -100, 2.0 ** 100
 MAX_EXPERTS = 1024
 MAX_ROWS = 1 << 22  # rows of one product
 
@@ -85,8 +84,8 @@ def _scale_tensor(g: Scale, n: int, device: torch.device, what: str) -> torch.Te
             raise ValueError(f"{what} must be a float32 tensor of {n} value(s) on {device}")
         return g if n == 1 else g.reshape(n).contiguous()
     g = float(g)
-    if not (math.isfinite(g) and g >= MIN_GLOBAL_SCALE):
-        raise ValueError(f"{what} must be finite and at least 2^-100, not {g}")
+    if not MIN_GLOBAL_SCALE <= g <= MAX_GLOBAL_SCALE:
+        raise ValueError(f"{what} must be within 2^-100 .. 2^100, not {g}")
     return torch.full((n,), g, dtype=torch.float32, device=device)
 
 
@@ -212,8 +211,8 @@ def quantize_fp4(x: torch.Tensor, kind: str = "nvfp4", global_scale: Scale = Non
 
     nvfp4: s = e4m3(max|x| / (6 g)) per 16 columns; mxfp4: s = 2^(floor(log2 max|x|) - 2) per 32; q = e2m1(x / (s g)).
     Roundings go by the exact quotients (nearest, ties to even, saturating); a block with an infinity or a NaN gets
-    the scale NaN.  ``global_scale`` (nvfp4): g as a float or a float32 [1] tensor, positive, finite, at least 2^-100;
-    None takes ``fp4_global_scale(x)``.  ``row_index`` int32 [n]: row i of the result is x[row_index[i]] (gathered in
+    the scale NaN.  ``global_scale`` (nvfp4): g as a float or a float32 [1] tensor, 2^-100 .. 2^100; None
+    takes ``fp4_global_scale(x)``.  ``row_index`` int32 [n]: row i of the result is x[row_index[i]] (gathered in
     the same pass), a row of zeros where the index is outside x.
     """
     x = _rows2d(x, "x")

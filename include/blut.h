@@ -482,7 +482,7 @@ BLUT_API int blut_fp4_global_scale(const void* x, int32_t dtype, int64_t rows, i
  * row_index[r] (an index outside [0, src_rows) gives a row of zeros), or from
  * row r with row_index NULL (src_rows = desc->rows then).
  *   NV: s = e4m3(max|x| / (6 g)), nearest even, at most 448; g = *global_scale
- *       (device; positive, finite, at least 2^-100)
+ *       (device; 2^-100 .. 2^100)
  *   MX: s = 2^(floor(log2 max|x|) - 2), within 2^-127 .. 2^125; global_scale unused
  *   q = e2m1(x / (s g)), nearest even, at most 6 in magnitude; 0 where s = 0
  * Both roundings go by the exact quotient.  A block that holds an infinity or
@@ -535,7 +535,7 @@ BLUT_API int blut_fp4_matmul(const blut_fp4_mm_args* args, void* stream);
  * quantised inside the product, more before it, with the product's weight
  * copies starting meanwhile.  args as for one matrix; x_codes and x_scales
  * are ignored, x_scale NULL (NV) takes x's own maximum
- * (blut_fp4_global_scale).  The workspace (16-byte aligned;
+ * (blut_fp4_global_scale).  y must not overlap x.  The workspace (16-byte aligned;
  * blut_fp4_linear_workspace_size bytes, which may be 0: NULL then, < 0 for
  * invalid arguments; scale_given: x_scale is not NULL) is free again when
  * the work is done; calls that can overlap need one each. */

@@ -103,7 +103,7 @@ def test_python_refusals():
         F.FP4Matrix.from_checkpoint("nvfp4", torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8), 64)
     with pytest.raises(ValueError, match="no global scale"):
         F._given_scale("mxfp4", 1.0, x.device)
-    for g in (0.0, -1.0, float("inf"), float("nan"), 1e-40, torch.ones(2), torch.ones(1, dtype=torch.float64)):
+    for g in (0.0, -1.0, float("inf"), float("nan"), 1e-40, 2e30, torch.ones(2), torch.ones(1, dtype=torch.float64)):
         with pytest.raises(ValueError, match="global_scale"):
             F._given_scale("nvfp4", g, x.device)
     m = F.FP4Matrix.empty("nvfp4", 4, 64, "cpu", torch.ones(1))

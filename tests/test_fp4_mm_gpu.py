@@ -129,6 +129,14 @@ def test_output_pitch(kind):
     check(y, x, w)
     assert (big[:, :11] == 7).all() and (big[:, 211:] == 7).all()
     assert F.fp4_matmul(F.quantize_fp4(torch.zeros(0, 256, device="cuda"), kind), W).shape == (0, 200)
+    # many tokens, on 16-byte boundaries and off them, the columns beside y as they were
+    xq, x = operand(333, 256, kind, 3)
+    for n, lo in ((200, 8), (200, 11), (129, 16), (40, 24)):
+        W2 = F.FP4Weight.from_quantized(operand(n, 256, kind, 4)[0])
+        w2 = operand(n, 256, kind, 4)[1]
+        big = torch.full((333 + 40, 304), 7.0, device="cuda", dtype=torch.float16)
+        check(F.fp4_matmul(xq, W2, out=big[:333, lo:lo + n]), x, w2)
+        assert (big[:333, :lo] == 7).all() and (big[:333, lo + n:] == 7).all() and (big[333:] == 7).all(), (n, lo)
 
 
 def runs_case(E, counts, lead, tail, n, k, kind, seed=0):
