@@ -218,6 +218,30 @@ __global__ void __launch_bounds__(32 * kQWarps, kPer > 1 ? 4 : 1)
   }
 }
 
+// Largest finite |silu(g) * u| of a warp's values, each rounded once to
+// float32 (top: its bits).  Only values within 2^-17 of the largest seen so
+// far are computed in float64; `run` is that largest in the float32 form,
+// whose error is below 2^-18.  For gates below -80 the float32 form ends;
+// |u| * 1.5e-33 is more than |silu(g) * u| there.
+template <int N>
+__device__ __forceinline__ void silu_top(const float (&g)[N], const float (&u)[N], uint32_t& run, uint32_t& top) {
+  float h[N], most = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const bool far = g[j] < -80.0f;
+    h[j] = far ? fabsf(u[j]) * 1.5e-33f : fabsf(silu_mul_f32(g[j], u[j]));
+    if (!far && h[j] < 3.4e38f) most = fmaxf(most, h[j]);
+  }
+  run = max(run, __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));
+  const float floor = __uint_as_float(run) * (1.0f - kSiluWin);
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (h[j] >= floor && h[j] > 0.0f) {
+      const uint32_t b = __float_as_uint(fabsf((float)silu_mul_f64((double)g[j], (double)u[j])));
+      if (b < 0x7F800000u) top = max(top, b);
+    }
+}
+
 // g = max(max|x| / 2688, 2^-100) over the finite values: with it the largest
 // block's scale is 448.  out[0]: g, out[1] and out[2]: the running maximum's
 // bits and the CTAs that are done (zeroed before the launch).  The maximum
@@ -226,7 +250,7 @@ template <int DT, bool kSilu, int kVec>
 __global__ void __launch_bounds__(256)
     fp4_global_scale_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t ld, int64_t rows, int cols,
                             const typename Elem<DT>::T* __restrict__ tail, int ntail, float* out) {
-  uint32_t top = 0;
+  uint32_t top = 0, run = 0;
   if (blockIdx.x == 0)  // what a matrix read as one long row leaves over
     for (int c = threadIdx.x; c < ntail; c += 256) {
       const uint32_t b = __float_as_uint(Elem<DT>::f(tail[c])) & 0x7FFFFFFFu;
@@ -247,11 +271,14 @@ __global__ void __launch_bounds__(256)
         v[j] = c < cols ? Elem<DT>::f(p[c]) : 0.0f;
         if constexpr (kSilu) u[j] = c < cols ? Elem<DT>::f(p[cols + c]) : 0.0f;
       }
+      if constexpr (kSilu) {
+        silu_top<8>(v, u, run, top);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (kSilu) v[j] = silu_mul_f32(v[j], u[j]);
-        const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-        top = max(top, b < 0x7F800000u ? b : 0u);
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+          top = max(top, b < 0x7F800000u ? b : 0u);
+        }
       }
       row += drow, st += dst;
       if (st >= stretches) st -= stretches, ++row;
@@ -264,7 +291,7 @@ __global__ void __launch_bounds__(256)
     const int scol = (int)(stride - srow * per_row);
     int64_t row = first / per_row;
     int c = (int)(first - row * per_row);
-    while (row < rows) {
+    while (__any_sync(0xFFFFFFFFu, row < rows)) {  // the warp stays together
       Raw<DT> raw[kDepth], raw_up[kSilu ? kDepth : 1];
       const typename Elem<DT>::T* p[kDepth];
       int n[kDepth];
@@ -272,7 +299,7 @@ __global__ void __launch_bounds__(256)
       for (int i = 0; i < kDepth; ++i) {
         n[i] = row < rows ? min(16, cols - 16 * c) : 0;
         p[i] = x + row * ld + 16 * c;
-        if (kVec && n[i] == 16) {
+        if (n[i] == 16) {
           raw_load<DT, kVec>(p[i], raw[i]);
           if constexpr (kSilu) raw_load<DT, kVec>(p[i] + cols, raw_up[i]);
         }
@@ -281,20 +308,19 @@ __global__ void __launch_bounds__(256)
       }
 #pragma unroll
       for (int i = 0; i < kDepth; ++i) {
-        if (!n[i]) continue;
         float v[16];
-        if (kVec && n[i] == 16)
+        if (n[i] == 16)
           raw_unpack<DT>(raw[i], v);
         else
           load16<DT>(p[i], n[i], v);
         if constexpr (kSilu) {
           float u[16];
-          if (kVec && n[i] == 16)
+          if (n[i] == 16)
             raw_unpack<DT>(raw_up[i], u);
           else
             load16<DT>(p[i] + cols, n[i], u);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = silu_mul_f32(v[j], u[j]);
+          silu_top<16>(v, u, run, top);
+          continue;
         }
         float most = 0.0f;
 #pragma unroll

@@ -473,8 +473,8 @@ BLUT_API int64_t blut_fp4_tiled_bytes(const blut_fp4_desc* desc);
 
 /* out[0] = max(max|x| / 2688, 2^-100) over the finite values of x [rows][cols]
  * (row pitch ld elements, BLUT_F16 / BF16 / F32), or, with silu_mul, of
- * silu(x[:, :cols]) * x[:, cols:2 cols] computed in float32.  out: 16 bytes,
- * 16-byte aligned; the last 8 are scratch. */
+ * silu(x[:, :cols]) * x[:, cols:2 cols], each rounded once to float32.  out:
+ * 16 bytes, 16-byte aligned; all but the first 4 are scratch. */
 BLUT_API int blut_fp4_global_scale(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
                                    int32_t silu_mul, float* out, void* stream);
 

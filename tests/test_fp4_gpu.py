@@ -180,11 +180,37 @@ def test_global_scale(dtype, rows, cols):
     zero = torch.zeros(rows, cols, dtype=dtype, device="cuda")
     assert float(F.fp4_global_scale(zero)) == 2.0 ** -100
     assert int(F.quantize_fp4(zero).codes.count_nonzero()) == 0
-    if cols % 2 == 0:
-        h = R.silu_mul(x).abs().max()
-        # at the largest value the exponential is at most 1, its error counts half: with the quotient and the two
-        # products below 2^-20 (far from it, where the gate nears -80, 2^-18)
-        assert abs(float(F.fp4_global_scale(x, silu_mul=True)) / float(h / 2688) - 1) < 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 7), (5, 1024), (300, 700), (77, 1159), (2000, 1408)])
+def test_global_scale_of_silu(dtype, rows, cols):
+    """The largest product to the last bit, though most are only estimated; next to what is not finite, and where the
+    gates are far below zero."""
+    F = fp4()
+
+    def want(gu):
+        h = R.silu_mul(gu).float().abs()  # past float32 is infinite
+        h = torch.where(torch.isfinite(h), h, torch.zeros_like(h)).max().double()
+        return (h / 2688).float().clamp(min=2.0 ** -100).reshape(1)
+
+    for seed in range(3):
+        r = gen(seed)
+        gu = (torch.randn(rows, 2 * cols, generator=r, device="cuda") * 2).to(dtype)
+        assert torch.equal(F.fp4_global_scale(gu, silu_mul=True), want(gu))
+        q = F.silu_mul_quantize_fp4(gu)
+        assert torch.equal(q.global_scale, want(gu))
+        assert_same_codes(q, R.quantize(R.silu_mul(gu), "nvfp4", want(gu)))
+        many = gu.clone()
+        many[:, cols:] = many[:, cols:].clamp(-1, 1)  # products near one another
+        many[:, :cols] = many[:, :cols].clamp(max=1.0)
+        assert torch.equal(F.fp4_global_scale(many, silu_mul=True), want(many))
+        gu[0, 0], gu[rows - 1, 2 * cols - 1] = float("nan"), float("inf")
+        assert torch.equal(F.fp4_global_scale(gu, silu_mul=True), want(gu))
+    low = torch.full((rows, 2 * cols), -90.0, device="cuda", dtype=dtype)
+    low[:, cols:] = 3e4
+    low[rows // 2, 0] = -85.0
+    assert torch.equal(F.fp4_global_scale(low, silu_mul=True), want(low))
 
 
 @pytest.mark.parametrize("kind", KINDS)
