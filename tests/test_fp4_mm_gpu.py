@@ -360,3 +360,39 @@ def test_large_codes_offset(kind):
     assert int(y.count_nonzero()) <= 5 * n and m * n > 2 ** 31 and xq.codes.numel() > 2 ** 31
     d = F.dequantize_fp4(xq)
     assert torch.equal(d[at], R.values(*R.quantize(x[at], kind, gv), kind, k, gv).float().bfloat16())
+
+
+def test_beside_other_work():
+    """Products of every variant, and a LUT matmul, on streams of their own at the same time: they share the SMs' tensor
+    memory and shared memory, and nothing else."""
+    from block_lut_b200.formats import LUTFormat, encode
+    from block_lut_b200.linear import LUTLinear
+    F = fp4()
+    jobs = []
+    for m, n, k, kind in ((1, 2048, 2048, "nvfp4"), (12, 1024, 4096, "mxfp4"), (60, 512, 2048, "nvfp4"), (100, 256, 2048, "mxfp4"),
+                          (700, 3000, 1024, "nvfp4"), (300, 20000, 512, "nvfp4")):
+        xq, _ = operand(m, k, kind, m)
+        W = F.FP4Weight.from_quantized(operand(n, k, kind, n)[0])
+        jobs.append(lambda xq=xq, W=W: F.fp4_matmul(xq, W))
+    m, xq, x, WE, ws, off = runs_case(5, [3, 0, 40, 7, 100], 1, 2, 640, 1024, "nvfp4")
+    jobs.append(lambda: F.fp4_grouped_matmul(xq, WE, off, out=torch.zeros(m, 640, device="cuda", dtype=torch.float16)))
+    lin = F.FP4Linear(F.FP4Weight.quantize(torch.randn(1024, 1024, generator=gen(3), device="cuda")))
+    xs = torch.randn(20, 1024, generator=gen(4), device="cuda").bfloat16()
+    jobs.append(lambda: lin(xs))
+    lut = LUTLinear(encode(torch.randn(1024, 1024, generator=gen(5), device="cuda"), LUTFormat("b", 4, 64)))
+    xl = torch.randn(64, 1024, generator=gen(6), device="cuda").half()
+    jobs.append(lambda: lut(xl))
+    want = [j() for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(20):
+        got = []
+        for j, s in zip(jobs, streams):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    out = j()
+                got.append(out)
+        torch.cuda.synchronize()
+        for i, (g, w) in enumerate(zip(got, want)):
+            assert torch.equal(g, w), i
+    F.fp4_check_status()
