@@ -46,11 +46,16 @@ def _desc(kind: str, rows: int, cols: int) -> _lib.FP4Desc:
     return _lib.FP4Desc(_KIND[kind], 0, int(rows), int(cols))
 
 
+@functools.lru_cache(maxsize=None)
+def _function(what: str):
+    return getattr(_lib.lib(), what)
+
+
 def _launch(what: str, t: torch.Tensor, stream, *args) -> None:
     """The library's ``blut_<what>`` on t's device and the given (default: current) stream."""
-    fn = getattr(_lib.lib(), what)
+    fn = _function(what)
     dev = t.get_device()
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():  # t is on the GPU, so CUDA is set up
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream)
     else:
         with torch.cuda.device(dev):
@@ -59,17 +64,23 @@ def _launch(what: str, t: torch.Tensor, stream, *args) -> None:
         _lib.check(rc, what[5:])
 
 
-def _rows2d(x: torch.Tensor, what: str) -> torch.Tensor:
-    """x as a CUDA matrix with contiguous rows (any row pitch), copied only when its rows are not."""
+def _rows2d(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int, int]:
+    """x as a CUDA matrix with contiguous rows (any row pitch), copied only when its rows are not, with its dtype's
+    code, rows, columns and row pitch."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor (no CPU path)")
-    if x.dtype not in _DT:
+    dt = _DT.get(x.dtype)
+    if dt is None:
         raise ValueError(f"{what} must be float16, bfloat16 or float32, not {x.dtype}")
-    if x.dim() != 2 or x.shape[1] == 0:
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0:
         raise ValueError(f"{what} must be a matrix [rows, columns] with at least one column")
-    if not x.is_contiguous() and (x.stride(1) != 1 or x.stride(0) < x.shape[1]):  # transposed, expanded, overlapping
-        x = x.contiguous()
-    return x
+    rows, cols = shape
+    if x.is_contiguous():
+        return x, dt, rows, cols, cols
+    if x.stride(1) != 1 or x.stride(0) < cols:  # transposed, expanded, overlapping
+        return x.contiguous(), dt, rows, cols, cols
+    return x, dt, rows, cols, x.stride(0)
 
 
 def _pitch(x: torch.Tensor) -> int:
@@ -97,6 +108,11 @@ def _bytes_view(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.uint8 else t.view(torch.uint8)
 
 
+def _data_bytes(kind: str, rows: int, cols: int) -> int:
+    """A row takes 64 bytes of codes and 8 (nvfp4) or 4 of scales for 128 columns."""
+    return rows * (72 if kind == "nvfp4" else 68) * ((cols + 127) // 128)
+
+
 @dataclass
 class FP4Matrix:
     """Rows in 4-bit form, as the quantisers write them (the FP4 layout of ``include/blut.h``): the codes, then the
@@ -110,8 +126,7 @@ class FP4Matrix:
     @classmethod
     def empty(cls, kind: str, rows: int, cols: int, device, global_scale: Optional[torch.Tensor] = None) -> "FP4Matrix":
         _desc(kind, rows, cols)
-        unit = 72 if kind == "nvfp4" else 68  # bytes of a row's 128 columns: 64 of codes, 8 or 4 of scales
-        return cls(kind, rows, cols, torch.empty(rows * unit * ((cols + 127) // 128), dtype=torch.uint8, device=device),
+        return cls(kind, rows, cols, torch.empty(_data_bytes(kind, rows, cols), dtype=torch.uint8, device=device),
                    global_scale)
 
     def _codes_bytes(self) -> int:
@@ -171,6 +186,7 @@ def _import(kind, codes, scales, cols, global_scale, stream=None) -> FP4Matrix:
 
 
 def _given_scale(kind: str, g: Scale, device) -> Optional[torch.Tensor]:
+    """The matrix' own scale as the kernels take it: none for mxfp4, 1 where none is given for nvfp4."""
     if kind == "mxfp4":
         if g is not None:
             raise ValueError("mxfp4 has no global scale")
@@ -182,26 +198,22 @@ def _given_scale(kind: str, g: Scale, device) -> Optional[torch.Tensor]:
 def fp4_global_scale(x: torch.Tensor, silu_mul: bool = False, stream=None) -> torch.Tensor:
     """The nvfp4 scale g of x [rows, cols], float32 [1]: max|x| / 2688 over the finite values (at least 2^-100), with
     which the largest block's scale is 448, e4m3's last.  ``silu_mul``: of silu(gate) * up, x = [gate | up]."""
-    x = _rows2d(x, "x")
-    cols = _gate_cols(x) if silu_mul else x.shape[1]
-    buf = torch.empty(4, dtype=torch.float32, device=x.device)
-    if x.shape[0] == 0:
+    x, dt, rows, width, ld = _rows2d(x, "x")
+    return _global_scale(x, dt, rows, _gate_cols(width) if silu_mul else width, ld, silu_mul, stream)
+
+
+def _global_scale(x, dt, rows, cols, ld, silu_mul, stream) -> torch.Tensor:
+    buf = x.new_empty(4, dtype=torch.float32)
+    if rows == 0:
         return buf.fill_(MIN_GLOBAL_SCALE)[:1]
-    _launch("blut_fp4_global_scale", x, stream, x.data_ptr(), _DT[x.dtype], x.shape[0], cols, _pitch(x), int(silu_mul),
-            buf.data_ptr())
+    _launch("blut_fp4_global_scale", x, stream, x.data_ptr(), dt, rows, cols, ld, int(silu_mul), buf.data_ptr())
     return buf[:1]
 
 
-def _gate_cols(x: torch.Tensor) -> int:
-    if x.shape[1] % 2:
-        raise ValueError(f"rows of gate and up have an even width, not {x.shape[1]}")
-    return x.shape[1] // 2
-
-
-def _row_scale(kind: str, g: Scale, x: torch.Tensor, silu_mul: bool) -> Optional[torch.Tensor]:
-    if g is None:
-        return fp4_global_scale(x, silu_mul) if kind == "nvfp4" else None
-    return _given_scale(kind, g, x.device)
+def _gate_cols(width: int) -> int:
+    if width % 2:
+        raise ValueError(f"rows of gate and up have an even width, not {width}")
+    return width // 2
 
 
 @_lib.stream_ordered
@@ -215,22 +227,24 @@ def quantize_fp4(x: torch.Tensor, kind: str = "nvfp4", global_scale: Scale = Non
     takes ``fp4_global_scale(x)``.  ``row_index`` int32 [n]: row i of the result is x[row_index[i]] (gathered in
     the same pass), a row of zeros where the index is outside x.
     """
-    x = _rows2d(x, "x")
-    n = x.shape[0]
+    x, dt, rows, cols, ld = _rows2d(x, "x")
+    n = rows
     if row_index is not None:
         if row_index.dim() != 1 or row_index.dtype != torch.int32 or row_index.device != x.device:
             raise ValueError("row_index must be an int32 vector on x's device")
         row_index = row_index.contiguous()
         n = row_index.shape[0]
-    d = _desc(kind, n, x.shape[1])
-    g = _row_scale(kind, global_scale, x, False)
-    m = FP4Matrix.empty(kind, n, x.shape[1], x.device, g)
+    d = _desc(kind, n, cols)
+    if global_scale is None and kind == "nvfp4":
+        g = _global_scale(x, dt, rows, cols, ld, False, stream)
+    else:
+        g = _given_scale(kind, global_scale, x.device)
+    m = FP4Matrix(kind, n, cols, x.new_empty(_data_bytes(kind, n, cols), dtype=torch.uint8), g)
     if n == 0:
         return m
-    if x.shape[0] == 0:
+    if rows == 0:
         raise ValueError("row_index into an x without rows")
-    _launch("blut_fp4_quantize", x, stream, C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(row_index), x.shape[0], _p(g),
-            *m._ptrs())
+    _launch("blut_fp4_quantize", x, stream, C.byref(d), x.data_ptr(), dt, ld, _p(row_index), rows, _p(g), *m._ptrs())
     return m
 
 
@@ -239,14 +253,17 @@ def silu_mul_quantize_fp4(gate_up: torch.Tensor, kind: str = "nvfp4", global_sca
                           stream=None) -> FP4Matrix:
     """silu(gate) * up in 4-bit form, gate_up = [gate | up] [rows, 2 cols] as the gate/up products write it; rounded
     once, from the exact product to its code.  Arguments as ``quantize_fp4``."""
-    x = _rows2d(gate_up, "gate_up")
-    cols = _gate_cols(x)
-    d = _desc(kind, x.shape[0], cols)
-    g = _row_scale(kind, global_scale, x, True)
-    m = FP4Matrix.empty(kind, x.shape[0], cols, x.device, g)
-    if x.shape[0] == 0:
+    x, dt, rows, width, ld = _rows2d(gate_up, "gate_up")
+    cols = _gate_cols(width)
+    d = _desc(kind, rows, cols)
+    if global_scale is None and kind == "nvfp4":
+        g = _global_scale(x, dt, rows, cols, ld, True, stream)
+    else:
+        g = _given_scale(kind, global_scale, x.device)
+    m = FP4Matrix(kind, rows, cols, x.new_empty(_data_bytes(kind, rows, cols), dtype=torch.uint8), g)
+    if rows == 0:
         return m
-    _launch("blut_fp4_silu_mul_quantize", x, stream, C.byref(d), x.data_ptr(), _DT[x.dtype], _pitch(x), _p(g), *m._ptrs())
+    _launch("blut_fp4_silu_mul_quantize", x, stream, C.byref(d), x.data_ptr(), dt, ld, _p(g), *m._ptrs())
     return m
 
 
@@ -439,8 +456,8 @@ class FP4Linear:
         """x [..., cols] -> [..., rows] in x's dtype (or ``out_dtype``)."""
         if x.dim() == 0 or x.shape[-1] != self.cols:
             raise ValueError(f"x must be [..., {self.cols}]")
-        x2 = _rows2d(x if x.dim() == 2 else x.reshape(-1, self.cols), "x")
-        m, w = x2.shape[0], self.weight
+        x2, dt, m, _, ld = _rows2d(x if x.dim() == 2 else x.reshape(-1, self.cols), "x")
+        w = self.weight
         if x2.get_device() != w.tiled.get_device():
             raise ValueError(f"x is on {x.device}, the weight on {w.tiled.device}")
         if out is not None:
@@ -449,7 +466,7 @@ class FP4Linear:
             y = out if out.dim() == 2 else out.view(-1, self.rows)
             _check_out(y, m, w, out_dtype)
             if out.untyped_storage().data_ptr() == x2.untyped_storage().data_ptr():
-                x2 = x2.clone()  # y is written while other parts of the product still read x
+                x2, ld = x2.contiguous().clone(), self.cols  # y is written while other parts of the product still read x
         else:
             if out_dtype is not None and out_dtype not in _DT:
                 raise ValueError("the output is float16, bfloat16 or float32")
@@ -462,9 +479,9 @@ class FP4Linear:
             if need < 0:
                 raise ValueError(f"at most {MAX_ROWS} rows in one product")
             a = _lib.FP4MMArgs.from_buffer_copy(self._args)  # calls from several host threads never share one
-            a.x_rows, a.y, a.y_ld, a.out_dtype = m, y.data_ptr(), _pitch(y), _DT[y.dtype]
+            a.x_rows, a.y, a.y_ld, a.out_dtype = m, y.data_ptr(), self.rows if out is None else _pitch(y), _DT[y.dtype]
             ws = x2.new_empty(need, dtype=torch.uint8) if need else None
-            _launch("blut_fp4_linear", x2, stream, C.byref(a), x2.data_ptr(), _DT[x2.dtype], _pitch(x2), _p(ws), need)
+            _launch("blut_fp4_linear", x2, stream, C.byref(a), x2.data_ptr(), dt, ld, _p(ws), need)
         if out is not None:
             return out
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.rows)

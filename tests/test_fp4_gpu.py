@@ -267,3 +267,13 @@ def test_checkpoint_round_trip(kind):
         if kind == "nvfp4":
             f8 = F.FP4Matrix.from_checkpoint(kind, codes, scales.view(torch.float8_e4m3fn), cols, global_scale=g)
             assert torch.equal(f8.scales, q.scales)
+
+
+@pytest.mark.parametrize("rows", [0, 1, 3])
+def test_odd_gate_width_refused(rows):
+    F = fp4()
+    x = torch.ones(rows, 33, device="cuda")
+    with pytest.raises(ValueError, match="even width"):
+        F.fp4_global_scale(x, silu_mul=True)
+    with pytest.raises(ValueError, match="even width"):
+        F.silu_mul_quantize_fp4(x)
