@@ -323,12 +323,15 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t saddr
 // token's rows side by side.  Plain stores alone kept the accumulator for
 // 4500 cycles of an item of 16 000 (128 x 192, K = 2048).  y: token 0, the warp's first row `row`,
 // of which `left` are rows of the matrix; vec: rows of y start on 16-byte
-// boundaries; c0, cstep: the warp's stretches; read: called once the
-// accumulator has been read.
+// boundaries; c0, cstep: the warp's stretches; pending: a bulk store of this
+// or an earlier item (whose row tile may have been a full one where this one
+// is cut) may still be reading the stage; read: called once the accumulator
+// has been read.
 template <int kOut, class Read>
 __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha, uint8_t* stage, uint16_t* y,
                                              int64_t ldy, int left, bool vec, int lane, int c0, int cstep,
-                                             const CUtensorMap* map, int row, int token0, int rows_in_y, Read read) {
+                                             const CUtensorMap* map, bool pending, int row, int token0, int rows_in_y,
+                                             Read read) {
   const uint32_t saddr = smem_u32(stage);
   if (c0 >= cnt) read();
 #pragma unroll 1
@@ -345,7 +348,7 @@ __device__ __forceinline__ void store_tile16(uint32_t tcol, int cnt, float alpha
       for (int rg = 0; rg < 4; ++rg)
         w[tg][rg] = pack2<kOut>(__uint_as_float(v[rg >> 1][4 * tg + 2 * (rg & 1)]) * alpha,
                                 __uint_as_float(v[rg >> 1][4 * tg + 2 * (rg & 1) + 1]) * alpha);
-    if (map) {  // the stage's last store has read it
+    if (pending) {  // not before the stage's last store has read it
       if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
     }
@@ -722,10 +725,10 @@ __global__ void __launch_bounds__(Fp4Cfg<kMX, NT>::kThreads, Fp4Cfg<kMX, NT>::kC
         const CUtensorMap* map = p.tma && left == 32 ? &ymap : nullptr;
         if (p.out_dtype == BLUT_BF16)
           store_tile16<BLUT_BF16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi, map,
-                                  (int)row, t.row0, (int)p.x_rows, read);
+                                  p.tma, (int)row, t.row0, (int)p.x_rows, read);
         else
           store_tile16<BLUT_F16>(tcol, t.cnt, alpha, stage, y, p.ldy, left, p.vec, lane, 32 * part, 32 * C::kEpi, map,
-                                 (int)row, t.row0, (int)p.x_rows, read);
+                                 p.tma, (int)row, t.row0, (int)p.x_rows, read);
       } else {
 #pragma unroll 1
         for (int c = 16 * part; c < t.cnt; c += 16 * C::kEpi) {

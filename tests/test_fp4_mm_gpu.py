@@ -63,6 +63,49 @@ def test_matmul_many_items(kind, m, n, k):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(40000, 264, 64), (40000, 328, 128), (5000, 5000, 128), (30000, 1160, 256), (50000, 296, 128)])
+def test_cut_row_tile_after_a_full_one(kind, dtype, m, n, k):
+    """CTAs go from full row tiles, which leave by bulk stores, to one that the matrix cuts, which does not, with next to
+    no K between: no row of y holds another tile's values.  (The row tiles' number does not divide the CTAs', so that
+    a CTA meets both kinds.)  The float32 output takes neither way, and rounding it is the
+    16-bit output to the bit (one accumulator, one factor)."""
+    F = fp4()
+    xq, x = operand(m, k, kind, 1)
+    wq, w = operand(n, k, kind, 2, 0.05)
+    W = F.FP4Weight.from_quantized(wq)
+    wide = F.fp4_matmul(xq, W, out_dtype=torch.float32)
+    check(wide, x, w, "float32")
+    want = wide.to(dtype)
+    outs = [torch.empty(m, n, device="cuda", dtype=dtype) for _ in range(8)]
+    for out in outs:  # back to back: the stores meet a busy memory
+        out.fill_(7.0)
+        F.fp4_matmul(xq, W, out=out)
+    for out in outs:
+        assert torch.equal(out, want)
+    F.fp4_check_status()
+
+
+@pytest.mark.parametrize("n", [264, 1160])
+def test_cut_row_tile_after_a_full_one_grouped(n):
+    """The same for runs of rows, some of which end inside a stretch."""
+    F = fp4()
+    counts = [9000, 0, 8001, 1, 7777, 4095]
+    m, xq, x, W, ws, off = runs_case(len(counts), counts, 3, 5, n, 128, "nvfp4")
+    wide = F.fp4_grouped_matmul(xq, W, off, out=torch.full((m, n), 7.0, device="cuda"))
+    at = off.tolist()
+    for e in range(len(counts)):
+        if counts[e]:
+            check(wide[at[e]:at[e + 1]], x[at[e]:at[e + 1]], ws[e], f"run {e}")
+    outs = [torch.full((m, n), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(8)]
+    for out in outs:
+        F.fp4_grouped_matmul(xq, W, off, out=out)
+    for out in outs:
+        assert torch.equal(out, wide.bfloat16())
+    F.fp4_check_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("n,k", [(200, 500), (1000, 4096), (60000, 1408), (129, 33)])
 def test_linear_is_quantize_then_matmul(kind, dtype, n, k):
