@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence, Union
 
@@ -185,13 +186,13 @@ def _import(kind, codes, scales, cols, global_scale, stream=None) -> FP4Matrix:
     return m
 
 
-def _given_scale(kind: str, g: Scale, device) -> Optional[torch.Tensor]:
+def _given_scale(kind: str, g: Scale, device, what: str = "global_scale") -> Optional[torch.Tensor]:
     """The matrix' own scale as the kernels take it: none for mxfp4, 1 where none is given for nvfp4."""
     if kind == "mxfp4":
         if g is not None:
             raise ValueError("mxfp4 has no global scale")
         return None
-    return _scale_tensor(1.0 if g is None else g, 1, device, "global_scale")
+    return _scale_tensor(1.0 if g is None else g, 1, device, what)
 
 
 @_lib.stream_ordered
@@ -360,11 +361,14 @@ def _weight_quantize(w, kind, stream=None) -> FP4Weight:
     return _pack(quantize_fp4(w, kind))
 
 
-def _weight_args(w: FP4Weight) -> _lib.FP4MMArgs:
-    a = _lib.FP4MMArgs()
-    a.w = _desc(w.kind, w.rows, w.cols)
-    a.w_tiled, a.w_stride, a.w_scale = w.tiled.data_ptr(), w.stride, _p(w.global_scale)
-    return a
+_MM = struct.Struct("iiqqPqPiiPPPPqPq")  # FP4MMArgs, packed at once: a field at a time takes 1.5 us more of a call
+
+
+def _mm_args(w: FP4Weight, experts, offsets, out_dtype, x_codes, x_scales, x_scale, x_rows, y, y_ld) -> _lib.FP4MMArgs:
+    """The products' arguments: addresses (0: none) of everything but the weight, which is taken as it is now."""
+    return _lib.FP4MMArgs.from_buffer_copy(_MM.pack(
+        _KIND[w.kind], 0, w.rows, w.cols, w.tiled.data_ptr(), w.stride, _p(w.global_scale) or 0, experts, out_dtype,
+        offsets, x_codes, x_scales, x_scale, x_rows, y, y_ld))
 
 
 def _check_out(out: torch.Tensor, m: int, w: FP4Weight, out_dtype: Optional[torch.dtype]) -> None:
@@ -390,13 +394,9 @@ def _product(x: FP4Matrix, w: FP4Weight, offsets, out, out_dtype, stream) -> tor
     _check_out(out, x.rows, w, out_dtype)
     if x.rows == 0:
         return out
-    a = _weight_args(w)
-    if offsets is not None:
-        a.num_experts, a.offsets = w.experts, offsets.data_ptr()
-    a.out_dtype = _DT[out.dtype]
-    a.x_codes, a.x_scales = x._ptrs()
-    a.x_scale = _p(x.global_scale)
-    a.x_rows, a.y, a.y_ld = x.rows, out.data_ptr(), _pitch(out)
+    experts, runs = (0, 0) if offsets is None else (w.experts, offsets.data_ptr())
+    codes, scales = x._ptrs()
+    a = _mm_args(w, experts, runs, _DT[out.dtype], codes, scales, _p(x.global_scale) or 0, x.rows, out.data_ptr(), _pitch(out))
     _launch("blut_fp4_matmul", out, stream, C.byref(a))
     return out
 
@@ -433,57 +433,85 @@ def fp4_check_status(device=None, stream=None) -> None:
         _lib.check(_lib.lib().blut_fp4_check_status(_lib.stream_ptr(stream)), "fp4 status")
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_ws(kind: str, rows: int, cols: int, m: int, given: bool) -> int:
+    """Workspace bytes of a linear call on m rows, with or without a given scale of x."""
+    need = int(_lib.lib().blut_fp4_linear_workspace_size(C.byref(_desc(kind, rows, cols)), m, int(given)))
+    if need < 0:
+        raise ValueError(f"at most {MAX_ROWS} rows in one product")
+    return need
+
+
 class FP4Linear:
     """y = x W^T with a 4-bit weight and activations quantised on the way in (``blut_fp4_linear``: the product's weight
     copies start beside the quantisation).
 
     ``act_scale`` (nvfp4): the activations' global scale, from calibration (float or float32 [1] tensor); None takes
-    each call's own maximum (one more pass over x).
+    each call's own maximum (one more pass over x).  ``weight`` and ``act_scale`` can be assigned: each call takes them
+    as they are.
     """
 
     def __init__(self, weight: FP4Weight, act_scale: Scale = None):
+        self.weight = weight
+        self.act_scale = act_scale
+
+    @property
+    def weight(self) -> FP4Weight:
+        return self._weight
+
+    @weight.setter
+    def weight(self, weight: FP4Weight) -> None:
         if weight.experts is not None:
             raise ValueError("FP4Linear takes a single matrix")
-        self.weight, self.rows, self.cols = weight, weight.rows, weight.cols
-        self.act_scale = None if act_scale is None else _given_scale(weight.kind, act_scale, weight.tiled.device)
-        self._args = _weight_args(weight)
-        self._args.x_scale = _p(self.act_scale)
-        self._ws = {}  # workspace bytes per row count
+        self._weight = weight
+
+    @property
+    def act_scale(self) -> Optional[torch.Tensor]:
+        return self._act_scale
+
+    @act_scale.setter
+    def act_scale(self, g: Scale) -> None:
+        w = self._weight
+        self._act_scale = None if g is None else _given_scale(w.kind, g, w.tiled.device, "act_scale")
+
+    @property
+    def rows(self) -> int:
+        return self._weight.rows
+
+    @property
+    def cols(self) -> int:
+        return self._weight.cols
 
     @_lib.stream_ordered
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
                 stream=None) -> torch.Tensor:
         """x [..., cols] -> [..., rows] in x's dtype (or ``out_dtype``)."""
-        if x.dim() == 0 or x.shape[-1] != self.cols:
-            raise ValueError(f"x must be [..., {self.cols}]")
-        x2, dt, m, _, ld = _rows2d(x if x.dim() == 2 else x.reshape(-1, self.cols), "x")
-        w = self.weight
+        w, g = self._weight, self._act_scale
+        if x.dim() == 0 or x.shape[-1] != w.cols:
+            raise ValueError(f"x must be [..., {w.cols}]")
+        x2, dt, m, _, ld = _rows2d(x if x.dim() == 2 else x.reshape(-1, w.cols), "x")
         if x2.get_device() != w.tiled.get_device():
             raise ValueError(f"x is on {x.device}, the weight on {w.tiled.device}")
         if out is not None:
-            if tuple(out.shape) != tuple(x.shape[:-1]) + (self.rows,):
-                raise ValueError(f"out must be {list(x.shape[:-1]) + [self.rows]}")
-            y = out if out.dim() == 2 else out.view(-1, self.rows)
+            if tuple(out.shape) != tuple(x.shape[:-1]) + (w.rows,):
+                raise ValueError(f"out must be {list(x.shape[:-1]) + [w.rows]}")
+            y = out if out.dim() == 2 else out.view(-1, w.rows)
             _check_out(y, m, w, out_dtype)
             if out.untyped_storage().data_ptr() == x2.untyped_storage().data_ptr():
-                x2, ld = x2.contiguous().clone(), self.cols  # y is written while other parts of the product still read x
+                x2, ld = x2.contiguous().clone(), w.cols  # y is written while other parts of the product still read x
         else:
             if out_dtype is not None and out_dtype not in _DT:
                 raise ValueError("the output is float16, bfloat16 or float32")
-            y = x2.new_empty((m, self.rows), dtype=out_dtype or x2.dtype)
+            y = x2.new_empty((m, w.rows), dtype=out_dtype or x2.dtype)
         if m:
-            need = self._ws.get(m)
-            if need is None:
-                need = self._ws[m] = int(_lib.lib().blut_fp4_linear_workspace_size(
-                    C.byref(_desc(w.kind, w.rows, w.cols)), m, int(self.act_scale is not None)))
-            if need < 0:
-                raise ValueError(f"at most {MAX_ROWS} rows in one product")
-            a = _lib.FP4MMArgs.from_buffer_copy(self._args)  # calls from several host threads never share one
-            a.x_rows, a.y, a.y_ld, a.out_dtype = m, y.data_ptr(), self.rows if out is None else _pitch(y), _DT[y.dtype]
+            if g is not None and w.kind == "mxfp4":
+                raise ValueError("mxfp4 has no global scale")
+            need = _linear_ws(w.kind, w.rows, w.cols, m, g is not None)
+            a = _mm_args(w, 0, 0, _DT[y.dtype], 0, 0, _p(g) or 0, m, y.data_ptr(), w.rows if out is None else _pitch(y))
             ws = x2.new_empty(need, dtype=torch.uint8) if need else None
             _launch("blut_fp4_linear", x2, stream, C.byref(a), x2.data_ptr(), dt, ld, _p(ws), need)
         if out is not None:
             return out
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.rows)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.rows)
 
     __call__ = forward

@@ -176,3 +176,39 @@ def test_linear_refusals():
             lin(x)
     with pytest.raises(ValueError, match="CUDA"):
         lin(torch.zeros(4, 64))
+
+
+def test_packed_arguments():
+    """The products' arguments are packed in the order and size of the C structure's fields."""
+    w = F.FP4Weight("mxfp4", 130, 70, 3, torch.zeros(64, dtype=torch.uint8), 11, torch.ones(3))
+    assert F._MM.size == C.sizeof(_lib.FP4MMArgs)
+    a = F._mm_args(w, 3, 21, 2, 22, 23, 24, 25, 26, 27)
+    assert (a.w.kind, a.w.reserved, a.w.rows, a.w.cols) == (2, 0, 130, 70)
+    assert (a.w_tiled, a.w_stride, a.w_scale) == (w.tiled.data_ptr(), 11, w.global_scale.data_ptr())
+    assert (a.num_experts, a.offsets, a.out_dtype, a.x_codes, a.x_scales, a.x_scale) == (3, 21, 2, 22, 23, 24)
+    assert (a.x_rows, a.y, a.y_ld) == (25, 26, 27)
+    w.global_scale = None
+    assert F._mm_args(w, 0, 0, 0, 0, 0, 0, 1, 1, 1).w_scale is None
+
+
+def test_linear_attributes():
+    """What is assigned after construction is checked like the constructor's arguments, and is what sizes go by."""
+    w = F.FP4Weight("nvfp4", 128, 64, None, torch.zeros(9216, dtype=torch.uint8), 9216, torch.ones(1))
+    ws = F.FP4Weight("nvfp4", 128, 64, 2, torch.zeros(2 * 9216, dtype=torch.uint8), 9216, torch.ones(2))
+    lin = F.FP4Linear(w, 0.5)
+    lin.weight = F.FP4Weight("nvfp4", 256, 32, None, torch.zeros(2 * 9216, dtype=torch.uint8), 9216, torch.ones(1))
+    assert (lin.rows, lin.cols) == (256, 32)
+    with pytest.raises(ValueError, match="x must be"):
+        lin(torch.zeros(4, 64))
+    with pytest.raises(ValueError, match="single"):
+        lin.weight = ws
+    for g in (0.0, float("nan"), torch.ones(2), torch.ones(1, dtype=torch.float64)):
+        with pytest.raises(ValueError, match="act_scale"):
+            lin.act_scale = g
+    assert float(lin.act_scale) == 0.5 and lin.rows == 256
+    lin.act_scale = None
+    assert lin.act_scale is None
+    # the workspace goes by whether a scale is given, not by what an earlier call of as many rows had
+    assert F._linear_ws("nvfp4", 256, 32, 3, True) == 0 and F._linear_ws("nvfp4", 256, 32, 3, False) == 256
+    with pytest.raises(ValueError, match="rows in one product"):
+        F._linear_ws("nvfp4", 256, 32, F.MAX_ROWS + 1, True)

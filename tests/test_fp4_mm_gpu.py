@@ -335,6 +335,45 @@ def test_expert_layer(kind):
     assert float((y.double() - full).norm() / full.norm()) < 0.5
 
 
+def test_linear_follows_its_attributes():
+    """A scale or a weight assigned after construction is the one used, on both sides of the rows that the product
+    quantises itself; the old tensors stay alive here, so that a stale pointer gives a wrong result and no fault."""
+    F = fp4()
+    ws = [torch.randn(n, 384, generator=gen(n), device="cuda") * 0.05 for n in (256, 256, 200)]
+    Ws = [F.FP4Weight.quantize(w) for w in ws]
+    mx = F.FP4Weight.quantize(ws[2], "mxfp4")
+    scales = [None, torch.tensor([0.002], device="cuda"), torch.tensor([0.003], device="cuda"), 0.004]
+    lin = F.FP4Linear(Ws[0], scales[1])
+    for m in (3, 20):
+        x = torch.randn(m, 384, generator=gen(m), device="cuda").bfloat16()
+
+        def want(W, scale):
+            return F.fp4_matmul(F.quantize_fp4(x, W.kind, scale), W)
+
+        for W in Ws:
+            lin.weight = W
+            assert (lin.rows, lin.cols) == (W.rows, W.cols)
+            for scale in scales + scales[::-1]:
+                lin.act_scale = scale
+                assert torch.equal(lin(x), want(W, scale)), (m, W.rows, scale)
+        lin.act_scale = scales[1]
+        lin.weight = mx
+        with pytest.raises(ValueError, match="no global scale"):
+            lin(x)
+        lin.act_scale = None
+        assert torch.equal(lin(x), want(mx, None))
+        lin.weight = own = F.FP4Weight.from_quantized(F.quantize_fp4(ws[0]))  # a weight whose parts are replaced
+        assert torch.equal(lin(x), want(Ws[0], None))
+        old = own.tiled, own.global_scale
+        own.tiled, own.global_scale = Ws[1].tiled.clone(), Ws[1].global_scale * 2
+        assert torch.equal(lin(x), want(own, None)) and not torch.equal(lin(x), want(Ws[0], None))
+        own.tiled, own.global_scale = old
+    with pytest.raises(ValueError, match="single"):
+        lin.weight = F.FP4Weight.from_quantized([F.quantize_fp4(w) for w in ws[:2]])
+    with pytest.raises(ValueError, match="act_scale"):
+        lin.act_scale = -1.0
+
+
 def test_linear_in_place():
     """An output that overlaps the input is written from the input as it was."""
     F = fp4()
