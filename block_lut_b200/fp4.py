@@ -36,6 +36,8 @@ MIN_GLOBAL_SCALE, MAX_GLOBAL_SCALE = 2.0 ** -100, 2.0 ** 100
 MAX_EXPERTS = 1024
 MAX_ROWS = 1 << 22  # rows of one product
 
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
 Scale = Union[None, float, torch.Tensor]
 
 
@@ -56,8 +58,8 @@ def _launch(what: str, t: torch.Tensor, stream, *args) -> None:
     """The library's ``blut_<what>`` on t's device and the given (default: current) stream."""
     fn = _function(what)
     dev = t.get_device()
-    if dev == torch._C._cuda_getDevice():  # t is on the GPU, so CUDA is set up
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream)
+    if dev == _current_device():  # t is on the GPU, so CUDA is set up
+        rc = fn(*args, _current_stream(dev) if stream is None else stream.cuda_stream)
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _lib.stream_ptr(stream))
@@ -114,8 +116,43 @@ def _data_bytes(kind: str, rows: int, cols: int) -> int:
     return rows * (72 if kind == "nvfp4" else 68) * ((cols + 127) // 128)
 
 
+@functools.lru_cache(maxsize=4096)
+def _tiled_bytes(kind: str, rows: int, cols: int) -> int:
+    """Bytes of a matrix in the tiled layout."""
+    n = int(_lib.lib().blut_fp4_tiled_bytes(C.byref(_desc(kind, rows, cols))))
+    if n <= 0:
+        raise ValueError(f"no 4-bit weight layout for [{rows}, {cols}]")
+    return n
+
+
+class _Operand:
+    """What kernels read through: looked over before the first use after an attribute was assigned, since matrices and
+    weights can be made and changed by hand, and a kernel would read past a short buffer, or on the host."""
+    _ok = False
+
+    def __setattr__(self, name, value):
+        self.__dict__[name] = value
+        self.__dict__["_ok"] = False
+
+    def __getstate__(self):  # a copy, or one loaded from a file onto another device, is looked over again
+        return {k: v for k, v in self.__dict__.items() if k != "_ok"}
+
+    def _look_over(self, t: torch.Tensor, need: int, n: int, what: str) -> None:
+        """t holds the ``need`` bytes of codes and scales, global_scale (if there is one) n values beside it."""
+        g = self.global_scale
+        if t.dtype is not torch.uint8 or t.numel() < need or not t.is_contiguous():
+            raise ValueError(f"{what} must be at least {need} contiguous bytes (uint8)")
+        if g is not None and self.kind == "mxfp4":
+            raise ValueError("mxfp4 has no global scale")
+        if g is not None and (g.dtype is not torch.float32 or g.numel() != n or g.device != t.device or not g.is_contiguous()):
+            raise ValueError(f"global_scale must be {n} float32 value(s) on the device of {what}")
+        if not t.is_cuda:
+            raise ValueError(f"{what} must be a CUDA tensor (no CPU path)")
+        self.__dict__["_ok"] = True
+
+
 @dataclass
-class FP4Matrix:
+class FP4Matrix(_Operand):
     """Rows in 4-bit form, as the quantisers write them (the FP4 layout of ``include/blut.h``): the codes, then the
     scales, in one buffer.  ``global_scale`` float32 [1] (nvfp4) or None."""
     kind: str
@@ -144,8 +181,16 @@ class FP4Matrix:
         return self.data[self._codes_bytes():].view(-1, self.rows, 4)
 
     def _ptrs(self) -> tuple[int, int]:
+        """Addresses of the codes and the scales, which the kernels are about to write."""
         p = self.data.data_ptr()
         return p, p + self._codes_bytes()
+
+    def _operand(self) -> tuple[int, int, int]:
+        """Addresses of the codes, the scales and the global scale (0: none), which they are about to read."""
+        if not self._ok:
+            self._look_over(self.data, _data_bytes(self.kind, self.rows, self.cols), 1, "FP4Matrix.data")
+        p, g = self.data.data_ptr(), self.global_scale
+        return p, p + self._codes_bytes(), 0 if g is None else g.data_ptr()
 
     @classmethod
     def from_checkpoint(cls, kind: str, codes: torch.Tensor, scales: torch.Tensor, cols: int,
@@ -163,8 +208,17 @@ class FP4Matrix:
         scales = torch.empty(self.rows, nb, dtype=torch.uint8, device=self.data.device)
         if self.rows:
             d = _desc(self.kind, self.rows, self.cols)
-            _launch("blut_fp4_export", codes, stream, C.byref(d), *self._ptrs(), codes.data_ptr(), scales.data_ptr())
+            _launch("blut_fp4_export", codes, stream, C.byref(d), *self._operand()[:2], codes.data_ptr(), scales.data_ptr())
         return codes, scales
+
+
+def _new_matrix(kind: str, rows: int, cols: int, x: torch.Tensor, g: Optional[torch.Tensor]) -> FP4Matrix:
+    """One to be written on x's device, with a g that has been checked."""
+    m = object.__new__(FP4Matrix)
+    d = m.__dict__
+    d["kind"], d["rows"], d["cols"], d["global_scale"], d["_ok"] = kind, rows, cols, g, True
+    d["data"] = x.new_empty(_data_bytes(kind, rows, cols), dtype=torch.uint8)
+    return m
 
 
 @_lib.stream_ordered
@@ -180,7 +234,7 @@ def _import(kind, codes, scales, cols, global_scale, stream=None) -> FP4Matrix:
         raise ValueError("codes and scales must be CUDA tensors of one device")
     codes, scales = codes.contiguous(), scales.contiguous()
     g = _given_scale(kind, global_scale, codes.device)
-    m = FP4Matrix.empty(kind, rows, cols, codes.device, g)
+    m = _new_matrix(kind, rows, cols, codes, g)
     if rows:
         _launch("blut_fp4_import", codes, stream, C.byref(d), codes.data_ptr(), scales.data_ptr(), *m._ptrs())
     return m
@@ -240,7 +294,7 @@ def quantize_fp4(x: torch.Tensor, kind: str = "nvfp4", global_scale: Scale = Non
         g = _global_scale(x, dt, rows, cols, ld, False, stream)
     else:
         g = _given_scale(kind, global_scale, x.device)
-    m = FP4Matrix(kind, n, cols, x.new_empty(_data_bytes(kind, n, cols), dtype=torch.uint8), g)
+    m = _new_matrix(kind, n, cols, x, g)
     if n == 0:
         return m
     if rows == 0:
@@ -261,7 +315,7 @@ def silu_mul_quantize_fp4(gate_up: torch.Tensor, kind: str = "nvfp4", global_sca
         g = _global_scale(x, dt, rows, cols, ld, True, stream)
     else:
         g = _given_scale(kind, global_scale, x.device)
-    m = FP4Matrix(kind, rows, cols, x.new_empty(_data_bytes(kind, rows, cols), dtype=torch.uint8), g)
+    m = _new_matrix(kind, rows, cols, x, g)
     if rows == 0:
         return m
     _launch("blut_fp4_silu_mul_quantize", x, stream, C.byref(d), x.data_ptr(), dt, ld, _p(g), *m._ptrs())
@@ -277,12 +331,12 @@ def dequantize_fp4(q: FP4Matrix, dtype: torch.dtype = torch.bfloat16, stream=Non
     if q.rows == 0:
         return out
     d = _desc(q.kind, q.rows, q.cols)
-    _launch("blut_fp4_dequantize", out, stream, C.byref(d), *q._ptrs(), _p(q.global_scale), out.data_ptr(), _DT[dtype], q.cols)
+    _launch("blut_fp4_dequantize", out, stream, C.byref(d), *q._operand(), out.data_ptr(), _DT[dtype], q.cols)
     return out
 
 
 @dataclass
-class FP4Weight:
+class FP4Weight(_Operand):
     """One weight matrix [rows, cols], or one per expert, in the products' tiled layout.
 
     ``experts`` None for a single matrix; ``global_scale`` float32 [max(experts, 1)] (nvfp4) or None.
@@ -312,6 +366,12 @@ class FP4Weight:
         """From float weights [rows, cols] or [experts, rows, cols], each matrix with a global scale of its own."""
         return _weight_quantize(w, kind, stream=stream)
 
+    def _fits(self) -> None:
+        one, n = _tiled_bytes(self.kind, self.rows, self.cols), self.experts or 1
+        if n > 1 and self.stride < one:
+            raise ValueError(f"FP4Weight.stride must be at least {one}")
+        self._look_over(self.tiled, one + (n - 1) * self.stride, n, "FP4Weight.tiled")
+
     def weight_bytes(self, experts: int = 1) -> int:
         """Bytes streamed for ``experts`` matrices."""
         return experts * self.stride
@@ -328,13 +388,11 @@ def _pack(mats, stream=None) -> FP4Weight:
         raise ValueError(f"at most {MAX_EXPERTS} experts")
     m0 = mats[0]
     d = _desc(m0.kind, m0.rows, m0.cols)
-    stride = int(_lib.lib().blut_fp4_tiled_bytes(C.byref(d)))
-    if stride <= 0:
-        raise ValueError(f"no 4-bit weight layout for [{m0.rows}, {m0.cols}]")
-    dev = m0.data.device
-    tiled = torch.empty(len(mats) * stride, dtype=torch.uint8, device=dev)
-    for i, m in enumerate(mats):
-        _launch("blut_fp4_pack_tiled", tiled, stream, C.byref(d), *m._ptrs(), tiled.data_ptr() + i * stride)
+    stride = _tiled_bytes(m0.kind, m0.rows, m0.cols)
+    parts = [m._operand()[:2] for m in mats]
+    tiled = torch.empty(len(mats) * stride, dtype=torch.uint8, device=m0.data.device)
+    for i, (codes, scales) in enumerate(parts):
+        _launch("blut_fp4_pack_tiled", tiled, stream, C.byref(d), codes, scales, tiled.data_ptr() + i * stride)
     g = None if m0.kind == "mxfp4" else torch.cat([m.global_scale.reshape(1) for m in mats])
     return FP4Weight(m0.kind, m0.rows, m0.cols, None if single else len(mats), tiled, stride, g)
 
@@ -366,8 +424,11 @@ _MM = struct.Struct("iiqqPqPiiPPPPqPq")  # FP4MMArgs, packed at once: a field at
 
 def _mm_args(w: FP4Weight, experts, offsets, out_dtype, x_codes, x_scales, x_scale, x_rows, y, y_ld) -> _lib.FP4MMArgs:
     """The products' arguments: addresses (0: none) of everything but the weight, which is taken as it is now."""
+    g = w.global_scale
+    if not w._ok:
+        w._fits()
     return _lib.FP4MMArgs.from_buffer_copy(_MM.pack(
-        _KIND[w.kind], 0, w.rows, w.cols, w.tiled.data_ptr(), w.stride, _p(w.global_scale) or 0, experts, out_dtype,
+        _KIND[w.kind], 0, w.rows, w.cols, w.tiled.data_ptr(), w.stride, 0 if g is None else g.data_ptr(), experts, out_dtype,
         offsets, x_codes, x_scales, x_scale, x_rows, y, y_ld))
 
 
@@ -390,13 +451,15 @@ def _product(x: FP4Matrix, w: FP4Weight, offsets, out, out_dtype, stream) -> tor
     if x.rows > MAX_ROWS:
         raise ValueError(f"at most {MAX_ROWS} rows in one product")
     if out is None:
+        if out_dtype is not None and out_dtype not in _DT:
+            raise ValueError("the output is float16, bfloat16 or float32")
         out = x.data.new_empty((x.rows, w.rows), dtype=out_dtype or torch.bfloat16)
-    _check_out(out, x.rows, w, out_dtype)
+    else:
+        _check_out(out, x.rows, w, out_dtype)
     if x.rows == 0:
         return out
     experts, runs = (0, 0) if offsets is None else (w.experts, offsets.data_ptr())
-    codes, scales = x._ptrs()
-    a = _mm_args(w, experts, runs, _DT[out.dtype], codes, scales, _p(x.global_scale) or 0, x.rows, out.data_ptr(), _pitch(out))
+    a = _mm_args(w, experts, runs, _DT[out.dtype], *x._operand(), x.rows, out.data_ptr(), _pitch(out))
     _launch("blut_fp4_matmul", out, stream, C.byref(a))
     return out
 
@@ -419,7 +482,7 @@ def fp4_grouped_matmul(x: FP4Matrix, w: FP4Weight, offsets: torch.Tensor, out: O
     the host and the call can be captured.  Runs may be empty or start anywhere.  Rows of ``out`` outside every run
     (before offsets[0], from offsets[-1]) are left as they were; without ``out`` they are undefined.
     """
-    if not isinstance(w, FP4Weight) or w.experts is None:
+    if not isinstance(w, FP4Weight) or not w.experts:
         raise ValueError("fp4_grouped_matmul takes a stack of experts")
     if not isinstance(offsets, torch.Tensor) or offsets.dtype != torch.int32 or tuple(offsets.shape) != (w.experts + 1,) \
             or offsets.device != w.tiled.device:
@@ -487,11 +550,17 @@ class FP4Linear:
                 stream=None) -> torch.Tensor:
         """x [..., cols] -> [..., rows] in x's dtype (or ``out_dtype``)."""
         w, g = self._weight, self._act_scale
-        if x.dim() == 0 or x.shape[-1] != w.cols:
+        flat = x.dim() == 2
+        if not flat and (x.dim() == 0 or x.shape[-1] != w.cols):
             raise ValueError(f"x must be [..., {w.cols}]")
-        x2, dt, m, _, ld = _rows2d(x if x.dim() == 2 else x.reshape(-1, w.cols), "x")
-        if x2.get_device() != w.tiled.get_device():
+        x2, dt, m, k, ld = _rows2d(x if flat else x.reshape(-1, w.cols), "x")
+        if k != w.cols:
+            raise ValueError(f"x must be [..., {w.cols}]")
+        dev = x2.get_device()
+        if dev != w.tiled.get_device():
             raise ValueError(f"x is on {x.device}, the weight on {w.tiled.device}")
+        if g is not None and (w.kind == "mxfp4" or g.get_device() != dev):  # the weight was another one when it was given
+            raise ValueError("act_scale: mxfp4 has no global scale" if w.kind == "mxfp4" else f"act_scale must be on {x.device}")
         if out is not None:
             if tuple(out.shape) != tuple(x.shape[:-1]) + (w.rows,):
                 raise ValueError(f"out must be {list(x.shape[:-1]) + [w.rows]}")
@@ -502,16 +571,15 @@ class FP4Linear:
         else:
             if out_dtype is not None and out_dtype not in _DT:
                 raise ValueError("the output is float16, bfloat16 or float32")
-            y = x2.new_empty((m, w.rows), dtype=out_dtype or x2.dtype)
+            y = x2.new_empty((m, w.rows), dtype=out_dtype) if out_dtype else x2.new_empty((m, w.rows))
         if m:
-            if g is not None and w.kind == "mxfp4":
-                raise ValueError("mxfp4 has no global scale")
             need = _linear_ws(w.kind, w.rows, w.cols, m, g is not None)
-            a = _mm_args(w, 0, 0, _DT[y.dtype], 0, 0, _p(g) or 0, m, y.data_ptr(), w.rows if out is None else _pitch(y))
+            a = _mm_args(w, 0, 0, _DT[y.dtype], 0, 0, 0 if g is None else g.data_ptr(), m, y.data_ptr(),
+                         w.rows if out is None else _pitch(y))
             ws = x2.new_empty(need, dtype=torch.uint8) if need else None
             _launch("blut_fp4_linear", x2, stream, C.byref(a), x2.data_ptr(), dt, ld, _p(ws), need)
         if out is not None:
             return out
-        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.rows)
+        return y if flat else y.reshape(*x.shape[:-1], w.rows)
 
     __call__ = forward

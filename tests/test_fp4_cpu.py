@@ -1,5 +1,7 @@
 """4-bit microscaled operators without a GPU: sizes, refusals, and the float64 restatement against itself."""
+import copy
 import ctypes as C
+import pickle
 
 import pytest
 import torch
@@ -180,15 +182,63 @@ def test_linear_refusals():
 
 def test_packed_arguments():
     """The products' arguments are packed in the order and size of the C structure's fields."""
-    w = F.FP4Weight("mxfp4", 130, 70, 3, torch.zeros(64, dtype=torch.uint8), 11, torch.ones(3))
     assert F._MM.size == C.sizeof(_lib.FP4MMArgs)
-    a = F._mm_args(w, 3, 21, 2, 22, 23, 24, 25, 26, 27)
+    a = _lib.FP4MMArgs.from_buffer_copy(F._MM.pack(2, 0, 130, 70, 10, 11, 12, 3, 2, 21, 22, 23, 24, 25, 26, 27))
     assert (a.w.kind, a.w.reserved, a.w.rows, a.w.cols) == (2, 0, 130, 70)
-    assert (a.w_tiled, a.w_stride, a.w_scale) == (w.tiled.data_ptr(), 11, w.global_scale.data_ptr())
+    assert (a.w_tiled, a.w_stride, a.w_scale) == (10, 11, 12)
     assert (a.num_experts, a.offsets, a.out_dtype, a.x_codes, a.x_scales, a.x_scale) == (3, 21, 2, 22, 23, 24)
     assert (a.x_rows, a.y, a.y_ld) == (25, 26, 27)
-    w.global_scale = None
-    assert F._mm_args(w, 0, 0, 0, 0, 0, 0, 1, 1, 1).w_scale is None
+
+
+@pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
+def test_operands_are_checked_where_they_are_read(kind):
+    """Matrices and weights can be made and changed by hand: what a kernel would read past, or on the host, is refused."""
+    b, unit = (72, 9216) if kind == "nvfp4" else (68, 8704)
+    g = torch.ones(1) if kind == "nvfp4" else None
+
+    def mat(n, dtype=torch.uint8, g=g):
+        return F.FP4Matrix(kind, 4, 130, torch.zeros(n, dtype=dtype), g)
+
+    def weight(n, experts=None, stride=4 * unit, g=g):
+        return F.FP4Weight(kind, 200, 130, experts, torch.zeros(n, dtype=torch.uint8), stride, g)
+
+    full = 4 * 2 * b
+    x, w, ws, off = mat(full), weight(4 * unit), weight(12 * unit, 3, g=None), torch.zeros(4, dtype=torch.int32)
+    for bad, match in ((mat(full - 1), "bytes"), (mat(full, torch.int8), "bytes"), (x, "CUDA")):
+        for call in (lambda: F.dequantize_fp4(bad), bad.to_checkpoint, lambda: F.FP4Weight.from_quantized(bad),
+                     lambda: F.FP4Weight.from_quantized([bad, bad])):
+            with pytest.raises(ValueError, match=match):
+                call()
+    bad = mat(2 * full)
+    bad.data = bad.data[::2]
+    with pytest.raises(ValueError, match="bytes"):
+        F.dequantize_fp4(bad)
+    with pytest.raises(ValueError, match="CUDA"):
+        F.fp4_matmul(x, w)
+    with pytest.raises(ValueError, match="CUDA"):
+        F.fp4_grouped_matmul(x, ws, off)
+    for bad, match in ((weight(4 * unit - 1), "bytes"), (weight(12 * unit - 1, 3), "bytes"), (weight(12 * unit, 3, 4 * unit - 16), "stride"),
+                       (weight(12 * unit, 3, 5 * unit), "bytes"), (weight(4 * unit), "CUDA")):
+        with pytest.raises(ValueError, match=match):
+            F._mm_args(bad, bad.experts or 0, 0, 1, 0, 0, 0, 4, 0, 200)
+    for t in (torch.ones(2), torch.ones(1, dtype=torch.float64), torch.ones(1, device="meta")):
+        with pytest.raises(ValueError, match="global.scale"):
+            F.dequantize_fp4(mat(full, g=t))
+        with pytest.raises(ValueError, match="global.scale"):
+            F._mm_args(weight(4 * unit, g=t), 0, 0, 1, 0, 0, 0, 4, 0, 200)
+    with pytest.raises(ValueError, match="global.scale"):
+        F._mm_args(weight(12 * unit, 3, g=torch.ones(6)[::2]), 3, 0, 1, 0, 0, 0, 4, 0, 200)
+    m = F._new_matrix(kind, 4, 130, torch.zeros(1), g)
+    assert m.data.numel() == full and m._operand()[0] == m.data.data_ptr()  # made to measure: taken as it is, until something is assigned
+    for again in (copy.copy(m), copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        assert (again.kind, again.rows, again.cols) == (kind, 4, 130) and torch.equal(again.data, m.data)
+        with pytest.raises(ValueError, match="CUDA"):
+            again._operand()
+    m.rows = 5
+    with pytest.raises(ValueError, match="bytes"):
+        m._operand()
+    with pytest.raises(ValueError, match="stack"):
+        F.fp4_grouped_matmul(x, weight(4 * unit, 0), off[:1])
 
 
 def test_linear_attributes():

@@ -407,6 +407,47 @@ def test_a_wait_that_runs_out_is_reported(m, n, k):
     F.fp4_check_status()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_operands_made_by_hand(kind):
+    """What a kernel would read past its end or on the host is refused before a launch; buffers that hold enough work."""
+    F = fp4()
+    xq, x = operand(20, 200, kind, 1)
+    wq, w = operand(130, 200, kind, 2)
+    W = F.FP4Weight.from_quantized(wq)
+    lin = F.FP4Linear(W)
+    xf = torch.randn(20, 200, generator=gen(3), device="cuda")
+    want, wl = F.fp4_matmul(xq, W), lin(xf)
+
+    def calls(q, v):
+        own = F.FP4Linear(v)
+        return ((q, lambda: F.dequantize_fp4(q)), (q, q.to_checkpoint), (q, lambda: F.FP4Weight.from_quantized(q)),
+                (q, lambda: F.fp4_matmul(q, W)), (v, lambda: F.fp4_matmul(xq, v)), (v, lambda: own(xf)), (v, lambda: own(xf[:2])))
+
+    def like(q=xq, v=W, **kw):
+        return (F.FP4Matrix(q.kind, q.rows, q.cols, kw.get("data", q.data), kw.get("gx", q.global_scale)),
+                F.FP4Weight(v.kind, v.rows, v.cols, None, kw.get("tiled", v.tiled), v.stride, kw.get("gw", v.global_scale)))
+
+    for kw in (dict(data=xq.data[:-16], tiled=W.tiled[:-16]), dict(data=xq.data.cpu(), tiled=W.tiled.cpu()),
+               dict(data=xq.data.view(torch.int8), tiled=W.tiled.view(torch.int8)), dict(gx=torch.ones(1), gw=torch.ones(1)),
+               dict(gx=torch.ones(2, device="cuda"), gw=torch.ones(2, device="cuda"))):
+        for _, call in calls(*like(**kw)):
+            with pytest.raises(ValueError):
+                call()
+    more, moreW = like(data=torch.cat((xq.data, xq.data)), tiled=torch.cat((W.tiled, W.tiled)))
+    assert torch.equal(F.fp4_matmul(more, moreW), want)
+    one, oneW = like(gx=None, gw=None)  # no scale: 1
+    if kind == "nvfp4":
+        gg = xq.global_scale * W.global_scale
+        assert torch.equal(F.fp4_matmul(one, oneW, out_dtype=torch.float32) * gg, F.fp4_matmul(xq, W, out_dtype=torch.float32))
+        lin.act_scale = torch.ones(1, device="cuda")
+        lin._act_scale = torch.ones(1)
+        for rows in (2, 20):
+            with pytest.raises(ValueError, match="act_scale"):
+                lin(xf[:rows])
+        lin.act_scale = None
+    assert torch.equal(lin(xf), wl) and torch.equal(F.fp4_matmul(xq, W), want)
+
+
 def test_first_call_in_a_capture():
     """A process whose first product is captured: the launch set-up works inside a capture."""
     import subprocess
