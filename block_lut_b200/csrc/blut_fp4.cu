@@ -44,7 +44,7 @@ __device__ __forceinline__ float silu_mul_f32(float g, float u) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * r * u;
+  return g * (r * u);  // g * r would lose digits where g is below float32's normal range
 }
 __device__ __forceinline__ double silu_mul_f64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
 

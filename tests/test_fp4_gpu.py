@@ -253,6 +253,27 @@ def test_silu_mul_range(kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_silu_mul_smallest_gates(kind, dtype):
+    """Gates below float32's normal range times an up that brings the product back into it."""
+    F = fp4()
+    r = gen(17)
+    least = {torch.bfloat16: -133, torch.float32: -149}[dtype]  # gates are small multiples of the smallest one
+    k = torch.randint(1, 200, (40, 64), generator=r, device="cuda").double()
+    k[:20] = torch.randint(1, 9, (20, 64), generator=r, device="cuda").double()
+    gate = k * 2.0 ** least * torch.where(torch.rand(40, 64, generator=r, device="cuda") < 0.5, -1, 1)
+    up = torch.exp2(torch.randint(95, 126, (40, 1), generator=r, device="cuda").double()).expand(-1, 64)
+    gu = torch.cat((gate, up), 1).to(dtype)
+    h = R.silu_mul(gu)
+    assert (gu[:20, :64].float().abs() < 2.0 ** -126).all() and gu[:, :64].count_nonzero() == gu[:, :64].numel()
+    for row in (slice(0, 40), slice(3, 4)):
+        gr = None if kind == "mxfp4" else (h[row].abs().max() / 2688).float().clamp(min=2.0 ** -100).reshape(1)
+        assert_same_codes(F.silu_mul_quantize_fp4(gu[row], kind, global_scale=gr), R.quantize(h[row], kind, 1.0 if gr is None else gr))
+        if kind == "nvfp4":
+            assert torch.equal(F.fp4_global_scale(gu[row], silu_mul=True), gr)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_checkpoint_round_trip(kind):
     F = fp4()
     for rows, cols in ((1, 5), (130, 200), (33, 1408)):
