@@ -61,6 +61,7 @@ __device__ __noinline__ void encode_block_f64(const typename Elem<DT>::T* row, i
   double m = fabs(x);
 #pragma unroll
   for (int d = 16; d; d >>= 1) m = fmax(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+  const bool bad = __any_sync(0xFFFFFFFFu, isnan(x)) || isinf((float)m);  // not finite as a float32
   uint32_t s;
   double unit;
   if constexpr (kMX) {
@@ -75,6 +76,7 @@ __device__ __noinline__ void encode_block_f64(const typename Elem<DT>::T* row, i
   for (uint32_t k = 0; k < 7; ++k)
     if (unit > 0.0 && q == k) q = e2m1_decide(fabs(x), unit, k);
   q |= signbit(x) ? 8u : 0u;
+  if (bad) s = kMX ? 0xFFu : 0x7Fu, q = 0;
   q <<= 4 * (lane & 7);  // eight lanes make a word
 #pragma unroll
   for (int d = 1; d < 8; d <<= 1) q |= __shfl_xor_sync(0xFFFFFFFFu, q, d);

@@ -84,6 +84,7 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* v) {
   return d;
 }
 
+constexpr uint32_t kSiluEnd = 0x7F7FFF00u;  // bits of the largest float32 less 2^-16 of it
 constexpr float kSiluWin = 0x1p-17f;  // twice the error of a float32 silu(gate) * up / (s g)
 
 template <int DT>
@@ -217,7 +218,10 @@ __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool& u
   for (int i = 0; i < 16; i += 2) most = max3_abs(most, v[i], v[i + 1]);
   uint32_t top = __float_as_uint(most) & 0x7FFFFFFFu;  // bits of non-negative floats order as integers, NaN last
   if (kMX) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-  const bool bad = top >= 0x7F800000u;  // an infinity or a NaN: the block has no scale
+  // an infinity or a NaN: the block has no scale (whether a product passes
+  // float32's end is not for an estimate to say)
+  const bool bad = kSilu ? top > 0x7F800000u : top >= 0x7F800000u;
+  if (kSilu) unsure |= top >= kSiluEnd;
   const float a = __uint_as_float(top);
   float r, unit = 0.0f;
   if constexpr (kMX) {

@@ -490,8 +490,9 @@ BLUT_API int blut_fp4_global_scale(const void* x, int32_t dtype, int64_t rows, i
 BLUT_API int blut_fp4_quantize(const blut_fp4_desc* desc, const void* x, int32_t dtype, int64_t ld,
                                const int32_t* row_index, int64_t src_rows, const float* global_scale, void* codes,
                                void* scales, void* stream);
-/* The same of silu(gate) * up, rounded once: gate_up [rows][2 cols], gate in
- * the first half of a row (the order of the gate/up products here). */
+/* The same of silu(gate) * up, rounded once (a product that a float32 cannot
+ * hold counts as an infinity): gate_up [rows][2 cols], gate in the first half
+ * of a row (the order of the gate/up products here). */
 BLUT_API int blut_fp4_silu_mul_quantize(const blut_fp4_desc* desc, const void* gate_up, int32_t dtype, int64_t ld,
                                         const float* global_scale, void* codes, void* scales, void* stream);
 /* FP4 layout -> out [rows][cols] (row pitch ld elements); global_scale NULL: 1. */

@@ -274,6 +274,34 @@ def test_silu_mul_smallest_gates(kind, dtype):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_silu_mul_end_of_range(kind):
+    """Products next to the largest float32: a block is finite exactly where its products round to finite float32."""
+    F = fp4()
+    top = torch.finfo(torch.float32).max
+    r = gen(23)
+    cols = 64
+    gate = 1.5 + 12 * torch.rand(1800, 1, generator=r, device="cuda").expand(-1, cols)
+    silu = gate.double() / (1 + torch.exp(-gate.double()))
+    at = (torch.rand(1800, 1, generator=r, device="cuda").double() - 0.5) * 2.0 ** -15  # within 2^-16 of the end, both sides,
+    at[::3] *= 2.0 ** -7  # and within a few of its last digits
+    at[1::3] *= 2.0 ** -8
+    up = (top / silu * (1 + at)).clamp(max=top).float()
+    up[:, 1::2] *= 0.3
+    up[1200:, cols - 1] = float("nan")
+    gu = torch.cat((gate, up), 1)
+    h = R.silu_mul(gu)
+    href = torch.where(torch.isinf(h.float()), torch.full_like(h, float("inf")), h)
+    finite = torch.isfinite(href[:1200]).all(1)
+    assert 200 < int(finite.sum()) < 1000
+    g = None if kind == "mxfp4" else torch.tensor([2.0 ** 100], device="cuda")
+    assert_same_codes(F.silu_mul_quantize_fp4(gu, kind, global_scale=g), R.quantize(href, kind, 1.0 if g is None else g))
+    one = gu[:1200][finite]
+    if kind == "nvfp4":
+        want = (R.silu_mul(one).abs().max().float().double() / 2688).float().reshape(1)
+        assert torch.equal(F.fp4_global_scale(one.contiguous(), silu_mul=True), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_checkpoint_round_trip(kind):
     F = fp4()
     for rows, cols in ((1, 5), (130, 200), (33, 1408)):
