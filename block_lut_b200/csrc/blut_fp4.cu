@@ -16,7 +16,7 @@
 // x's own maximum (0.8 % of bf16 values are ties) and cost a few instructions
 // each.  silu(gate) * up is
 // rounded once, to its code: it is computed in float32 from the hardware's
-// approximate exponential and reciprocal (relative error below 2^-18, window
+// approximate exponential and reciprocal (relative error below 2^-17.8, window
 // 2^-17); a block with a value near a border is done again in float64, a
 // column a lane (about 1 block in 3000).
 //
@@ -38,8 +38,11 @@ constexpr int kQCols = 512;    // columns per CTA, 16 per lane
 constexpr int kQChunks = kQCols / 32;
 constexpr float kMinGlobal = 7.888609052210118e-31f;  // 2^-100
 
-// silu(g) * u in float32 for g >= -80: the exponent's rounding costs at most
-// 2^-18.5 (at g = -80), ex2 and rcp 2^-22 each, three products 2^-24 each.
+// silu(g) * u in float32 for g >= -80, relative error below 2^-17.8: at g =
+// -80 the exponent g * log2(e) is rounded by up to 2^-18, and its constant,
+// off by 2^-25.6, moves it by 2^-19.3, which together cost ln 2 * 5.36e-6 =
+// 3.72e-6; ex2 costs 2^-22, rcp 2^-23, the sum and two products 2^-24 each:
+// 4.25e-6 in all.
 __device__ __forceinline__ float silu_mul_f32(float g, float u) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
@@ -221,9 +224,9 @@ __global__ void __launch_bounds__(32 * kQWarps, kPer > 1 ? 4 : 1)
 }
 
 // Largest finite |silu(g) * u| of a warp's values, each rounded once to
-// float32 (top: its bits).  Only values within 2^-17 of the largest seen so
-// far are computed in float64; `run` is that largest in the float32 form,
-// whose error is below 2^-18.  For gates below -80 the float32 form ends;
+// float32 (top: its bits).  Only values within 2^-16 of the largest seen so
+// far are computed in float64: both this value and `run`, that largest in the
+// float32 form, are off by less than 2^-17.  For gates below -80 the float32 form ends;
 // |u| * 1.5e-33 is more than |silu(g) * u| there.
 template <int N>
 __device__ __forceinline__ void silu_top(const float (&g)[N], const float (&u)[N], uint32_t& run, uint32_t& top) {
@@ -235,7 +238,7 @@ __device__ __forceinline__ void silu_top(const float (&g)[N], const float (&u)[N
     if (!far && h[j] < 3.4e38f) most = fmaxf(most, h[j]);
   }
   run = max(run, __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));
-  const float floor = __uint_as_float(run) * (1.0f - kSiluWin);
+  const float floor = __uint_as_float(run) * (1.0f - 2.0f * kSiluWin);
 #pragma unroll
   for (int j = 0; j < N; ++j)
     if (h[j] >= floor && h[j] > 0.0f) {

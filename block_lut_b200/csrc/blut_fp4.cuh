@@ -85,7 +85,9 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* v) {
 }
 
 constexpr uint32_t kSiluEnd = 0x7F7FFF00u;  // bits of the largest float32 less 2^-16 of it
-constexpr float kSiluWin = 0x1p-17f;  // twice the error of a float32 silu(gate) * up / (s g)
+// More than the error of a float32 estimate of silu(gate) * up / (s g): 2^-17.8
+// of the product (silu_mul_f32), four roundings of the quotient.
+constexpr float kSiluWin = 0x1p-17f;
 
 template <int DT>
 struct Elem;

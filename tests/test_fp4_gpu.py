@@ -301,6 +301,27 @@ def test_silu_mul_end_of_range(kind):
         assert torch.equal(F.fp4_global_scale(one.contiguous(), silu_mul=True), want)
 
 
+@pytest.mark.parametrize("low,high", [(-80, -60), (-64, -46), (-80, -1)])
+def test_global_scale_of_near_products(low, high):
+    """Products within float32's rounding of one another, at gates whose estimates are least exact: the largest is found."""
+    F = fp4()
+    rows, cols = 400, 512
+    r = gen(-low)
+    for seed in range(4):
+        gate = (low + (high - low) * torch.rand(rows, cols, generator=r, device="cuda")).clamp(min=-80.0)
+        silu = R.silu_mul(torch.cat((gate, torch.ones_like(gate)), 1))
+        near = 1 + torch.rand(rows, cols, generator=r, device="cuda").double() * 2.0 ** (-17 - seed)
+        gu = torch.cat((gate, (1000 * near / silu).float()), 1)
+        h = R.silu_mul(gu)
+        want = (h.abs().max().float().double() / 2688).float().reshape(1)
+        assert torch.equal(F.fp4_global_scale(gu, silu_mul=True), want)
+        at = int(h.abs().argmax())  # that value alone among the smallest of the others
+        gu[:, cols:] *= 1 - 2.0 ** -18
+        gu.view(-1)[at // cols * 2 * cols + cols + at % cols] /= 1 - 2.0 ** -18
+        want = (R.silu_mul(gu).abs().max().float().double() / 2688).float().reshape(1)
+        assert torch.equal(F.fp4_global_scale(gu, silu_mul=True), want)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_checkpoint_round_trip(kind):
     F = fp4()
