@@ -297,8 +297,9 @@ def quantize_fp4(x: torch.Tensor, kind: str = "nvfp4", global_scale: Scale = Non
     m = _new_matrix(kind, n, cols, x, g)
     if n == 0:
         return m
-    if rows == 0:
-        raise ValueError("row_index into an x without rows")
+    if rows == 0:  # every index is outside x
+        m.data.zero_()
+        return m
     _launch("blut_fp4_quantize", x, stream, C.byref(d), x.data_ptr(), dt, ld, _p(row_index), rows, _p(g), *m._ptrs())
     return m
 

@@ -160,6 +160,20 @@ def test_quantize_strides_and_gather(kind, dtype):
     assert F.quantize_fp4(x, kind, global_scale=g, row_index=idx[:0]).codes.numel() == 0
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_gather_from_no_rows(kind):
+    """Every index is outside an x without rows: rows of zeros."""
+    F = fp4()
+    x = torch.empty(0, 200, device="cuda")
+    idx = torch.tensor([0, -1, 5], dtype=torch.int32, device="cuda")
+    for g in (None, 0.5) if kind == "nvfp4" else (None,):
+        q = F.quantize_fp4(x, kind, global_scale=g, row_index=idx)
+        assert (q.rows, q.cols) == (3, 200) and int(q.data.count_nonzero()) == 0
+        assert torch.equal(F.dequantize_fp4(q, torch.float32), torch.zeros(3, 200, device="cuda"))
+        q = F.quantize_fp4(x, kind, global_scale=g, row_index=idx[:0])
+        assert q.rows == 0 and q.codes.numel() == 0
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 7), (5, 2048), (300, 1400), (77, 2319), (1, 9001)])
 def test_global_scale(dtype, rows, cols):
