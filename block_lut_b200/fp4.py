@@ -394,7 +394,9 @@ def _pack(mats, stream=None) -> FP4Weight:
     tiled = torch.empty(len(mats) * stride, dtype=torch.uint8, device=m0.data.device)
     for i, (codes, scales) in enumerate(parts):
         _launch("blut_fp4_pack_tiled", tiled, stream, C.byref(d), codes, scales, tiled.data_ptr() + i * stride)
-    g = None if m0.kind == "mxfp4" else torch.cat([m.global_scale.reshape(1) for m in mats])
+    g = None
+    if m0.kind == "nvfp4":  # (no scale: 1, as in the products)
+        g = torch.cat([tiled.new_ones(1, dtype=torch.float32) if m.global_scale is None else m.global_scale.reshape(1) for m in mats])
     return FP4Weight(m0.kind, m0.rows, m0.cols, None if single else len(mats), tiled, stride, g)
 
 

@@ -408,6 +408,22 @@ def test_a_wait_that_runs_out_is_reported(m, n, k):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_no_global_scale_is_one(kind):
+    """A matrix without a global scale stands for g = 1 as an operand, on the way back, and as a weight."""
+    F = fp4()
+    for rows in (20, 130):
+        xq, x = operand(rows, 200, kind, 1)
+        bare = F.FP4Matrix(kind, rows, 200, xq.data)
+        one = F.FP4Matrix(kind, rows, 200, xq.data, None if kind == "mxfp4" else torch.ones(1, device="cuda"))
+        assert torch.equal(F.dequantize_fp4(bare), F.dequantize_fp4(one))
+        W, W1 = F.FP4Weight.from_quantized(bare), F.FP4Weight.from_quantized(one)
+        assert torch.equal(F.fp4_matmul(bare, W), F.fp4_matmul(one, W1))
+        E, E1 = F.FP4Weight.from_quantized([bare, xq]), F.FP4Weight.from_quantized([one, xq])
+        off = torch.tensor([0, 7, rows], dtype=torch.int32, device="cuda")
+        assert torch.equal(F.fp4_grouped_matmul(bare, E, off), F.fp4_grouped_matmul(one, E1, off))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_operands_made_by_hand(kind):
     """What a kernel would read past its end or on the host is refused before a launch; buffers that hold enough work."""
     F = fp4()
