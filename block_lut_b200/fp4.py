@@ -91,6 +91,16 @@ def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+def _overlap(rows: int, a: int, a_pitch: int, a_width: int, b: int, b_pitch: int, b_width: int) -> bool:
+    """Whether two matrices of as many rows may share a byte (address, bytes between rows, bytes of a row)."""
+    if a + (rows - 1) * a_pitch + a_width <= b or b + (rows - 1) * b_pitch + b_width <= a:
+        return False
+    if a_pitch != b_pitch or rows == 1:
+        return True
+    d = (b - a) % a_pitch  # columns of one array side by side
+    return d < a_width or d + b_width > a_pitch
+
+
 def _scale_tensor(g: Scale, n: int, device: torch.device, what: str) -> torch.Tensor:
     """g as n float32 values on the device."""
     if isinstance(g, torch.Tensor):
@@ -569,8 +579,10 @@ class FP4Linear:
                 raise ValueError(f"out must be {list(x.shape[:-1]) + [w.rows]}")
             y = out if out.dim() == 2 else out.view(-1, w.rows)
             _check_out(y, m, w, out_dtype)
-            if out.untyped_storage().data_ptr() == x2.untyped_storage().data_ptr():
-                x2, ld = x2.contiguous().clone(), w.cols  # y is written while other parts of the product still read x
+            if _overlap(m, x2.data_ptr(), ld * x2.element_size(), k * x2.element_size(),
+                        y.data_ptr(), _pitch(y) * y.element_size(), w.rows * y.element_size()):
+                # y is written while other parts of the product still read x
+                x2, ld = x2.clone(memory_format=torch.contiguous_format), k
         else:
             if out_dtype is not None and out_dtype not in _DT:
                 raise ValueError("the output is float16, bfloat16 or float32")

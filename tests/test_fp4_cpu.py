@@ -262,3 +262,26 @@ def test_linear_attributes():
     assert F._linear_ws("nvfp4", 256, 32, 3, True) == 0 and F._linear_ws("nvfp4", 256, 32, 3, False) == 256
     with pytest.raises(ValueError, match="rows in one product"):
         F._linear_ws("nvfp4", 256, 32, F.MAX_ROWS + 1, True)
+
+
+def test_overlap():
+    """Against the bytes themselves, where pitches differ at least never missed."""
+    r = torch.Generator().manual_seed(3)
+
+    def draw(lo, hi):
+        return int(torch.randint(lo, hi, (1,), generator=r))
+
+    def taken(a, pitch, width, rows):
+        return {a + i * pitch + j for i in range(rows) for j in range(width)}
+
+    seen = [0, 0]
+    for _ in range(3000):
+        rows, pa = draw(1, 5), draw(4, 20)
+        pb = pa if draw(0, 2) else draw(4, 20)
+        wa, wb = draw(1, min(pa, pb) + 1), draw(1, pb + 1)
+        a, b = draw(0, 60), draw(0, 60)
+        shares = bool(taken(a, pa, wa, rows) & taken(b, pb, wb, rows))
+        got = F._overlap(rows, a, pa, wa, b, pb, wb)
+        assert got == shares if pa == pb or rows == 1 else got >= shares
+        seen[got] += 1
+    assert min(seen) > 300

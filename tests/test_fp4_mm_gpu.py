@@ -385,6 +385,28 @@ def test_linear_in_place():
         assert lin(x, out=x) is x and torch.equal(x, want)
 
 
+@pytest.mark.parametrize("m", [3, 20])
+def test_linear_beside_its_input(m):
+    """An output next to the input in one array is no overlap; one that reaches into it is written from it as it was."""
+    F = fp4()
+    W = F.FP4Weight.quantize(torch.randn(640, 512, generator=gen(1), device="cuda") * 0.05)
+    lin = F.FP4Linear(W, 0.002)
+    for x_at, y_at, fresh in ((0, 512, False), (640, 0, False), (0, 500, True), (600, 0, True), (128, 128, True)):
+        arena = torch.randn(2 * m, 1152, generator=gen(2), device="cuda").bfloat16()
+        x, out = arena[:m, x_at:x_at + 512], arena[:m, y_at:y_at + 640]
+        want, rest = lin(x), arena.clone()
+        rest[:m, y_at:y_at + 640] = want
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        lin(x, out=out)
+        after = torch.cuda.memory_stats()["allocation.all.allocated"]
+        assert torch.equal(arena, rest), (x_at, y_at)
+        assert after - before == fresh + (m > 8)  # the copy of x, and the workspace
+        below = arena[m:, 64:64 + 640]  # rows behind x's
+        x.normal_(generator=gen(3))
+        want = lin(x)
+        assert torch.equal(lin(x, out=below), want)
+
+
 @pytest.mark.parametrize("m,n,k", [(3, 256, 2048), (40, 256, 2048), (500, 3000, 2048)])
 def test_a_wait_that_runs_out_is_reported(m, n, k):
     """With a limit of 1 ns the kernels' waits give up: the call ends, the status says so once, the next call is right."""
