@@ -266,6 +266,67 @@ def test_silu_mul_range(kind):
     assert s[0, 3 // b] == nan and s[1, 6 // b] == nan and s[2, 5 // b] == nan
 
 
+# Several rows a warp from rows * ceil(cols / 512) >= 18944 on: as many rows as leave the last CTA a few, for rows on
+# 32-byte and on 16-byte boundaries (columns or padding), and on any other (one row a warp, many CTAs).
+MANY = [(6401, 1408), (6403, 1392), (18977, 500), (6405, 1399)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", MANY)
+def test_many_rows(kind, dtype, rows, cols):
+    """Bit for bit, the quantiser and the way back, at the boundaries of x's rows that the kernels tell apart."""
+    F = fp4()
+    per16 = 16 // dtype.itemsize
+    for pad, lo in ((-cols % (2 * per16), 0), (-cols % (2 * per16) + per16, per16), (0, 0)):
+        big = rand(rows, cols + pad + lo, dtype, rows)
+        x = big[:, lo:lo + cols]
+        finite = torch.where(torch.isfinite(x), x, torch.zeros_like(x))  # (some float16 values are past its end)
+        g = g_of(kind, finite, pow2=lo > 0)
+        gr = 1.0 if g is None else g
+        q = F.quantize_fp4(x, kind, global_scale=g)
+        ref = R.quantize(x, kind, gr)
+        assert_same_codes(q, ref, f"pad {pad}")
+        v = R.values(*ref, kind, cols, gr).float().to(dtype)
+        assert torch.allclose(F.dequantize_fp4(q, dtype), v, rtol=0, atol=0, equal_nan=True)
+        assert int(v.isnan().sum()) <= 10 * R.BLOCK[kind]
+        if kind == "nvfp4":
+            assert torch.equal(F.fp4_global_scale(x), (finite.double().abs().max() / 2688).float().reshape(1))
+        idx = torch.randint(-3, rows + 3, (rows,), generator=gen(cols), device="cuda", dtype=torch.int32)
+        inside = (idx >= 0) & (idx < rows)
+        want = torch.where(inside[:, None], x[idx.clamp(0, rows - 1).long()], torch.zeros((), dtype=dtype, device="cuda"))
+        assert_same_codes(F.quantize_fp4(x, kind, global_scale=g, row_index=idx), R.quantize(want, kind, gr), "gathered")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", MANY)
+def test_silu_mul_many_rows(kind, dtype, rows, cols):
+    """The same of the SiLU form, with gates that only the float64 redo holds in the last rows and here and there."""
+    F = fp4()
+    per16 = 16 // dtype.itemsize
+    r = gen(rows)
+    for pad, lo in ((-2 * cols % (2 * per16), 0), (-2 * cols % (2 * per16) + per16, per16)):
+        big = (torch.randn(rows, 2 * cols + pad + lo, generator=r, device="cuda") * 2).to(dtype)
+        gu = big[:, lo:lo + 2 * cols]
+        far = torch.rand(rows, cols, generator=r, device="cuda") < 0.002
+        far[-20:] |= torch.rand(20, cols, generator=r, device="cuda") < 0.3
+        far[-1] = True
+        gate, up = gu[:, :cols], gu[:, cols:]
+        gate.copy_(torch.where(far, -60 - 40 * torch.rand(rows, cols, generator=r, device="cuda"), gate.float()))
+        up.copy_(torch.where(far, up.float() * 3e3, up.float()))
+        h = R.silu_mul(gu)
+        g = g_of(kind, h, pow2=lo > 0)
+        gr = 1.0 if g is None else g
+        q = F.silu_mul_quantize_fp4(gu, kind, global_scale=g)
+        assert_same_codes(q, R.quantize(h, kind, gr), f"pad {pad}")
+        assert torch.equal(F.dequantize_fp4(q), F.dequantize_fp4(F.silu_mul_quantize_fp4(gu.contiguous(), kind, global_scale=g)))
+        if kind == "nvfp4":
+            assert torch.equal(F.fp4_global_scale(gu, silu_mul=True), (h.abs().max().float().double() / 2688).float().reshape(1))
+            tiny = torch.tensor([2.0 ** -100], device="cuda")  # the far gates' products are the ones that have digits
+            assert_same_codes(F.silu_mul_quantize_fp4(gu[-40:], kind, global_scale=tiny), R.quantize(h[-40:], kind, tiny))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_silu_mul_smallest_gates(kind, dtype):
