@@ -232,7 +232,7 @@ __device__ __forceinline__ uint2 encode16(const float (&v)[16], float g, bool& u
     r = __uint_as_float((254u - sbyte) << 23);
     if (kSilu) {  // near a power of two, or where float32 has lost digits
       unsure |= (__float_as_uint(a * (1.0f + kSiluWin)) >> 23) != (__float_as_uint(a * (1.0f - kSiluWin)) >> 23);
-      unsure |= a < 0x1p-100f && top != 0;
+      unsure |= top - 1u < 0x0D800000u - 1u;  // 0 < a < 2^-100
     }
   } else {
     const float t = a * __frcp_rn(6.0f * g);
