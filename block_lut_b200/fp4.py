@@ -193,14 +193,14 @@ class FP4Matrix(_Operand):
     def _ptrs(self) -> tuple[int, int]:
         """Addresses of the codes and the scales, which the kernels are about to write."""
         p = self.data.data_ptr()
-        return p, p + self._codes_bytes()
+        return p, p + self.rows * 64 * ((self.cols + 127) // 128)
 
     def _operand(self) -> tuple[int, int, int]:
         """Addresses of the codes, the scales and the global scale (0: none), which they are about to read."""
         if not self._ok:
             self._look_over(self.data, _data_bytes(self.kind, self.rows, self.cols), 1, "FP4Matrix.data")
         p, g = self.data.data_ptr(), self.global_scale
-        return p, p + self._codes_bytes(), 0 if g is None else g.data_ptr()
+        return p, p + self.rows * 64 * ((self.cols + 127) // 128), 0 if g is None else g.data_ptr()
 
     @classmethod
     def from_checkpoint(cls, kind: str, codes: torch.Tensor, scales: torch.Tensor, cols: int,
@@ -336,13 +336,14 @@ def silu_mul_quantize_fp4(gate_up: torch.Tensor, kind: str = "nvfp4", global_sca
 @_lib.stream_ordered
 def dequantize_fp4(q: FP4Matrix, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """The values q stands for, [rows, cols] in ``dtype`` (float32 products, rounded once to 16 bits)."""
-    if dtype not in _DT:
+    dt = _DT.get(dtype)
+    if dt is None:
         raise ValueError(f"dtype must be float16, bfloat16 or float32, not {dtype}")
     out = q.data.new_empty((q.rows, q.cols), dtype=dtype)
     if q.rows == 0:
         return out
-    d = _desc(q.kind, q.rows, q.cols)
-    _launch("blut_fp4_dequantize", out, stream, C.byref(d), *q._operand(), out.data_ptr(), _DT[dtype], q.cols)
+    codes, scales, g = q._operand()
+    _launch("blut_fp4_dequantize", out, stream, C.byref(_desc(q.kind, q.rows, q.cols)), codes, scales, g, out.data_ptr(), dt, q.cols)
     return out
 
 
