@@ -374,6 +374,59 @@ def test_linear_follows_its_attributes():
         lin.act_scale = -1.0
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens", [1, 50])
+def test_routed_layer_in_a_graph(kind, tokens):
+    """From the router to the weighted sum without a word from the host: captured, and replayed on other tokens."""
+    from block_lut_b200 import router
+    F = fp4()
+    k, E, H, I = 3, 12, 256, 136
+    r = gen(4)
+    w_router = torch.randn(E, H, generator=r, device="cuda").bfloat16()
+    W13 = F.FP4Weight.quantize(torch.randn(E, 2 * I, H, generator=r, device="cuda") * 0.08, kind)
+    W2 = F.FP4Weight.quantize(torch.randn(E, H, I, generator=r, device="cuda") * 0.08, kind)
+    every = torch.arange(E + 1, dtype=torch.int32, device="cuda")
+
+    def layer(x):
+        ids, weights, _ = router(x, w_router, k)
+        expert_of_row, order = ids.flatten().sort(stable=True)
+        offsets = torch.searchsorted(expert_of_row, every, out_int32=True)
+        xq = F.quantize_fp4(x, kind, row_index=(order // k).int())
+        h = F.silu_mul_quantize_fp4(F.fp4_grouped_matmul(xq, W13, offsets), kind)
+        y = F.fp4_grouped_matmul(h, W2, offsets)
+        rows = torch.empty_like(y).index_copy_(0, order, y)
+        return (rows.view(len(x), k, -1) * weights[..., None]).sum(1), ids, weights, xq.global_scale
+
+    x = torch.randn(tokens, H, generator=r, device="cuda").bfloat16()
+    for _ in range(2):
+        layer(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer(x)
+    for seed in range(3):
+        x.copy_(torch.randn(tokens, H, generator=gen(seed), device="cuda"))
+        graph.replay()
+        want = layer(x)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        out, ids, weights, g = want
+        xq = F.quantize_fp4(x, kind, global_scale=g)
+        per = []  # every expert on every row, without sorting: rows and matrix scales are the same
+        for e in range(E):
+            off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+            off[e + 1:] = tokens
+            per.append(F.fp4_grouped_matmul(xq, W13, off))
+        gu = torch.stack(per)[ids.long(), torch.arange(tokens, device="cuda")[:, None]]  # [tokens, k, 2 I]
+        h = F.silu_mul_quantize_fp4(gu.view(tokens * k, -1), kind)
+        per = []
+        for e in range(E):
+            off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+            off[e + 1:] = tokens * k
+            per.append(F.fp4_grouped_matmul(h, W2, off).view(tokens, k, H))
+        y = torch.stack(per).gather(0, ids.long()[None, :, :, None].expand(1, -1, -1, H))[0]
+        assert torch.equal(out, (y * weights[..., None]).sum(1))  # a row's product does not depend on its run
+
+
 def test_linear_in_place():
     """An output that overlaps the input is written from the input as it was."""
     F = fp4()
