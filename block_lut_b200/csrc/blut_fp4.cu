@@ -518,7 +518,10 @@ inline int64_t elem_size(int dtype) { return dtype == BLUT_F32 ? 4 : 2; }
 inline int launched() { return cudaGetLastError() == cudaSuccess ? BLUT_OK : BLUT_ERR_LAUNCH; }
 
 // Rows a warp takes: several once that still leaves every SM a few CTAs, one
-// below (32 rows x 2048: 1.7 us with one; 32768 x 2048: 44 us with one).
+// below.  nvfp4 of bf16 rows x 2048, one against several: 32 rows 1.7 against
+// 3.1 us, 4096 (below the border) 7.8 against 8.2, 8192 (above) 13.4 against
+// 12.4, 32768 45.0 against 36.1; the way back 1.9 against 2.5, 7.2 against 5.8,
+// 13.1 against 8.2, 45.0 against 30.5.
 inline bool many_rows(int64_t rows, int kp) {
   return rows * ((kp + kQCols - 1) / kQCols) >= 148ll * 4 * 4 * kQWarps;
 }
@@ -539,9 +542,13 @@ int launch_quantize(const blut_fp4_desc& d, const void* x, int64_t ld, const int
   const int vec = alignment(x, ld * es, kSilu ? d.cols * es : 0);
   const int kp = fp4_kblocks(d.cols) * kFp4BlockCols;
   // Four CTAs per SM, and the rows that their 64 registers hold: nvfp4 of
-  // 32768 x 2048 bf16 takes 38.1 us with 4 rows (3 CTAs: 40.1, 2 rows: 41.5,
-  // one: 42.2), mxfp4 30.8 (33.3, 34.1, 36.7); the SiLU form of 196608 x 1408
-  // 237 us with 2 rows (3 CTAs: 273, one row: 239, 4 rows: 308).
+  // 32768 x 2048 bf16 takes 36.1 us with 4 rows (3 CTAs: 37.9, 2 rows: 39.9,
+  // one: 44.9), mxfp4 31.2 (33.4, 33.7, 36.5); float32 52.6 with 2 (3 CTAs:
+  // 55.9, one row: 54.5, 4 rows: 84.5); the SiLU form of 196608 x 1408, mxfp4
+  // fp16, 238 with 2 (3 CTAs: 265, one row: 280, 4 rows: 293).  Rows on other
+  // than 16-byte boundaries take one row a warp whatever their number: 20000 x
+  // 2319 bf16 42.5 us (nvfp4) and 38.8 (mxfp4) against 41.3 and 37.9 with 4,
+  // too little for another set of kernels.
   constexpr int kMany = kSilu || DT == BLUT_F32 ? 2 : 4;
   const bool many = many_rows(d.rows, kp);
 #define BLUT_Q(MX, VEC, PER) \

@@ -852,10 +852,10 @@ int launch(Fp4Params& p, int64_t items, bool early, cudaStream_t stream) {
 }
 
 // Tokens of an item for one matrix and more than 128 tokens: as few tiles as
-// 192 allow, cut evenly.  Against tiles of 192: 256 x 11264 x 2048 10.8 ->
-// 10.3 us, 300 x 2816 x 2048 10.3 -> 9.8.  More and smaller tiles that fill
-// the last round of CTAs better do not pay (1999 x 5000 x 1400: 15.3 us with
-// 192, 16.1 with 144).
+// 192 allow, cut evenly.  Against tiles of 192: 256 x 11264 x 2048 11.5 ->
+// 11.2 us, 300 x 2816 x 2048 10.5 either way.  More and smaller tiles that
+// fill the last round of CTAs better gain next to nothing (1999 x 5000 x 1400:
+// 16.6 us with 192, 16.4 with 176, 160 and 144, 18.7 with 128).
 int tokens_per_item(int64_t m) {
   const int64_t tiles = (m + 191) / 192;
   return (int)(((m + tiles - 1) / tiles + 15) / 16 * 16);
@@ -864,7 +864,20 @@ int tokens_per_item(int64_t m) {
 template <bool kMX>
 int dispatch(Fp4Params& p, int64_t m, int fuse, bool early, cudaStream_t stream) {
   p.row_tiles = (p.n + 127) / 128;
-  // tokens per matrix: their number for one matrix, the mean for runs
+  // Tokens per matrix: their number for one matrix, the mean for runs (their
+  // lengths are on the device).  In us with items of 32, 64, 128, 192 tokens:
+  //   one matrix 11264 x 2048,  32 tokens   9.6   9.5
+  //                             64          9.7  11.0   9.7  10.3
+  //                            128         10.3  11.0  11.4  11.1
+  //                            256         14.7  11.2  10.7  11.2
+  //   64 of 2816 x 2048, mean   12         39.1  39.7  37.9  41.4
+  //                             48         47.5  45.5  42.8  45.2
+  //                             96         69.5  55.1  48.4  54.5
+  //                            192          121  80.6  69.5  64.5
+  // The mean cannot see a few runs with most of the rows, nor rows behind the
+  // last run: 22 runs of 3072 rows, the longest 509, take 31.6 (64) against
+  // 25.9 (128), one run of 2048 25.6 (32) against 13.7 (192), and 128 rows of
+  // 45 runs in a buffer of 7808 33.3 (192) against 30.6 (32).
   const int64_t mean = p.experts ? (m + p.experts - 1) / p.experts : m;
   const int nt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 192;
   p.tn = nt == 192 && !p.experts ? tokens_per_item(m) : nt;

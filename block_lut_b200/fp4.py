@@ -164,7 +164,7 @@ class _Operand:
 @dataclass
 class FP4Matrix(_Operand):
     """Rows in 4-bit form, as the quantisers write them (the FP4 layout of ``include/blut.h``): the codes, then the
-    scales, in one buffer.  ``global_scale`` float32 [1] (nvfp4) or None."""
+    scales, in one buffer.  ``global_scale`` float32 [1] (nvfp4; kept as given, not copied) or None (1)."""
     kind: str
     rows: int
     cols: int
