@@ -141,7 +141,7 @@ class _Operand:
     _ok = False
 
     def __setattr__(self, name, value):
-        self.__dict__[name] = value
+        object.__setattr__(self, name, value)
         self.__dict__["_ok"] = False
 
     def __getstate__(self):  # a copy, or one loaded from a file onto another device, is looked over again

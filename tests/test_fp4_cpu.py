@@ -234,6 +234,8 @@ def test_operands_are_checked_where_they_are_read(kind):
         assert (again.kind, again.rows, again.cols) == (kind, 4, 130) and torch.equal(again.data, m.data)
         with pytest.raises(ValueError, match="CUDA"):
             again._operand()
+    with pytest.raises(AttributeError):
+        m.codes = m.data
     m.rows = 5
     with pytest.raises(ValueError, match="bytes"):
         m._operand()
