@@ -36,7 +36,9 @@ MIN_GLOBAL_SCALE, MAX_GLOBAL_SCALE = 2.0 ** -100, 2.0 ** 100
 MAX_EXPERTS = 1024
 MAX_ROWS = 1 << 22  # rows of one product
 
-_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# looked up once; a torch without CUDA, which has neither, can still import the package
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 Scale = Union[None, float, torch.Tensor]
 
