@@ -875,8 +875,8 @@ int dispatch(Fp4Params& p, int64_t m, int fuse, bool early, cudaStream_t stream)
   //                             96         69.5  55.1  48.4  54.5
   //                            192          121  80.6  69.5  64.5
   // The mean cannot see a few runs with most of the rows, nor rows behind the
-  // last run: 22 runs of 3072 rows, the longest 509, take 31.6 (64) against
-  // 25.9 (128), one run of 2048 25.6 (32) against 13.7 (192), and 128 rows of
+  // last run: 22 runs of 512 tokens' six rows each, the longest 509, take 31.6
+  // (64) against 25.9 (128), one run of 2048 25.6 (32) against 13.7 (192), and 128 rows of
   // 45 runs in a buffer of 7808 33.3 (192) against 30.6 (32).
   const int64_t mean = p.experts ? (m + p.experts - 1) / p.experts : m;
   const int nt = mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : 192;
